@@ -467,6 +467,34 @@ SKL_FUNC void skl_cvt_f8e4m3_bf16_sm100a(skl_bf16_t *pDst, const uint8_t *pSrc, 
 SKL_FUNC void skl_cvt_f8e5m2_bf16_sm100a(skl_bf16_t *pDst, const uint8_t *pSrc, size_t n);
 SKL_FUNC void skl_cvt_f4e2m1_f8e4m3_sm100a(uint8_t *pDst, const uint8_t *pSrc, size_t n);
 
+/* ------------------------------------------------------------------ cvt, OCP MX-FP4 (no SKL counterpart)
+ * To and from the operand format of skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a above.  A packed row of k elements is
+ * B = ceil(k / 32) blocks: 16 B bytes of E2M1 codes (low nibble first) and B scale bytes, the last block filled up with
+ * zeros -- so a matrix of any k can be multiplied with k rounded up to a multiple of 32.
+ *
+ * skl_cvt_<t>rc_mxf4e2m1: element (i, kk) of the source at pSrc + i*rs + kk*cs (elements), rows packed along kk at
+ * pDst + i*rsd and pScale + i*rss (bytes; rsd >= 16 B, rss >= B).  With (rs, cs) = (1, ld) the columns of a row-major
+ * matrix become packed rows.  For a block with largest magnitude A:
+ *     s    = floor(log2 A) - 2 + 127, at least 0     (0 for a block of zeros)
+ *     code = round to nearest even (x / 2^(s - 127)), magnitudes above 6 become 6, the sign of a zero is kept
+ * which is the format's own rule (OCP Microscaling Formats v1.0, section 6.3).  A block that holds an infinity or a NaN gets
+ * s = 255 (NaN) and zero codes.
+ * skl_cvt_mxf4e2m1_<t>: the way back to a row-major matrix (row stride rsd >= k elements): value(code) * 2^(s - 127),
+ * exact wherever <t> holds it, else rounded once to nearest even; s = 255 gives NaN.
+ * Source and destination must not overlap; m or k = 0 is a no-op; m and k are below 2^31. */
+SKL_FUNC void skl_cvt_f32rc_mxf4e2m1_sm100a(uint8_t *pDst, size_t rsd, uint8_t *pScale, size_t rss, const float *pSrc,
+                                            size_t rs, size_t cs, size_t m, size_t k);
+SKL_FUNC void skl_cvt_bf16rc_mxf4e2m1_sm100a(uint8_t *pDst, size_t rsd, uint8_t *pScale, size_t rss, const skl_bf16_t *pSrc,
+                                             size_t rs, size_t cs, size_t m, size_t k);
+SKL_FUNC void skl_cvt_f16rc_mxf4e2m1_sm100a(uint8_t *pDst, size_t rsd, uint8_t *pScale, size_t rss, const skl_f16_t *pSrc,
+                                            size_t rs, size_t cs, size_t m, size_t k);
+SKL_FUNC void skl_cvt_mxf4e2m1_f32_sm100a(float *pDst, size_t rsd, const uint8_t *pSrc, size_t rsa, const uint8_t *pScale,
+                                          size_t rss, size_t m, size_t k);
+SKL_FUNC void skl_cvt_mxf4e2m1_bf16_sm100a(skl_bf16_t *pDst, size_t rsd, const uint8_t *pSrc, size_t rsa,
+                                           const uint8_t *pScale, size_t rss, size_t m, size_t k);
+SKL_FUNC void skl_cvt_mxf4e2m1_f16_sm100a(skl_f16_t *pDst, size_t rsd, const uint8_t *pSrc, size_t rsa,
+                                          const uint8_t *pScale, size_t rss, size_t m, size_t k);
+
 /* ------------------------------------------------------------------ pack / unpack / transpose
  * Parameter lists of src/pack/pack_e8_zve32x.h:49-113 (ref/pack/pack_e8rc_e8rcprc.h,
  * unpack_e8rcprc_e8rc.h, transpose_e8.h) and the e16 / e32 siblings. */

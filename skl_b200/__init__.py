@@ -34,6 +34,9 @@ _GEMM_P_F = [_SZ] * 6 + [_F, _VP] + [_SZ] * 4 + [_VP] + [_SZ] * 4 + [_F, _VP] + 
 _GEMM_TE_I = [_SZ, _SZ, _SZ, _I32, _VP, _SZ, _SZ, _VP, _SZ, _SZ, _I32, _VP, _SZ, _SZ, _SZ, _SZ]
 _GEMM_TE_F = [_SZ, _SZ, _SZ, _F, _VP, _SZ, _SZ, _VP, _SZ, _SZ, _F, _VP, _SZ, _SZ, _SZ, _SZ]
 
+_CVT_TO_MX = [_VP, _SZ, _VP, _SZ, _VP, _SZ, _SZ, _SZ, _SZ]
+_CVT_FROM_MX = [_VP, _SZ, _VP, _SZ, _VP, _SZ, _SZ, _SZ]
+
 # every symbol include/skl-b200.h declares -> ctypes argument list (restype None unless noted)
 SIGNATURES = {
     "skl_b200_last_status": ([], _I),
@@ -111,6 +114,12 @@ SIGNATURES = {
     "skl_cvt_f8e4m3_bf16_sm100a": ([_VP, _VP, _SZ], None),
     "skl_cvt_f8e5m2_bf16_sm100a": ([_VP, _VP, _SZ], None),
     "skl_cvt_f4e2m1_f8e4m3_sm100a": ([_VP, _VP, _SZ], None),
+    "skl_cvt_f32rc_mxf4e2m1_sm100a": (_CVT_TO_MX, None),
+    "skl_cvt_bf16rc_mxf4e2m1_sm100a": (_CVT_TO_MX, None),
+    "skl_cvt_f16rc_mxf4e2m1_sm100a": (_CVT_TO_MX, None),
+    "skl_cvt_mxf4e2m1_f32_sm100a": (_CVT_FROM_MX, None),
+    "skl_cvt_mxf4e2m1_bf16_sm100a": (_CVT_FROM_MX, None),
+    "skl_cvt_mxf4e2m1_f16_sm100a": (_CVT_FROM_MX, None),
     "skl_pack_e8rc_e8rcprc_sm100a": ([_SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, C.c_uint8],
                                      None),
     "skl_pack_e16rc_e16rcprc_sm100a": ([_SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ,

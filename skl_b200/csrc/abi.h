@@ -131,6 +131,13 @@ int skl_b200_launch_cvt_f8_to_bf16_2d_transposed(void *dst, size_t ld_dst, const
 int skl_b200_launch_cvt_selfcheck(int dst_fmt, int saturate, uint64_t first, uint64_t count,
                                   unsigned long long *mismatches, void *stream);
 
+/* MX-FP4 quantisation of an m x k matrix (src_type F32 / BF16 / F16, element strides rs, cs) and the way back (row-major
+ * dst); rsd / rsa: bytes between packed rows, rss: scale bytes between rows.  m, k >= 1. */
+int skl_b200_launch_quant_mxf4(void *dst, int64_t rsd, void *scales, int64_t rss, const void *src, int src_type, int64_t rs,
+                               int64_t cs, uint32_t m, uint32_t k, void *stream);
+int skl_b200_launch_widen_mxf4(void *dst, int dst_type, int64_t rsd, const void *src, int64_t rsa, const void *scales,
+                               int64_t rss, uint32_t m, uint32_t k, void *stream);
+
 /* pack / unpack / transpose; esize in {1, 2, 4}. */
 int skl_b200_launch_pack(size_t esize, size_t m, size_t n, const void *src, size_t rs, size_t cs,
                          size_t m0, size_t n0, void *dst, size_t rs0, size_t cs0, size_t rs1,

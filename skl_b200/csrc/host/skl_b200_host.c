@@ -1188,6 +1188,94 @@ void skl_cvt_f4e2m1_f8e4m3_sm100a(uint8_t *pDst, const uint8_t *pSrc, size_t n) 
   run_cvt_widen(pDst, pSrc, 1, 0, n);
 }
 
+/* ------------------------------------------------------------------ cvt, MX-FP4 */
+
+static int rows_back(void *host, const void *dev, size_t pitch, size_t width, size_t rows) {
+  if (rows == 1) pitch = width;
+  return cuda_ok(cudaMemcpy2DAsync(host, pitch, dev, pitch, width, rows, cudaMemcpyDeviceToHost, (cudaStream_t)g_ctx.stream));
+}
+
+/* A call refused before anything of it ran (no device needed to say so). */
+static void refuse(skl_b200_status_t s) {
+  g_ctx.status = s;
+  g_ctx.cuda_err[0] = 0;
+  g_ctx.last_launches = 0;
+}
+
+static void run_cvt_to_mxf4_body(uint8_t *dst, size_t rsd, uint8_t *scales, size_t rss, const void *src, int type, size_t rs,
+                                 size_t cs, size_t m, size_t k) {
+  if (m == 0 || k == 0) return;
+  const size_t kb = (k + 31) / 32;
+  int host_any = 0;
+  const void *dsrc = src;
+  uint8_t *ddst = dst, *dsc = scales;
+  if (!on_device(src)) {
+    host_any = 1;
+    dsrc = stage_in(WS_A, src, span4(m, k, 1, 1, (int64_t)rs, (int64_t)cs, 0, 0) * dt_size(type));
+    if (!dsrc) return;
+  }
+  const int dst_host = !on_device(dst), sc_host = !on_device(scales);
+  if (dst_host && !(ddst = (uint8_t *)workspace(WS_C, (m - 1) * rsd + 16 * kb))) return;
+  if (sc_host && !(dsc = (uint8_t *)workspace(WS_ROW, (m - 1) * rss + kb))) return;
+  if (!cuda_ok((cudaError_t)skl_b200_launch_quant_mxf4(ddst, (int64_t)rsd, dsc, (int64_t)rss, dsrc, type, (int64_t)rs,
+                                                       (int64_t)cs, (uint32_t)m, (uint32_t)k, g_ctx.stream)))
+    return;
+  if (dst_host && !rows_back(dst, ddst, rsd, 16 * kb, m)) return;
+  if (sc_host && !rows_back(scales, dsc, rss, kb, m)) return;
+  finish(host_any || dst_host || sc_host);
+}
+
+static void run_cvt_from_mxf4_body(void *dst, int type, size_t rsd, const uint8_t *src, size_t rsa, const uint8_t *scales,
+                                   size_t rss, size_t m, size_t k) {
+  if (m == 0 || k == 0) return;
+  const size_t kb = (k + 31) / 32, es = dt_size(type);
+  int host_any = 0;
+  const void *dsrc = src, *dsc = scales;
+  void *ddst = dst;
+  if (!on_device(src)) {
+    host_any = 1;
+    if (!(dsrc = stage_in(WS_A, src, (m - 1) * rsa + 16 * kb))) return;
+  }
+  if (!on_device(scales)) {
+    host_any = 1;
+    if (!(dsc = stage_in(WS_ROW, scales, (m - 1) * rss + kb))) return;
+  }
+  const int dst_host = !on_device(dst);
+  if (dst_host && !(ddst = workspace(WS_C, ((m - 1) * rsd + k) * es))) return;
+  if (!cuda_ok((cudaError_t)skl_b200_launch_widen_mxf4(ddst, type, (int64_t)rsd, dsrc, (int64_t)rsa, dsc, (int64_t)rss,
+                                                       (uint32_t)m, (uint32_t)k, g_ctx.stream)))
+    return;
+  if (dst_host && !rows_back(dst, ddst, rsd * es, k * es, m)) return;
+  finish(host_any || dst_host);
+}
+
+/* the packed side of an m x k matrix: both pointers, strides that hold a row, sizes the kernels index with 32 bits */
+static int mxf4_rows_ok(const void *codes, size_t rs, const void *scales, size_t rss, size_t m, size_t k) {
+  if (m == 0 || k == 0) return 1;
+  if (m >= (1ull << 31) || k >= (1ull << 31) || !codes || !scales) return 0;
+  const size_t kb = (k + 31) / 32;
+  return rs >= 16 * kb && rss >= kb;
+}
+
+#define SKL_B200_DEF_CVT_MXF4(SUF, TYPE, DT)                                                                              \
+  void skl_cvt_##SUF##rc_mxf4e2m1_sm100a(uint8_t *pDst, size_t rsd, uint8_t *pScale, size_t rss, const TYPE *pSrc,        \
+                                         size_t rs, size_t cs, size_t m, size_t k) {                                      \
+    if (!mxf4_rows_ok(pDst, rsd, pScale, rss, m, k) || (m && k && !pSrc)) { refuse(SKL_B200_ERR_INVALID_ARGUMENT); return; } \
+    if (!begin_call()) return;                                                                                            \
+    run_cvt_to_mxf4_body(pDst, rsd, pScale, rss, pSrc, DT, rs, cs, m, k);                                                 \
+    leave_call();                                                                                                         \
+  }                                                                                                                       \
+  void skl_cvt_mxf4e2m1_##SUF##_sm100a(TYPE *pDst, size_t rsd, const uint8_t *pSrc, size_t rsa, const uint8_t *pScale,    \
+                                       size_t rss, size_t m, size_t k) {                                                  \
+    if (!mxf4_rows_ok(pSrc, rsa, pScale, rss, m, k) || (m && k && (!pDst || rsd < k))) { refuse(SKL_B200_ERR_INVALID_ARGUMENT); return; } \
+    if (!begin_call()) return;                                                                                            \
+    run_cvt_from_mxf4_body(pDst, DT, rsd, pSrc, rsa, pScale, rss, m, k);                                                  \
+    leave_call();                                                                                                         \
+  }
+SKL_B200_DEF_CVT_MXF4(f32, float, SKL_DT_F32)
+SKL_B200_DEF_CVT_MXF4(bf16, skl_bf16_t, SKL_DT_BF16)
+SKL_B200_DEF_CVT_MXF4(f16, skl_f16_t, SKL_DT_F16)
+
 /* ------------------------------------------------------------------ MX-FP4 GEMM (block-scaled E2M1) */
 
 /* Device operands with TMA-compatible packed rows run on the block-scaled tensor-core kernel; otherwise both operands

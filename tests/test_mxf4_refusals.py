@@ -1,0 +1,24 @@
+"""What the MX-FP4 entry points refuse, before any device is touched (runs without a GPU)."""
+import numpy as np
+import pytest
+
+import skl_b200 as S
+
+INVALID, UNSUPPORTED = 1, 5
+B = S.ptr(np.zeros(4096, np.uint8))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_cvt_refusals(skl, t):
+    to, back = getattr(skl, f"skl_cvt_{t}rc_mxf4e2m1_sm100a"), getattr(skl, f"skl_cvt_mxf4e2m1_{t}_sm100a")
+    good_to, good_back = [B, 32, B, 2, B, 33, 1, 2, 33], [B, 33, B, 32, B, 2, 2, 33]
+    for at, bad in [(0, 0), (2, 0), (4, 0), (1, 31), (3, 1), (7, 1 << 31), (8, 1 << 31)]:
+        args = list(good_to)
+        args[at] = bad
+        to(*args)
+        assert skl.skl_b200_last_status() == INVALID, (at, bad)
+    for at, bad in [(0, 0), (2, 0), (4, 0), (1, 32), (3, 31), (5, 1), (6, 1 << 31), (7, 1 << 31)]:
+        args = list(good_back)
+        args[at] = bad
+        back(*args)
+        assert skl.skl_b200_last_status() == INVALID, (at, bad)
