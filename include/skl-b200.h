@@ -283,6 +283,47 @@ SKL_FUNC void skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k
                                                     size_t csb, const uint8_t *sb, size_t cssb, float beta, float *c,
                                                     size_t rsc);
 
+/* ------------------------------------------------------------------ GEMM, 16-bit activations x MX-FP4 weights (no SKL counterpart)
+ * skl_gemm_<ta>_mxf4e2m1_<tc>:   C[i, j] = beta * C[i, j] + alpha * sum_kk A[i, kk] * W[j, kk]     (m x n, k deep)
+ *     W one output column per packed row, as B of the entry above (column j starts at b + j*csb, its scales at sb + j*cssb):
+ *     a layer's forward product, from one token to a whole prompt.
+ * skl_gemm_<ta>_mxf4e2m1r_<tc>:  C[i, j] = beta * C[i, j] + alpha * sum_kk A[i, kk] * W[kk, j]
+ *     W row-major, packed along n (row kk starts at b + kk*rsb, its scales at sb + kk*rssb): with A the gradient of the
+ *     layer's output and the same packed matrix this is the gradient of its input.
+ * A (bf16 or fp16) and C are row-major with row strides rsa >= k and rsc >= n elements.  Packed rows are as
+ * skl_cvt_<t>rc_mxf4e2m1 writes them: any length, ceil(length / 32) blocks; codes behind the length are ignored (a scale
+ * of 255 makes every product with its block NaN, in a row's last block too).  Products are exact, sums are fp32; bf16 / fp16
+ * C is rounded once.  beta == 0 does not read C; k == 0 gives beta * C.
+ * A row of A that holds an infinity or a NaN gives results that are not finite where the sum is not; the results of other
+ * rows do not depend on it.
+ * Few rows run on a kernel that streams the packed weights once; more rows widen W exactly to bf16 in device memory taken
+ * from the stream (cudaMallocAsync: captured calls own theirs, so graphs may run side by side) and run on the bf16
+ * tensor-core kernel; fp16 activations then enter as the exact sum of two bf16 matrices. */
+SKL_FUNC void skl_gemm_bf16_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                                const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,
+                                                float *c, size_t rsc);
+SKL_FUNC void skl_gemm_bf16_mxf4e2m1_bf16_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                                 const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,
+                                                 skl_bf16_t *c, size_t rsc);
+SKL_FUNC void skl_gemm_f16_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                               const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,
+                                               float *c, size_t rsc);
+SKL_FUNC void skl_gemm_f16_mxf4e2m1_f16_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                               const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,
+                                               skl_f16_t *c, size_t rsc);
+SKL_FUNC void skl_gemm_bf16_mxf4e2m1r_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                                 const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,
+                                                 float *c, size_t rsc);
+SKL_FUNC void skl_gemm_bf16_mxf4e2m1r_bf16_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                                  const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,
+                                                  skl_bf16_t *c, size_t rsc);
+SKL_FUNC void skl_gemm_f16_mxf4e2m1r_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                                const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,
+                                                float *c, size_t rsc);
+SKL_FUNC void skl_gemm_f16_mxf4e2m1r_f16_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                                const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,
+                                                skl_f16_t *c, size_t rsc);
+
 /* ------------------------------------------------------------------ GEMM, int8 with 4-deep k blocks
  * Same parameter list as skl_gemm_i8rcp1x4_i8p4x1c_i32_xsfvqdotq
  * (src/gemm/gemm_i8rcp1x4_i8p4x1c_i32_xsfvqdotq.h:70-75): A in 1 x 4 blocks (element (i, k) at

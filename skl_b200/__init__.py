@@ -34,6 +34,7 @@ _GEMM_P_F = [_SZ] * 6 + [_F, _VP] + [_SZ] * 4 + [_VP] + [_SZ] * 4 + [_F, _VP] + 
 _GEMM_TE_I = [_SZ, _SZ, _SZ, _I32, _VP, _SZ, _SZ, _VP, _SZ, _SZ, _I32, _VP, _SZ, _SZ, _SZ, _SZ]
 _GEMM_TE_F = [_SZ, _SZ, _SZ, _F, _VP, _SZ, _SZ, _VP, _SZ, _SZ, _F, _VP, _SZ, _SZ, _SZ, _SZ]
 
+_GEMM_MXW = [_SZ, _SZ, _SZ, _F, _VP, _SZ, _VP, _SZ, _VP, _SZ, _F, _VP, _SZ]
 _CVT_TO_MX = [_VP, _SZ, _VP, _SZ, _VP, _SZ, _SZ, _SZ, _SZ]
 _CVT_FROM_MX = [_VP, _SZ, _VP, _SZ, _VP, _SZ, _SZ, _SZ]
 
@@ -72,6 +73,14 @@ SIGNATURES = {
     "skl_gemm_f8e5m2c_f8e5m2_f32_sm100a": (_GEMM_R_F, None),
     "skl_b200_te": ([], _SZ),
     "skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a": ([_SZ, _SZ, _SZ, _F, _VP, _SZ, _VP, _SZ, _VP, _SZ, _VP, _SZ, _F, _VP, _SZ], None),
+    "skl_gemm_bf16_mxf4e2m1_f32_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_bf16_mxf4e2m1_bf16_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_f16_mxf4e2m1_f32_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_f16_mxf4e2m1_f16_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_bf16_mxf4e2m1r_f32_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_bf16_mxf4e2m1r_bf16_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_f16_mxf4e2m1r_f32_sm100a": (_GEMM_MXW, None),
+    "skl_gemm_f16_mxf4e2m1r_f16_sm100a": (_GEMM_MXW, None),
     "skl_gemm_i8rcptex1c_i8rcp1xte_i32rcptexterc_sm100a": (_GEMM_TE_I, None),
     "skl_gemm_bf16rcptex1c_bf16rcp1xte_f32rcptexterc_sm100a": (_GEMM_TE_F, None),
     "skl_gemm_f16rcptex1c_f16rcp1xte_f32rcptexterc_sm100a": (_GEMM_TE_F, None),

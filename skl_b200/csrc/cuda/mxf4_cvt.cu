@@ -81,7 +81,6 @@ template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     quant_rows_kernel(uint8_t *__restrict__ dst, int64_t rsd, uint8_t *__restrict__ scales, int64_t rss,
                       const void *__restrict__ src, int64_t rs, uint32_t m, uint32_t k, uint32_t kblocks) {
-  dep_launch();
   dep_wait();
   const uint32_t per_row = kblocks * 4u;  // groups of 8 elements
   const uint64_t first = (uint64_t)blockIdx.x * (THREADS * UNROLL);
@@ -129,7 +128,6 @@ template <int DT>
 __global__ void __launch_bounds__(THREADS)
     quant_any_kernel(uint8_t *__restrict__ dst, int64_t rsd, uint8_t *__restrict__ scales, int64_t rss,
                      const void *__restrict__ src, int64_t rs, int64_t cs, uint32_t m, uint32_t k, uint32_t kblocks) {
-  dep_launch();
   dep_wait();
   const uint64_t total = (uint64_t)m * kblocks, stride = (uint64_t)gridDim.x * (THREADS / 32);
   const int lane = threadIdx.x & 31;
@@ -158,7 +156,6 @@ __global__ void __launch_bounds__(THREADS)
   constexpr int ROWS = 32 * RPL, PITCH = 128 + 16;
   __shared__ __align__(16) uint8_t codes[ROWS * PITCH];
   __shared__ uint8_t sc[ROWS][8];
-  dep_launch();
   dep_wait();
   const uint32_t tile_r = blockIdx.x % row_tiles, tile_k = blockIdx.x / row_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -259,7 +256,6 @@ template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     widen_rows_kernel(void *__restrict__ dst, int64_t rsd, const uint8_t *__restrict__ src, int64_t rsa,
                       const uint8_t *__restrict__ scales, int64_t rss, uint32_t m, uint32_t k, int vec) {
-  dep_launch();
   dep_wait();
   const uint32_t per_row = (k + 7u) / 8u;
   const uint64_t first = (uint64_t)blockIdx.x * (THREADS * UNROLL);
@@ -307,6 +303,23 @@ __global__ void __launch_bounds__(THREADS)
       for (int e = 0; e < 8; ++e)
         if ((uint32_t)e < left) store_one<DT>(dst, at + e, x[e]);
     }
+  }
+}
+
+// fp16 as the exact sum of two bf16 values: hi keeps 8 of the 11 significant bits, lo the rest (x - hi is exact in fp32, has
+// at most 3 significant bits and an exponent that bf16 holds).  An infinity or NaN stays in hi, lo is then zero.
+// dst: rows of 2 * ld elements, hi at 0, lo at ld; the columns behind k are zeros.
+__global__ void __launch_bounds__(THREADS)
+    split_f16_kernel(uint16_t *__restrict__ dst, uint32_t ld, const uint16_t *__restrict__ src, int64_t rs, uint32_t m, uint32_t k) {
+  dep_wait();
+  const uint64_t total = (uint64_t)m * ld, stride = (uint64_t)gridDim.x * THREADS;
+  for (uint64_t i = (uint64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += stride) {
+    const uint32_t row = (uint32_t)(i / ld), col = (uint32_t)(i - (uint64_t)row * ld);
+    const float x = col < k ? dec_f16(ld_u16(src + (int64_t)row * rs + col)) : 0.0f;
+    const uint32_t hi = enc_bf16(x);
+    const bool finite = (f2u(x) & 0x7F800000u) != 0x7F800000u;
+    dst[(uint64_t)row * 2 * ld + col] = (uint16_t)hi;
+    dst[(uint64_t)row * 2 * ld + ld + col] = (uint16_t)(finite ? enc_bf16(x - dec_bf16(hi)) : 0u);
   }
 }
 
@@ -397,4 +410,11 @@ extern "C" int skl_b200_launch_widen_mxf4(void *dst, int dst_type, int64_t rsd, 
     case SKL_DT_F16: return (int)launch_widen<SKL_DT_F16>(dst, rsd, p, rsa, sc, rss, m, k, s);
     default: return (int)cudaErrorInvalidValue;
   }
+}
+
+extern "C" int skl_b200_launch_split_f16(void *dst, uint32_t ld, const void *src, int64_t rs, uint32_t m, uint32_t k,
+                                         void *stream) {
+  uint64_t grid = ceil_div((uint64_t)m * ld, THREADS * 4);
+  if (grid > 148 * 32) grid = 148 * 32;
+  return (int)launch(split_f16_kernel, grid, (cudaStream_t)stream, (uint16_t *)dst, ld, (const uint16_t *)src, rs, m, k);
 }

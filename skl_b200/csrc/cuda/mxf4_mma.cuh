@@ -1,0 +1,166 @@
+// mxf4_mma.cuh -- the inner step shared by the skinny 16-bit x MX-FP4 product and the experts' layer.
+//
+// One warp multiplies 16 weight rows by a few activation rows with mma.sync.m16n8k16 (fp16 operands, fp32 sums).  The
+// weights stay as they lie in memory: lane (g, t) = (lane / 4, lane % 4) loads the 16 bytes of block t of a 128-element
+// chunk of row g (and of row g + 8), i.e. a whole block of 32 elements with one scale, and turns them into fp16 pairs with
+// the hardware conversion of E2M1, which is exact.  An mma adds over the four lanes of a quad, whose blocks have different
+// scales, so the eight columns of the other operand are used to keep the blocks apart: column 4 * token + b holds the
+// token's activations in the k positions of lane b and zeros elsewhere.  After the eight mmas of a chunk the accumulator of
+// (row, 4 * token + b) is the unscaled sum of block b, which is multiplied by the weight block's and the activation block's
+// scale and added to the running fp32 sum: 4 multiply-adds for 64 weights per lane.  A group of columns thus serves two
+// tokens.  Measured: the conversion with the mma behind it runs at 22 T elements/s on the whole chip, against 12 T that HBM
+// delivers (17/32 byte per element at 6.4 TB/s); placing the bits of bf16 with integer instructions reached 12 T.
+//
+// fp16 activations are used as they are.  bf16 activations are brought into fp16's range with one power of two per block of
+// 32 that puts the block's largest magnitude into [2^14, 2^15): a bf16 value has 8 significant bits, so every value down to
+// 2^-31 of the block's largest stays exact, smaller ones are rounded to a multiple of 2^-38 of it -- far under the rounding
+// of the fp32 sums.
+#pragma once
+
+#include <cstdint>
+
+#include "loads.cuh"
+#include "numerics.cuh"
+
+namespace sklb {
+namespace mxmma {
+
+constexpr int STEP = 256;  // elements of k that a warp takes at a time: two chunks, 128 bytes of each of its 16 rows
+
+// the E8M0 scale of byte b: 2^(b - 127); 0 is the subnormal 2^-127, 255 NaN
+__device__ __forceinline__ float e8m0(uint32_t b) {
+  return u2f(max(b << 23, 0x00400000u) | ((b + 1u) >> 8) << 22);
+}
+
+// 8 E2M1 codes of a word as 4 fp16 pairs
+__device__ __forceinline__ void e2m1_to_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The weights of one step as a lane holds them: blocks t and t + 4 of rows g and g + 8, and the 8 scale bytes of each row.
+struct Weights {
+  uint4 code[2][2];   // [row half][chunk]
+  uint2 scale[2];     // [row half]
+};
+
+// How a warp addresses its 16 rows.
+struct RowPair {
+  const uint8_t *code[2];   // row g, row g + 8: first byte of the row
+  const uint8_t *scale[2];  // first scale byte
+};
+
+// VEC: 16-byte aligned packed rows and 8-byte aligned scale rows; otherwise single bytes.
+// Blocks behind the last one count as zeros with scale 1.
+template <bool VEC>
+__device__ __forceinline__ void load_step(Weights &w, const RowPair &rows, uint32_t step, uint32_t kblocks, int t) {
+  const uint32_t b0 = step * 8u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t b = b0 + 4u * c + t;
+      w.code[h][c] = make_uint4(0u, 0u, 0u, 0u);
+      if (b < kblocks) {
+        const uint8_t *p = rows.code[h] + (size_t)b * 16;
+        if (VEC) {
+          w.code[h][c] = ld_stream_v4(p);
+        } else {
+          uint32_t q[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            q[i] = ld_u8(p + 4 * i) | ld_u8(p + 4 * i + 1) << 8 | ld_u8(p + 4 * i + 2) << 16 | ld_u8(p + 4 * i + 3) << 24;
+          w.code[h][c] = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+      }
+    }
+    if (VEC && b0 + 8u <= kblocks) {
+      w.scale[h] = ld_v2(rows.scale[h] + b0);
+    } else {
+      uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (b0 + i < kblocks) q[i >> 2] = (q[i >> 2] & ~(0xFFu << (8 * (i & 3)))) | ld_u8(rows.scale[h] + b0 + i) << (8 * (i & 3));
+      w.scale[h] = make_uint2(q[0], q[1]);
+    }
+  }
+}
+
+// Activations in shared memory, for TG groups of two tokens: fp16 elements [token][elements] and one fp32 factor per block
+// [token][elements / 32].  `x` / `f`: shared addresses of token 0's element / block 0 of the step; the pitches are in bytes.
+// y[group][row half]: the running sums of this lane's token (2 * group + t / 2), over blocks 2 (t % 2) and 2 (t % 2) + 1
+// of every chunk: the lanes t and t ^ 1 hold the two halves of a sum.
+template <int TG, bool FACTORS>
+__device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch,
+                                              uint32_t zeros, int g, int t, float (&y)[TG][2]) {
+  const bool mine = (g & 3) == t;
+  const uint32_t token = (uint32_t)(g >> 2);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float acc[TG][4];
+#pragma unroll
+    for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
+    const uint32_t lo[4] = {w.code[0][c].x, w.code[0][c].y, w.code[0][c].z, w.code[0][c].w};
+    const uint32_t hi[4] = {w.code[1][c].x, w.code[1][c].y, w.code[1][c].z, w.code[1][c].w};
+    uint32_t at[TG];
+#pragma unroll
+    for (int q = 0; q < TG; ++q) at[q] = mine ? x + (2u * q + token) * x_pitch + c * 256u + t * 64u : zeros;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a[4], b[4];
+      e2m1_to_f16(lo[j], a);
+      e2m1_to_f16(hi[j], b);
+#pragma unroll
+      for (int q = 0; q < TG; ++q) {
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                     : "r"(at[q] + 16u * j));
+        mma_f16(acc[q], a[0], b[0], a[1], b[1], v[0], v[1]);
+        mma_f16(acc[q], a[2], b[2], a[3], b[3], v[2], v[3]);
+      }
+    }
+    float s[2][2];  // [row half][block of this lane's pair]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t word = (c ? w.scale[h].y : w.scale[h].x) >> (16 * (t & 1));
+      s[h][0] = e8m0(word & 0xFFu);
+      s[h][1] = e8m0((word >> 8) & 0xFFu);
+    }
+#pragma unroll
+    for (int q = 0; q < TG; ++q) {
+      float f0 = 1.0f, f1 = 1.0f;
+      if (FACTORS)
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(f0), "=f"(f1)
+                     : "r"(f + (2u * q + (uint32_t)(t >> 1)) * f_pitch + c * 16u + (uint32_t)(t & 1) * 8u));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float p0 = FACTORS ? acc[q][2 * h] * f0 : acc[q][2 * h], p1 = FACTORS ? acc[q][2 * h + 1] * f1 : acc[q][2 * h + 1];
+        y[q][h] = __fmaf_rn(p0, s[h][0], y[q][h]);
+        y[q][h] = __fmaf_rn(p1, s[h][1], y[q][h]);
+      }
+    }
+  }
+}
+
+// The power of two that brings a block into fp16's range, from the magnitude bits of its largest value (fp32 pattern):
+// the largest ends in [2^14, 2^15).  Returns the factor for the elements; `back` undoes it.
+__device__ __forceinline__ float block_factor(uint32_t top, float &back) {
+  const int ef = (int)(top >> 23);
+  int e = 141 - ef;  // 14 - (ef - 127)
+  e = e > 126 ? 126 : e;
+  back = u2f((uint32_t)(127 - e) << 23);
+  return u2f((uint32_t)(127 + e) << 23);
+}
+
+}  // namespace mxmma
+}  // namespace sklb

@@ -324,8 +324,11 @@ void skl_b200_synchronize(void) {
   }
 }
 
+static void scratch_trim(void);
+
 void skl_b200_release_workspace(void) {
   (void)cudaStreamSynchronize((cudaStream_t)g_ctx.stream);
+  scratch_trim();
   release_resources();
 }
 
@@ -1343,6 +1346,199 @@ void skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k, float a
   } while (0);
   leave_call();
 }
+
+/* ------------------------------------------------------------------ GEMM, 16-bit activations x MX-FP4 weights */
+
+/* Scratch memory of one call, taken from and given back to the library stream (one pool per device, kept until
+ * skl_b200_release_workspace).  Under capture the allocation becomes a node of the graph: every graph owns its scratch, and
+ * two graphs, or a graph and a later call, never share it. */
+#define MAX_DEVICES 64
+static cudaMemPool_t g_pool[MAX_DEVICES];
+static pthread_mutex_t g_pool_lock = PTHREAD_MUTEX_INITIALIZER;
+
+static void *scratch_get(size_t bytes) {
+  void *p = 0;
+  const int dev = g_ctx.device;
+  if (dev < 0 || dev >= MAX_DEVICES) {
+    set_err(SKL_B200_ERR_CUDA);
+    return 0;
+  }
+  pthread_mutex_lock(&g_pool_lock);
+  if (!g_pool[dev]) {
+    struct cudaMemPoolProps props;
+    memset(&props, 0, sizeof props);
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    uint64_t keep = UINT64_MAX; /* freed scratch stays in the pool: no device-wide stall at each synchronisation */
+    cudaMemPool_t pool = 0;
+    if (cuda_ok(cudaMemPoolCreate(&pool, &props)) && cuda_ok(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep)))
+      g_pool[dev] = pool;
+  }
+  cudaMemPool_t pool = g_pool[dev];
+  pthread_mutex_unlock(&g_pool_lock);
+  if (!pool) return 0;
+  cudaError_t e = cudaMallocFromPoolAsync(&p, bytes ? bytes : 16, pool, (cudaStream_t)g_ctx.stream);
+  if (e == cudaErrorMemoryAllocation) {
+    (void)cudaGetLastError();
+    set_err(SKL_B200_ERR_ALLOC);
+    return 0;
+  }
+  return cuda_ok(e) ? p : 0;
+}
+
+static void scratch_put(void *p) {
+  if (p) (void)cuda_ok(cudaFreeAsync(p, (cudaStream_t)g_ctx.stream));
+}
+
+static void scratch_trim(void) {
+  if (g_ctx.device < 0 || g_ctx.device >= MAX_DEVICES) return;
+  pthread_mutex_lock(&g_pool_lock);
+  if (g_pool[g_ctx.device]) (void)cudaMemPoolTrimTo(g_pool[g_ctx.device], 0);
+  pthread_mutex_unlock(&g_pool_lock);
+}
+
+typedef struct {
+  size_t m, n, k, rsa, rsb, rss, rsc;
+  int ta, tc, along_n; /* along_n: W is packed along n (k packed rows), else along k (n packed rows) */
+  float alpha, beta;
+  const void *a;
+  const uint8_t *b, *sb;
+  void *c;
+} mxf4_product_t;
+
+/* W widened exactly to bf16 and the product on the 16-bit tensor-core kernel.  fp16 activations become [hi | lo], two bf16
+ * matrices side by side, against W twice: every product stays exact.  All pointers are device memory here. */
+static void mxf4_product_widened(const mxf4_product_t *q) {
+  const int split = q->ta == SKL_DT_F16;
+  const size_t k8 = (q->k + 7) / 8 * 8, n8 = (q->n + 7) / 8 * 8, copies = split ? 2 : 1;
+  const size_t kdeep = split ? 2 * k8 : q->k;
+  const size_t wbytes = (q->along_n ? copies * k8 * n8 : q->n * copies * k8) * 2, abytes = split ? q->m * 2 * k8 * 2 : 0;
+  uint8_t *w = (uint8_t *)scratch_get(wbytes + abytes);
+  if (!w) return;
+  do {
+    int ok = 1;
+    for (size_t i = 0; ok && i < copies; ++i) {
+      if (q->along_n) {
+        uint8_t *at = w + i * k8 * n8 * 2;
+        ok = cuda_ok((cudaError_t)skl_b200_launch_widen_mxf4(at, SKL_DT_BF16, (int64_t)n8, q->b, (int64_t)q->rsb, q->sb,
+                                                             (int64_t)q->rss, (uint32_t)q->k, (uint32_t)q->n, g_ctx.stream));
+        if (ok && split && k8 > q->k)
+          ok = cuda_ok(cudaMemsetAsync(at + q->k * n8 * 2, 0, (k8 - q->k) * n8 * 2, (cudaStream_t)g_ctx.stream));
+      } else {
+        ok = cuda_ok((cudaError_t)skl_b200_launch_widen_mxf4(w + i * k8 * 2, SKL_DT_BF16, (int64_t)(copies * k8), q->b,
+                                                             (int64_t)q->rsb, q->sb, (int64_t)q->rss, (uint32_t)q->n,
+                                                             (uint32_t)(split ? k8 : q->k), g_ctx.stream));
+      }
+    }
+    if (!ok) break;
+    if (split && !cuda_ok((cudaError_t)skl_b200_launch_split_f16(w + wbytes, (uint32_t)k8, q->a, (int64_t)q->rsa,
+                                                                 (uint32_t)q->m, (uint32_t)q->k, g_ctx.stream)))
+      break;
+    skl_b200_gemm_args g;
+    memset(&g, 0, sizeof g);
+    g.m0 = q->m; g.n0 = q->n; g.k0 = kdeep;
+    g.m1 = g.n1 = g.k1 = 1;
+    g.ta = g.tb = SKL_DT_BF16; g.tc = q->tc;
+    g.epilogue = SKL_EPI_FLOAT;
+    g.a = split ? w + wbytes : q->a;
+    g.rsa0 = (int64_t)(split ? 2 * k8 : q->rsa); g.csa0 = 1;
+    g.b = w;
+    if (q->along_n) { g.rsb0 = (int64_t)n8; g.csb0 = 1; }
+    else { g.rsb0 = 1; g.csb0 = (int64_t)(copies * k8); }
+    g.c = q->c; g.rsc0 = (int64_t)q->rsc; g.csc0 = 1;
+    g.alpha_f = q->alpha; g.beta_f = q->beta;
+    /* straight to the dispatcher: every pointer is device memory, and scratch of a call under capture is not mapped yet, so
+     * that asking the driver about it would call it host memory */
+    (void)dispatch_launch(&g);
+  } while (0);
+  scratch_put(w);
+}
+
+static void run_mxf4_product(mxf4_product_t *q) {
+  g_ctx.last_path = SKL_B200_PATH_NONE;
+  if (q->m == 0 || q->n == 0) return;
+  const int static_before = g_ctx.static_weights;
+  int host_any = 0, static_b = static_before;
+  const size_t rows = q->along_n ? q->k : q->n, len = q->along_n ? q->n : q->k, kb = (len + 31) / 32;
+  if (q->k != 0) {
+    if (!on_device(q->a)) {
+      host_any = 1;
+      if (!(q->a = stage_in(WS_A, q->a, ((q->m - 1) * q->rsa + q->k) * 2))) return;
+    }
+    if (!on_device(q->b)) {
+      host_any = 1, static_b = 0;
+      if (!(q->b = (const uint8_t *)stage_in(WS_B, q->b, (rows - 1) * q->rsb + 16 * kb))) return;
+    }
+    if (!on_device(q->sb)) {
+      host_any = 1, static_b = 0;
+      if (!(q->sb = (const uint8_t *)stage_in(WS_COL, q->sb, (rows - 1) * q->rss + kb))) return;
+    }
+  }
+  out_stage_t out;
+  const int c_host = !on_device(q->c);
+  if (c_host) {
+    host_any = 1;
+    const size_t es = dt_size(q->tc);
+    if (!stage_out_begin(&out, q->c, ((q->m - 1) * q->rsc + q->n) * es, q->n * es, q->m,
+                         (q->m == 1 ? q->n : q->rsc) * es, q->beta != 0.0f))
+      return;
+    q->c = out.dev;
+  }
+  if (q->k == 0) {
+    skl_b200_gemm_args g; /* C = beta * C on the any-stride kernel */
+    memset(&g, 0, sizeof g);
+    g.m0 = q->m; g.n0 = q->n;
+    g.m1 = g.n1 = g.k1 = 1;
+    g.ta = g.tb = SKL_DT_BF16; g.tc = q->tc;
+    g.epilogue = SKL_EPI_FLOAT;
+    g.c = q->c; g.rsc0 = (int64_t)q->rsc; g.csc0 = 1;
+    g.alpha_f = q->alpha; g.beta_f = q->beta;
+    run_gemm_body(&g);
+  } else if (!q->along_n && q->m <= 8 && g_ctx.force_path == 0 && skl_b200_mxf4_skinny_supported(q->m, q->n, q->k)) {
+    g_ctx.last_path = SKL_B200_PATH_GEMV;
+    (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_skinny((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
+                                                           (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
+                                                           q->beta, q->c, q->tc, (int64_t)q->rsc, static_b, g_ctx.stream));
+  } else {
+    g_ctx.static_weights = 0; /* the widened copy is written by this call */
+    mxf4_product_widened(q);
+    g_ctx.static_weights = static_before;
+  }
+  if (g_ctx.status != SKL_B200_OK) return;
+  if (c_host && !stage_out_end(&out)) return;
+  finish(host_any);
+}
+
+static void mxf4_product(int ta, int tc, int along_n, size_t m, size_t n, size_t k, float alpha, const void *a, size_t rsa,
+                         const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rss, float beta, void *c, size_t rsc) {
+  const int none = m == 0 || n == 0;
+  if (!none && (m >= (1ull << 31) || n >= (1ull << 31) || k >= (1ull << 31) || !c || rsc < n ||
+                (k != 0 && (!a || rsa < k || !mxf4_rows_ok(b, rsb, sb, rss, along_n ? k : n, along_n ? n : k))))) {
+    refuse(SKL_B200_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  mxf4_product_t q = {m, n, k, rsa, rsb, rss, rsc, ta, tc, along_n, alpha, beta, a, b, sb, c};
+  if (!begin_call()) return;
+  run_mxf4_product(&q);
+  leave_call();
+}
+
+#define SKL_B200_DEF_GEMM_MXF4(TA, TC, TYPE_A, TYPE_C, DT_A, DT_C)                                                          \
+  void skl_gemm_##TA##_mxf4e2m1_##TC##_sm100a(size_t m, size_t n, size_t k, float alpha, const TYPE_A *a, size_t rsa,       \
+                                              const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,     \
+                                              TYPE_C *c, size_t rsc) {                                                      \
+    mxf4_product(DT_A, DT_C, 0, m, n, k, alpha, a, rsa, b, csb, sb, cssb, beta, c, rsc);                                    \
+  }                                                                                                                         \
+  void skl_gemm_##TA##_mxf4e2m1r_##TC##_sm100a(size_t m, size_t n, size_t k, float alpha, const TYPE_A *a, size_t rsa,      \
+                                               const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,    \
+                                               TYPE_C *c, size_t rsc) {                                                     \
+    mxf4_product(DT_A, DT_C, 1, m, n, k, alpha, a, rsa, b, rsb, sb, rssb, beta, c, rsc);                                    \
+  }
+SKL_B200_DEF_GEMM_MXF4(bf16, f32, skl_bf16_t, float, SKL_DT_BF16, SKL_DT_F32)
+SKL_B200_DEF_GEMM_MXF4(bf16, bf16, skl_bf16_t, skl_bf16_t, SKL_DT_BF16, SKL_DT_BF16)
+SKL_B200_DEF_GEMM_MXF4(f16, f32, skl_f16_t, float, SKL_DT_F16, SKL_DT_F32)
+SKL_B200_DEF_GEMM_MXF4(f16, f16, skl_f16_t, skl_f16_t, SKL_DT_F16, SKL_DT_F16)
 
 /* ------------------------------------------------------------------ pack / unpack / transpose */
 

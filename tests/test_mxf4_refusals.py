@@ -22,3 +22,16 @@ def test_cvt_refusals(skl, t):
         args[at] = bad
         back(*args)
         assert skl.skl_b200_last_status() == INVALID, (at, bad)
+
+
+@pytest.mark.parametrize("name", ["bf16_mxf4e2m1_f32", "bf16_mxf4e2m1_bf16", "f16_mxf4e2m1_f32", "f16_mxf4e2m1_f16",
+                                  "bf16_mxf4e2m1r_f32", "bf16_mxf4e2m1r_bf16", "f16_mxf4e2m1r_f32", "f16_mxf4e2m1r_f16"])
+def test_product_refusals(skl, name):
+    """m, n, k, alpha, a, rsa, b, rsb, sb, rssb, beta, c, rsc with n = k = 33: two blocks to a packed row either way."""
+    fn = getattr(skl, f"skl_gemm_{name}_sm100a")
+    good = [2, 33, 33, 1.0, B, 33, B, 32, B, 2, 0.0, B, 33]
+    for at, bad in [(4, 0), (6, 0), (8, 0), (11, 0), (5, 32), (7, 31), (9, 1), (12, 32), (0, 1 << 31), (1, 1 << 31), (2, 1 << 31)]:
+        args = list(good)
+        args[at] = bad
+        fn(*args)
+        assert skl.skl_b200_last_status() == INVALID, (at, bad)
