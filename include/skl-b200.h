@@ -324,6 +324,34 @@ SKL_FUNC void skl_gemm_f16_mxf4e2m1r_f16_sm100a(size_t m, size_t n, size_t k, fl
                                                 const uint8_t *b, size_t rsb, const uint8_t *sb, size_t rssb, float beta,
                                                 skl_f16_t *c, size_t rsc);
 
+/* ------------------------------------------------------------------ mixture of experts for few tokens (no SKL counterpart)
+ * One layer from the router's logits (row i of m at logits + i*rsl, `experts` of them, fp32; e.g. a skl_gemm_..._f32 of the
+ * activations and the router's weights) to the combined output:
+ *     ids[i][j]    the topk largest logits, largest first, ties to the lowest index (NaN counts as largest)
+ *     gates[i][j]  exp(logit - largest) / sum, the sum over the chosen ones (renormalise != 0) or over all experts
+ *     h            silu(G x_i) * (U x_i)                       silu as SKL_B200_ACT_SWISH with act_param 1
+ *     y_i          sum_j gates[i][j] * W2[ids[i][j]] h         (bf16, row stride rsy >= d; x: row stride rsx >= d)
+ * w1: [experts][2 f][d], rows 0..f-1 of an expert are G, rows f..2f-1 are U; w2: [experts][d][f]; dense.  The mxf4e2m1 form
+ * takes packed rows as skl_cvt_<t>rc_mxf4e2m1 writes them with dense strides (16 ceil(d / 32) code bytes and ceil(d / 32)
+ * scale bytes to a row of w1 / s1, the same with f for w2 / s2).
+ * A chosen expert whose logit is minus infinity is masked: gate 0, its weights are not used; a token whose logits are all
+ * minus infinity gets zeros.  Sums are fp32, h is kept in fp32 and enters the second product with at least 11 significant
+ * bits, y is rounded once.
+ * 1 <= topk <= 32, experts <= 1024, m <= 64, d and f from 1 to 32768; larger calls are refused (SKL_B200_ERR_UNSUPPORTED).
+ * All pointers are device memory.  `workspace`: skl_b200_moe_workspace_size bytes of the caller's, 4-byte aligned (16 is
+ * faster), not initialised, one for each call or captured graph that may run at the same time; ids and gates are dense
+ * m x topk outputs.  Outputs must not overlap inputs.  Nothing is allocated, so the call can be captured. */
+SKL_FUNC size_t skl_b200_moe_workspace_size(size_t m, size_t f, size_t experts, size_t topk);
+SKL_FUNC void skl_moe_swiglu_bf16_bf16_bf16_sm100a(size_t m, size_t d, size_t f, size_t experts, size_t topk, int renormalise,
+                                                   const float *logits, size_t rsl, const skl_bf16_t *x, size_t rsx,
+                                                   const skl_bf16_t *w1, const skl_bf16_t *w2, skl_bf16_t *y, size_t rsy,
+                                                   int32_t *ids, float *gates, void *workspace, size_t workspace_bytes);
+SKL_FUNC void skl_moe_swiglu_bf16_mxf4e2m1_bf16_sm100a(size_t m, size_t d, size_t f, size_t experts, size_t topk,
+                                                       int renormalise, const float *logits, size_t rsl, const skl_bf16_t *x,
+                                                       size_t rsx, const uint8_t *w1, const uint8_t *s1, const uint8_t *w2,
+                                                       const uint8_t *s2, skl_bf16_t *y, size_t rsy, int32_t *ids,
+                                                       float *gates, void *workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ GEMM, int8 with 4-deep k blocks
  * Same parameter list as skl_gemm_i8rcp1x4_i8p4x1c_i32_xsfvqdotq
  * (src/gemm/gemm_i8rcp1x4_i8p4x1c_i32_xsfvqdotq.h:70-75): A in 1 x 4 blocks (element (i, k) at

@@ -129,6 +129,10 @@ SIGNATURES = {
     "skl_cvt_mxf4e2m1_f32_sm100a": (_CVT_FROM_MX, None),
     "skl_cvt_mxf4e2m1_bf16_sm100a": (_CVT_FROM_MX, None),
     "skl_cvt_mxf4e2m1_f16_sm100a": (_CVT_FROM_MX, None),
+    "skl_b200_moe_workspace_size": ([_SZ] * 4, _SZ),
+    "skl_moe_swiglu_bf16_bf16_bf16_sm100a": ([_SZ] * 5 + [_I, _VP, _SZ, _VP, _SZ, _VP, _VP, _VP, _SZ, _VP, _VP, _VP, _SZ], None),
+    "skl_moe_swiglu_bf16_mxf4e2m1_bf16_sm100a": ([_SZ] * 5 + [_I, _VP, _SZ, _VP, _SZ, _VP, _VP, _VP, _VP, _VP, _SZ, _VP,
+                                                              _VP, _VP, _SZ], None),
     "skl_pack_e8rc_e8rcprc_sm100a": ([_SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, C.c_uint8],
                                      None),
     "skl_pack_e16rc_e16rcprc_sm100a": ([_SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _SZ, _SZ, _SZ, _SZ,

@@ -147,6 +147,19 @@ int skl_b200_launch_mxf4_skinny(uint32_t m, uint32_t n, uint32_t k, float alpha,
                                 const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
                                 int64_t rsc, int static_b, void *stream);
 
+/* Mixture-of-experts layer for few tokens (device pointers; see moe.cu).  mx: the weights are MX-FP4 with scales s1 / s2,
+ * else bf16.  workspace: skl_b200_moe_scratch_bytes, 4-byte aligned. */
+typedef struct skl_b200_moe_args {
+  uint32_t m, d, f, experts, topk;
+  int32_t renormalise, mx;
+  const void *logits, *x, *w1, *s1, *w2, *s2;
+  void *y, *ids, *gates, *workspace;
+  int64_t rsl, rsx, rsy;
+} skl_b200_moe_args;
+int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64_t experts, uint64_t topk);
+size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk);
+int skl_b200_launch_moe(const skl_b200_moe_args *args, void *stream);
+
 /* pack / unpack / transpose; esize in {1, 2, 4}. */
 int skl_b200_launch_pack(size_t esize, size_t m, size_t n, const void *src, size_t rs, size_t cs,
                          size_t m0, size_t n0, void *dst, size_t rs0, size_t cs0, size_t rs1,

@@ -96,13 +96,19 @@ __device__ __forceinline__ void load_step(Weights &w, const RowPair &rows, uint3
 
 // Activations in shared memory, for TG groups of two tokens: fp16 elements [token][elements] and one fp32 factor per block
 // [token][elements / 32].  `x` / `f`: shared addresses of token 0's element / block 0 of the step; the pitches are in bytes.
+// `last`: the last token there is; columns of further ones repeat it (columns do not mix) and are ignored by the caller.
 // y[group][row half]: the running sums of this lane's token (2 * group + t / 2), over blocks 2 (t % 2) and 2 (t % 2) + 1
 // of every chunk: the lanes t and t ^ 1 hold the two halves of a sum.
 template <int TG, bool FACTORS>
 __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch,
-                                              uint32_t zeros, int g, int t, float (&y)[TG][2]) {
+                                              uint32_t last, uint32_t zeros, int g, int t, float (&y)[TG][2]) {
   const bool mine = (g & 3) == t;
-  const uint32_t token = (uint32_t)(g >> 2);
+  uint32_t xrow[TG], frow[TG];
+#pragma unroll
+  for (int q = 0; q < TG; ++q) {
+    xrow[q] = mine ? x + min(2u * q + (uint32_t)(g >> 2), last) * x_pitch + t * 64u : zeros;
+    frow[q] = f + min(2u * q + (uint32_t)(t >> 1), last) * f_pitch + (uint32_t)(t & 1) * 8u;
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float acc[TG][4];
@@ -110,9 +116,7 @@ __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint
     for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
     const uint32_t lo[4] = {w.code[0][c].x, w.code[0][c].y, w.code[0][c].z, w.code[0][c].w};
     const uint32_t hi[4] = {w.code[1][c].x, w.code[1][c].y, w.code[1][c].z, w.code[1][c].w};
-    uint32_t at[TG];
-#pragma unroll
-    for (int q = 0; q < TG; ++q) at[q] = mine ? x + (2u * q + token) * x_pitch + c * 256u + t * 64u : zeros;
+    const uint32_t skip = mine ? c * 256u : 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t a[4], b[4];
@@ -123,7 +127,7 @@ __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint
         uint32_t v[4];
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                     : "r"(at[q] + 16u * j));
+                     : "r"(xrow[q] + skip + 16u * j));
         mma_f16(acc[q], a[0], b[0], a[1], b[1], v[0], v[1]);
         mma_f16(acc[q], a[2], b[2], a[3], b[3], v[2], v[3]);
       }
@@ -141,7 +145,7 @@ __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint
       if (FACTORS)
         asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
                      : "=f"(f0), "=f"(f1)
-                     : "r"(f + (2u * q + (uint32_t)(t >> 1)) * f_pitch + c * 16u + (uint32_t)(t & 1) * 8u));
+                     : "r"(frow[q] + c * 16u));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float p0 = FACTORS ? acc[q][2 * h] * f0 : acc[q][2 * h], p1 = FACTORS ? acc[q][2 * h + 1] * f1 : acc[q][2 * h + 1];

@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(512) skinny_kernel(const SkinnyParams p) {
     Weights wn;
     if (next < last_step) load_step<VEC>(wn, rows, next, p.kblocks, t);
     const uint32_t s = step - first_step;
-    multiply_step<TG, BF16>(w, x + s * (STEP * 2), x_pitch, f + s * (STEP / 8), f_pitch, zeros, g, t, y);
+    multiply_step<TG, BF16>(w, x + s * (STEP * 2), x_pitch, f + s * (STEP / 8), f_pitch, 2 * TG - 1, zeros,
+                                   g, t, y);
     w = wn;
     step = next;
   }

@@ -1540,6 +1540,66 @@ SKL_B200_DEF_GEMM_MXF4(bf16, bf16, skl_bf16_t, skl_bf16_t, SKL_DT_BF16, SKL_DT_B
 SKL_B200_DEF_GEMM_MXF4(f16, f32, skl_f16_t, float, SKL_DT_F16, SKL_DT_F32)
 SKL_B200_DEF_GEMM_MXF4(f16, f16, skl_f16_t, skl_f16_t, SKL_DT_F16, SKL_DT_F16)
 
+/* ------------------------------------------------------------------ mixture of experts */
+
+size_t skl_b200_moe_workspace_size(size_t m, size_t f, size_t experts, size_t topk) {
+  if (!skl_b200_moe_supported(m, 1, f, experts, topk)) return 0;
+  return skl_b200_moe_scratch_bytes(m, f, experts, topk);
+}
+
+static void run_moe(skl_b200_moe_args *q) {
+  const void *all[] = {q->logits, q->x, q->w1, q->s1, q->w2, q->s2, q->y, q->ids, q->gates, q->workspace};
+  if (!begin_call()) return;
+  int ok = 1;
+  for (size_t i = 0; ok && i < sizeof all / sizeof *all; ++i) ok = on_device(all[i]);
+  if (!ok) set_err(SKL_B200_ERR_INVALID_ARGUMENT);
+  else if (cuda_ok((cudaError_t)skl_b200_launch_moe(q, g_ctx.stream))) finish(0);
+  leave_call();
+}
+
+static void moe(int mx, size_t m, size_t d, size_t f, size_t experts, size_t topk, int renormalise, const float *logits,
+                size_t rsl, const void *x, size_t rsx, const void *w1, const void *s1, const void *w2, const void *s2, void *y,
+                size_t rsy, int32_t *ids, float *gates, void *workspace, size_t workspace_bytes) {
+  if (m != 0) {
+    if (d == 0 || f == 0 || topk == 0 || topk > experts || rsl < experts || rsx < d || rsy < d || !logits || !x || !w1 || !w2 ||
+        (mx && (!s1 || !s2)) || !y || !ids || !gates || !workspace || ((uintptr_t)workspace & 3u)) {
+      refuse(SKL_B200_ERR_INVALID_ARGUMENT);
+      return;
+    }
+    if (!skl_b200_moe_supported(m, d, f, experts, topk)) {
+      refuse(SKL_B200_ERR_UNSUPPORTED);
+      return;
+    }
+    if (workspace_bytes < skl_b200_moe_scratch_bytes(m, f, experts, topk)) {
+      refuse(SKL_B200_ERR_INVALID_ARGUMENT);
+      return;
+    }
+  }
+  skl_b200_moe_args q = {(uint32_t)m, (uint32_t)d, (uint32_t)f, (uint32_t)experts, (uint32_t)topk, renormalise != 0, mx,
+                         logits, x, w1, s1, w2, s2, y, ids, gates, workspace, (int64_t)rsl, (int64_t)rsx, (int64_t)rsy};
+  if (m == 0) {
+    if (begin_call()) leave_call();
+    return;
+  }
+  run_moe(&q);
+}
+
+void skl_moe_swiglu_bf16_bf16_bf16_sm100a(size_t m, size_t d, size_t f, size_t experts, size_t topk, int renormalise,
+                                          const float *logits, size_t rsl, const skl_bf16_t *x, size_t rsx,
+                                          const skl_bf16_t *w1, const skl_bf16_t *w2, skl_bf16_t *y, size_t rsy, int32_t *ids,
+                                          float *gates, void *workspace, size_t workspace_bytes) {
+  moe(0, m, d, f, experts, topk, renormalise, logits, rsl, x, rsx, w1, 0, w2, 0, y, rsy, ids, gates, workspace,
+      workspace_bytes);
+}
+void skl_moe_swiglu_bf16_mxf4e2m1_bf16_sm100a(size_t m, size_t d, size_t f, size_t experts, size_t topk, int renormalise,
+                                              const float *logits, size_t rsl, const skl_bf16_t *x, size_t rsx,
+                                              const uint8_t *w1, const uint8_t *s1, const uint8_t *w2, const uint8_t *s2,
+                                              skl_bf16_t *y, size_t rsy, int32_t *ids, float *gates, void *workspace,
+                                              size_t workspace_bytes) {
+  moe(1, m, d, f, experts, topk, renormalise, logits, rsl, x, rsx, w1, s1, w2, s2, y, rsy, ids, gates, workspace,
+      workspace_bytes);
+}
+
 /* ------------------------------------------------------------------ pack / unpack / transpose */
 
 /* op: 0 pack, 1 unpack, 2 transpose.  `plain` is the 2-D side, `blk` the blocked side. */

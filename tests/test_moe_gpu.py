@@ -1,0 +1,294 @@
+"""The experts' layer through the C ABI against 64-bit arithmetic.
+
+Tolerances, carried forward step by step (u = 2^-24, gamma(k) = 2 ((1 + u)^(k + 2) - 1), the reference suite's bound of a
+k-deep fp32 sum): the first products are off by gamma(d) |W1||x| (and 2^-38 of a block's largest |x| per product in the
+4-bit form); silu has a slope below 1.1, so h is off by 1.1 e_gate |up| + |silu| e_up + e_gate e_up + 2^-20 |h|; h enters the
+second product with 11 significant bits of its own or, below 2^-17 of its block's largest, 2^-39 of that (4-bit weights), or
+with 16 bits (two bf16 values); the second sums add gamma(f + topk); gates are off by 2^-20 of themselves; the result is
+rounded to bf16, 2^-8 of the value."""
+import numpy as np
+import pytest
+
+import helpers as H
+import mxf4_plain as MX
+import skl_b200 as S
+
+pytestmark = pytest.mark.gpu
+
+
+def gamma(k):
+    return 2 * ((1 + 2.0 ** -24) ** (k + 2) - 1)
+
+
+def bf(x):
+    return H.f32_to_bf16_bits(np.asarray(x, np.float32))
+
+
+def f64(b):
+    return H.bf16_bits_to_f32(b).astype(np.float64)
+
+
+def choose(logits, topk, renormalise):
+    """ids and gates of the definition: NaN first, then by value, ties to the lowest index; masked slots get gate 0."""
+    l = logits.astype(np.float64)
+    ids = np.stack([np.lexsort((np.arange(l.shape[1]), -np.where(np.isnan(r), np.inf, r), ~np.isnan(r)))[:topk] for r in l])
+    val = np.take_along_axis(l, ids, 1)
+    with np.errstate(invalid="ignore", over="ignore"):
+        e = np.where(val == -np.inf, 0.0, np.exp(val - val[:, :1]))
+        total = e.sum(1, keepdims=True) if renormalise else np.where(l == -np.inf, 0.0, np.exp(l - val[:, :1])).sum(1, keepdims=True)
+        gates = np.where(val == -np.inf, 0.0, e / np.where(total == 0, 1.0, total))
+    return ids, gates, val != -np.inf
+
+
+def layer(x, w1, w2, ids, gates, routed, mx):
+    """y and its tolerance before the last rounding; w1 [E][2f][d], w2 [E][d][f] in 64 bits."""
+    m, d = x.shape
+    f = w1.shape[1] // 2
+    y, tol = np.zeros((m, d)), np.zeros((m, d))
+    for i in range(m):
+        for j, e in enumerate(ids[i]):
+            if not routed[i, j]:
+                continue
+            full, absf = w1[e] @ x[i], np.abs(w1[e]) @ np.abs(x[i])
+            err = gamma(d) * absf
+            if mx:
+                blocks = np.abs(np.pad(x[i], (0, -d % 32)).reshape(-1, 32)).max(1).repeat(32)[:d]
+                err = err + 2.0 ** -38 * (np.abs(w1[e]) @ blocks)
+            g, u, eg, eu = full[:f], full[f:], err[:f], err[f:]
+            silu = g / (1 + np.exp(-g))
+            h = silu * u
+            eh = 1.1 * eg * np.abs(u) + np.abs(silu) * eu + 1.1 * eg * eu + 2.0 ** -20 * np.abs(h)
+            if mx:
+                top = np.abs(np.pad(h, (0, -f % 32)).reshape(-1, 32)).max(1).repeat(32)[:f]
+                eh = eh + np.maximum(2.0 ** -11 * np.abs(h), 2.0 ** -39 * top)
+            else:
+                eh = eh + 2.0 ** -16 * np.abs(h)
+            part, absp = w2[e] @ h, np.abs(w2[e]) @ (np.abs(h) + eh)
+            ep = np.abs(w2[e]) @ eh + gamma(f + ids.shape[1]) * absp
+            y[i] += gates[i, j] * part
+            tol[i] += gates[i, j] * (ep + (2.0 ** -20 + gamma(ids.shape[1])) * (np.abs(part) + ep))
+    return y, tol
+
+
+class Case:
+    def __init__(self, m, d, f, experts, topk, mx, renormalise=1, seed=0, pad=0, logits=None, off=0):
+        import torch
+
+        g = H.rng(seed * 7919 + m * 131 + d * 7 + f + experts * 3 + topk)
+        self.shape, self.mx, self.renormalise = (m, d, f, experts, topk), mx, renormalise
+        self.logits = g.standard_normal((m, experts)).astype(np.float32) * 2 if logits is None else np.asarray(logits, np.float32)
+        self.rsl, self.rsx, self.rsy = experts + pad, d + pad, d + pad
+        x = bf(g.standard_normal((m, d)))
+        self.x = f64(x)
+        L, X = np.full((m, self.rsl), 9e9, np.float32), bf(np.full((m, self.rsx), 5.0))
+        L[:, :experts], X[:, :d] = self.logits, x
+        put = lambda v, o=0: self._put(torch, v, o)  # noqa: E731
+        self.tl, self.tx = put(L), put(X, 2 * off)
+        if mx:
+            # weights of about 1 / sqrt(columns): scale bytes around 127 - log2(3 sqrt(columns))
+            c1, s1 = MX.random_packed(g, (experts, 2 * f, d), 121 - int(np.log2(d) / 2), 125 - int(np.log2(d) / 2))
+            c2, s2 = MX.random_packed(g, (experts, d, f), 121 - int(np.log2(f) / 2), 125 - int(np.log2(f) / 2))
+            self.w = [put(v, off) for v in (c1, s1, c2, s2)]
+            self.w1, self.w2 = MX.values(c1, s1, d), MX.values(c2, s2, f)
+        else:
+            b1, b2 = bf(g.standard_normal((experts, 2 * f, d)) / np.sqrt(d)), bf(g.standard_normal((experts, d, f)) / np.sqrt(f))
+            self.w = [put(v, 2 * off) for v in (b1, b2)]
+            self.w1, self.w2 = f64(b1), f64(b2)
+        self.out()
+
+    @staticmethod
+    def _put(torch, v, off):
+        raw = np.concatenate([np.zeros(off, np.uint8), np.ascontiguousarray(v).view(np.uint8).reshape(-1)])
+        return torch.from_numpy(raw).cuda()[off:]
+
+    def out(self):
+        import torch
+
+        m, d, f, experts, topk = self.shape
+        self.y = torch.full((m, self.rsy), 7.0, dtype=torch.bfloat16, device="cuda")
+        self.ids = torch.full((m, topk), -7, dtype=torch.int32, device="cuda")
+        self.gates = torch.full((m, topk), -7.0, device="cuda")
+        size = S.lib().skl_b200_moe_workspace_size(m, f, experts, topk)
+        self.work = torch.full((size + 64,), 255, dtype=torch.uint8, device="cuda")
+        self.size = size
+
+    def call(self):
+        lib = S.lib()
+        m, d, f, experts, topk = self.shape
+        fn = lib.skl_moe_swiglu_bf16_mxf4e2m1_bf16_sm100a if self.mx else lib.skl_moe_swiglu_bf16_bf16_bf16_sm100a
+        fn(m, d, f, experts, topk, self.renormalise, self.tl.data_ptr(), self.rsl, self.tx.data_ptr(), self.rsx,
+           *[w.data_ptr() for w in self.w], self.y.data_ptr(), self.rsy, self.ids.data_ptr(), self.gates.data_ptr(),
+           self.work.data_ptr(), self.size)
+        assert lib.skl_b200_last_status() == 0
+
+    def check(self):
+        import torch
+
+        torch.cuda.synchronize()
+        m, d, f, experts, topk = self.shape
+        ids, gates, routed = choose(self.logits, topk, self.renormalise)
+        assert np.array_equal(self.ids.cpu().numpy(), ids)
+        got = self.gates.cpu().numpy().astype(np.float64)
+        nan = np.isnan(gates)
+        assert np.array_equal(np.isnan(got), nan)
+        assert np.all(np.abs(got - gates)[~nan] <= 2.0 ** -20 * gates[~nan] + 2.0 ** -126)
+        y = f64(self.y.view(torch.int16).cpu().numpy().view(np.uint16))
+        assert np.all(y[:, d:] == 7.0), "the gap behind a row of y was written"
+        assert torch.all(self.work[self.size:] == 255), "written behind the workspace"
+        bad = nan.any(1)
+        want, tol = layer(self.x, self.w1, self.w2, ids, np.where(nan, 0.0, gates), routed, self.mx)
+        tol = tol + 2.0 ** -8 * (np.abs(want) + tol) + 2.0 ** -130
+        assert np.all(np.isnan(y[bad, :d]))
+        err = np.abs(y[:, :d] - want)[~bad]
+        assert np.all(err <= tol[~bad]), (self.shape, float(np.max(err / tol[~bad])))
+
+
+SHAPES = [(1, 64, 32, 4, 2), (1, 256, 256, 8, 8), (2, 512, 128, 16, 4), (3, 300, 100, 6, 3), (4, 1024, 512, 8, 1), (5, 40, 17, 3, 2),
+          (8, 33, 65, 60, 6), (16, 384, 272, 32, 8), (17, 128, 96, 2, 2), (40, 160, 64, 5, 4), (64, 96, 32, 1, 1), (64, 64, 64, 128, 8)]
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_layer(skl, shape, mx):
+    for renormalise in (0, 1):
+        c = Case(*shape, mx, renormalise, seed=renormalise)
+        c.call()
+        c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_larger_layer(skl, mx):
+    c = Case(16, 2048, 1024, 16, 4, mx)
+    c.call()
+    c.check()
+    c = Case(1, 4096, 1000, 8, 2, mx, seed=3)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_strides_and_alignment(skl, mx):
+    for pad, off in ((8, 0), (3, 0), (0, 1), (5, 3)):
+        c = Case(3, 256, 256, 4, 2, mx, pad=pad, off=off, seed=pad)
+        c.call()
+        c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_every_token_to_one_expert(skl, mx):
+    """More tokens of one expert than a pass takes."""
+    logits = np.zeros((37, 5), np.float32)
+    logits[:, 3] = 5.0
+    c = Case(37, 128, 96, 5, 1, mx, logits=logits)
+    c.call()
+    c.check()
+
+
+def test_ties_masks_and_nan(skl):
+    inf = np.inf
+    rows = [[0, 0, 0, 0, 0, 0], [1, 3, 3, 3, 0, 1], [-0.0, 0.0, -0.0, -1, -1, 0.0], [-inf, 2, -inf, -inf, -inf, -inf], [-inf] * 6,
+            [5, -inf, 5, -inf, 4, -inf], [1e38, -1e38, 0, 0, 0, 0], [-200, -201, -300, -299, -inf, -200.5], [0, np.nan, 1, 2, 3, 4]]
+    for mx in (False, True):
+        for renormalise in (0, 1):
+            c = Case(len(rows), 64, 48, 6, 3, mx, renormalise, logits=rows)
+            c.call()
+            c.check()
+            assert np.all(f64(c.y.view(__import__("torch").int16).cpu().numpy().view(np.uint16))[4, :64] == 0.0)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_a_masked_expert_may_hold_anything(skl, mx):
+    """NaN and infinities in the weights of an expert that no unmasked logit chooses do not reach the output."""
+    import torch
+
+    logits = np.array([[1.0, -np.inf, -np.inf]] * 2)
+    c = Case(2, 64, 32, 3, 2, mx, logits=logits)
+    if mx:
+        c.w[1].view(3, -1)[1:] = 255
+        c.w[3].view(3, -1)[1:] = 255
+    else:
+        for w in c.w:
+            w.view(torch.int16).view(3, -1)[1:] = 0x7FC0
+    c.w1[1:], c.w2[1:] = 0.0, 0.0
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_same_bits_every_time(skl, mx):
+    import torch
+
+    c = Case(9, 512, 320, 12, 4, mx)
+    first = None
+    for _ in range(4):
+        c.out()
+        c.call()
+        torch.cuda.synchronize()
+        first = c.y if first is None else first
+        assert torch.equal(first, c.y)
+    c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_captured_side_by_side_and_on_other_streams(skl, mx):
+    """Two captured layers with a workspace each, replayed together; new inputs between replays change the routing."""
+    import torch
+
+    cases = [Case(4, 256, 192, 8, 3, mx, seed=s) for s in (1, 2)]
+    cases[0].call()
+    streams, graphs = [torch.cuda.Stream() for _ in cases], []
+    skl.skl_b200_set_async(1)
+    try:
+        for c, st in zip(cases, streams):
+            skl.skl_b200_set_stream(st.cuda_stream)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                c.call()
+            graphs.append(graph)
+        for turn in range(3):
+            for c in cases:
+                c.logits = H.rng(50 + turn).standard_normal((4, 8)).astype(np.float32)
+                c.tl.copy_(torch.from_numpy(c.logits.view(np.uint8).reshape(-1)))
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for graph, st in zip(graphs, streams):
+                    with torch.cuda.stream(st):
+                        graph.replay()
+            for c in cases:
+                c.check()
+    finally:
+        skl.skl_b200_set_stream(None)
+        skl.skl_b200_set_async(0)
+
+
+def test_from_the_router_on(skl):
+    """The run of a layer: logits from the library's GEMM, weights quantised by the library, the experts on the result."""
+    import torch
+
+    m, d, f, experts, topk = 6, 128, 64, 8, 2
+    g = H.rng(12)
+    c = Case(m, d, f, experts, topk, True, seed=4)
+    router = bf(g.standard_normal((d, experts)) / np.sqrt(d))
+    tr = torch.from_numpy(router.view(np.int16)).cuda()
+    skl.skl_gemm_bf16_bf16_f32_sm100a(m, experts, d, 1.0, c.tx.data_ptr(), d, tr.data_ptr(), experts, 0.0, c.tl.data_ptr(), experts)
+    S.check()
+    c.logits = c.tl.cpu().numpy().view(np.float32).reshape(m, experts).copy()
+    assert np.allclose(c.logits, c.x @ f64(router), atol=1e-3)
+    for i, (rows, cols) in enumerate(((2 * f, d), (d, f))):
+        w = (g.standard_normal((experts * rows, cols)) / np.sqrt(cols)).astype(np.float32)
+        tw = torch.from_numpy(w).cuda()
+        skl.skl_cvt_f32rc_mxf4e2m1_sm100a(c.w[2 * i].data_ptr(), cols // 2, c.w[2 * i + 1].data_ptr(), cols // 32, tw.data_ptr(), cols,
+                                          1, experts * rows, cols)
+        S.check()
+        setattr(c, f"w{i + 1}", MX.values(*MX.quantise(w), cols).reshape(experts, rows, cols))
+    c.call()
+    c.check()
+
+
+def test_host_pointers_are_refused(skl):
+    c = Case(2, 64, 32, 4, 2, False)
+    host = np.zeros(2 * 64, np.uint16)
+    skl.skl_moe_swiglu_bf16_bf16_bf16_sm100a(2, 64, 32, 4, 2, 1, c.tl.data_ptr(), 4, S.ptr(host), 64, c.w[0].data_ptr(),
+                                             c.w[1].data_ptr(), c.y.data_ptr(), 64, c.ids.data_ptr(), c.gates.data_ptr(),
+                                             c.work.data_ptr(), c.size)
+    assert skl.skl_b200_last_status() == 1 and skl.skl_b200_last_launch_count() == 0

@@ -35,3 +35,27 @@ def test_product_refusals(skl, name):
         args[at] = bad
         fn(*args)
         assert skl.skl_b200_last_status() == INVALID, (at, bad)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_moe_refusals(skl, mx):
+    fn = skl.skl_moe_swiglu_bf16_mxf4e2m1_bf16_sm100a if mx else skl.skl_moe_swiglu_bf16_bf16_bf16_sm100a
+    size = skl.skl_b200_moe_workspace_size(2, 16, 4, 2)
+    assert size >= 2 * 2 * 16 * 4 and skl.skl_b200_moe_workspace_size(65, 16, 4, 2) == 0
+    weights = [B] * (4 if mx else 2)
+    good = [2, 32, 16, 4, 2, 1, B, 4, B, 32, *weights, B, 32, B, B, B, size]
+    y = 10 + len(weights)
+    for at, bad, status in [(1, 0, INVALID), (2, 0, INVALID), (4, 0, INVALID), (4, 5, INVALID), (6, 0, INVALID), (7, 3, INVALID),
+                            (8, 0, INVALID), (9, 31, INVALID), (10, 0, INVALID), (y - 1, 0, INVALID), (y, 0, INVALID),
+                            (y + 1, 31, INVALID), (y + 2, 0, INVALID), (y + 3, 0, INVALID), (y + 4, 0, INVALID),
+                            (y + 4, B + 2, INVALID), (y + 5, size - 1, INVALID), (0, 65, UNSUPPORTED)]:
+        args = list(good)
+        args[at] = bad
+        fn(*args)
+        assert skl.skl_b200_last_status() == status, (at, bad)
+    for at, bad in [(1, 32769), (2, 32769), (3, 1025), (4, 33)]:
+        args = list(good)
+        args[3], args[7], args[9], args[y + 1] = 1024, 4096, 40000, 40000
+        args[at] = bad
+        fn(*args)
+        assert skl.skl_b200_last_status() == UNSUPPORTED, (at, bad)
