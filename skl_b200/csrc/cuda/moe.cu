@@ -5,15 +5,16 @@
 //   y = sum_j gate[j] * W2_e h
 //
 // With few tokens the layer is a stream of the met experts' weights from HBM (2 bytes or 17/32 byte per element) with a few
-// multiply-adds each; everything is laid out so that each weight is read once and many loads are in flight:
-//   route     the pairs sorted by expert: a list of the experts that are met, each with its pairs in token order;
-//   up        one CTA for 32 features of one met expert: warps take 8 gate rows with their 8 up rows (one 16-row mma tile) and
-//             a part of d; the sums of the parts meet in shared memory, where h is formed; h stays fp32;
-//   down      a cluster of CTAs for 16 or 32 rows of W2: its warps take (expert, 256 elements of f) items in turn, each
-//             adding gate * product into sums of its own, which are added over warps and CTAs in a fixed order at the end.
-// Columns of the mma hold the tokens of an expert.  16-bit weights: mma.sync bf16, eight columns; x enters as it is, h as the
-// sum of two bf16 values in two columns (16 significant bits, so that h is not rounded to 8).  4-bit weights: mxf4_mma.cuh;
-// h enters as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result).
+// multiply-adds each.  Two kernels of one CTA of 16 warps per SM; each warp streams 16-row pieces of the weights through a
+// ring in shared memory (mxf4_mma.cuh), so that about 100 KB are in flight on an SM and no weight is read twice:
+//   up     every CTA finds the routing itself (a warp per token; cheaper than a kernel before it) and takes an equal run of the
+//          tiles of all met experts, 8 gate rows with their 8 up rows to a tile, so that both sums of a feature end in the
+//          same CTA.  Warps split d, their sums meet in shared memory, where h is formed; h stays fp32.
+//   down   a CTA owns up to 16 rows of W2 of every expert, so nothing has to be added across CTAs; its warps take (expert,
+//          piece of f) items in turn, each adding gate * product to sums of its own, which are added in order at the end.
+// Columns of the mma hold the tokens of an expert, at most 4 at a time.  16-bit weights: mma.sync bf16; x enters as it is, h as
+// the sum of two bf16 values in two columns (16 significant bits, so that h is not rounded to 8).  4-bit weights:
+// mxf4_mma.cuh; h enters as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result).
 #include "mxf4_mma.cuh"
 
 namespace sklb {
@@ -21,14 +22,15 @@ namespace {
 
 using namespace mxmma;
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int UP_TILES = 4, UP_PARTS = WARPS / UP_TILES;  // 8-feature tiles of a CTA, parts of d
-constexpr int BSTEP = 128;                                // elements of k of one 16-bit step
+constexpr int WARPS = 16, THREADS = 32 * WARPS;
+constexpr int PASS = 4;  // tokens of an expert at a time
 constexpr int MAX_TOKENS = 64, MAX_EXPERTS = 1024, MAX_TOPK = 32;
+constexpr size_t MAX_SMEM = 226 * 1024;
 
-// What route leaves in the workspace: n | expert[n] | first pair[n + 1] | pairs (token * topk + j), sorted by expert
+// The routed pairs (token * topk + j) sorted by expert: n experts met, in ascending order, expert[a] with the pairs
+// pairs[first[a]] .. pairs[first[a + 1] - 1], in token order; they are taken `per_pass` at a time, passes before expert a: turn[a].
 struct Lists {
-  int32_t *n, *expert, *first, *pairs;
+  int32_t *n, *expert, *first, *turn, *pairs;
 };
 struct MoeParams {
   const float *logits;
@@ -40,9 +42,26 @@ struct MoeParams {
   int64_t rsy;
   int32_t *ids;
   float *gates, *h;
-  Lists list;
-  uint32_t m, d, f, experts, topk;
+  Lists list;  // in the workspace, for the second kernel
+  uint32_t m, d, f, experts, topk, met;  // met: the most experts that can be met
+  uint32_t per_pass, k_warps, down_rows;
   int renormalise, x_vec, h_vec;
+};
+
+// What differs between the two weight formats: elements of a 128-byte step, bytes of a slot, elements of an item of `down`
+// and its slots.
+template <bool MX>
+struct Format {
+  static constexpr uint32_t K = MX ? 256 : 64;
+  static constexpr uint32_t SLOT = MX ? SLOT_BYTES : CODE_BYTES;
+  static constexpr uint32_t ITEM = MX ? 256 : 128;
+  static constexpr uint32_t ITEM_SLOTS = ITEM / K;
+  static __host__ __device__ uint32_t row_bytes(uint32_t cols) { return MX ? (cols + 31u) / 32u * 16u : cols * 2u; }
+  static __host__ __device__ uint32_t steps(uint32_t cols) { return (cols + K - 1u) / K; }
+  // a token's activations in shared memory: fp16 and a factor per block, or bf16 with a pitch 64 bytes more than a multiple
+  // of 128, so that the eight rows of an mma operand are read without bank conflicts
+  static __host__ __device__ uint32_t x_pitch(uint32_t steps) { return MX ? steps * (K * 2u) : steps * (K * 2u) + 64u; }
+  static __host__ __device__ uint32_t f_pitch(uint32_t steps) { return MX ? steps * (K / 8u) : 0u; }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -53,10 +72,11 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
   const uint32_t u = f2u(__fadd_rn(v, 0.0f));
   return v != v ? 0xFFFFFFFFu : ((u >> 31) ? ~u : u | 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(uint32_t key) { return u2f((key >> 31) ? key & 0x7FFFFFFFu : ~key); }
 
-// One warp, one token: ids and gates to global memory, the ids of the routed slots (-1: a logit of minus infinity, which
-// routes nowhere) to `slots`.  keys: `experts` words of this warp's shared memory.
-__device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, uint32_t *keys, int32_t *slots, int lane) {
+// One warp, one token: the routed slots (-1: a logit of minus infinity, which routes nowhere) and, with `write`, ids and
+// gates to global memory.  keys: `experts` words of this warp's shared memory.
+__device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, uint32_t *keys, int32_t *slots, int lane, bool write) {
   const float *row = p.logits + (int64_t)tok * p.rsl;
   uint32_t best = 0u, at = 0xFFFFFFFFu;  // this lane's largest key and its lowest index
   for (uint32_t e = lane; e < p.experts; e += 32u) {
@@ -64,18 +84,25 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
     keys[e] = key;
     if (key > best) best = key, at = e;
   }
-  __syncwarp();
-  float top = 0.0f, mine = 0.0f;  // the largest logit; lane j keeps exp(logit_j - top)
+  float top = 0.0f, mine = 0.0f, all = 0.0f;  // the largest logit; lane j keeps exp(logit_j - top)
   bool routed = false;
   int32_t my_id = -1;
   for (uint32_t j = 0; j < p.topk; ++j) {
     const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, best);
     const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, best == k ? at : 0xFFFFFFFFu);
-    const float v = u2f(ld_u32(row + e));
-    if (j == 0) top = v;
+    const float v = key_logit(k);
+    if (j == 0) {
+      top = v;
+      if (write && !p.renormalise) {
+        for (uint32_t i = lane; i < p.experts; i += 32u) {
+          const float w = key_logit(keys[i]);
+          all += w == -INFINITY ? 0.0f : expf(__fsub_rn(w, top));
+        }
+      }
+    }
     if ((uint32_t)lane == j) {
       my_id = (int32_t)e;
-      routed = k != 0x007FFFFFu;  // the key of minus infinity
+      routed = v != -INFINITY;
       mine = routed ? expf(__fsub_rn(v, top)) : 0.0f;
     }
     if (at == e) {  // the owner of the winner looks for its next one
@@ -87,73 +114,72 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
       }
     }
   }
-  float sum = 0.0f;
-  if (p.renormalise) {
-    sum = mine;
-  } else {
-    for (uint32_t e = lane; e < p.experts; e += 32u) {
-      const float v = u2f(ld_u32(row + e));
-      sum += v == -INFINITY ? 0.0f : expf(__fsub_rn(v, top));
-    }
-  }
+  if ((uint32_t)lane < p.topk) slots[tok * p.topk + lane] = routed ? my_id : -1;
+  if (!write) return;
+  float sum = p.renormalise ? mine : all;
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xFFFFFFFFu, sum, off));
   if ((uint32_t)lane < p.topk) {
-    const uint32_t pair = tok * p.topk + lane;
-    slots[pair] = routed ? my_id : -1;
-    p.ids[pair] = my_id;
-    p.gates[pair] = routed ? __fdiv_rn(mine, sum) : 0.0f;
+    p.ids[tok * p.topk + lane] = my_id;
+    p.gates[tok * p.topk + lane] = routed ? __fdiv_rn(mine, sum) : 0.0f;
   }
 }
 
-// One CTA: every token's choice, then the lists.  Shared memory: keys [warps][experts] | slots [m * topk] | counts [experts].
-__global__ void __launch_bounds__(512) route_kernel(const MoeParams p) {
-  extern __shared__ __align__(16) uint32_t rsmem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+// The whole CTA: every token's choice, then the lists.  scratch: keys [warps][experts] | slots [m * topk] | counts [experts].
+__device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, bool write) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t pairs = p.m * p.topk;
-  uint32_t *keys = rsmem + warp * p.experts;
-  int32_t *slots = reinterpret_cast<int32_t *>(rsmem + warps * p.experts);
-  int32_t *counts = slots + pairs;
-  dep_wait();
-  for (uint32_t tok = warp; tok < p.m; tok += warps) route_token(p, tok, keys, slots, lane);
+  int32_t *slots = reinterpret_cast<int32_t *>(scratch + WARPS * p.experts), *counts = slots + pairs;
+  for (uint32_t tok = warp; tok < p.m; tok += WARPS) route_token(p, tok, scratch + warp * p.experts, slots, lane, write);
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < p.experts; e += blockDim.x) {
+  for (uint32_t e = threadIdx.x; e < p.experts; e += THREADS) {
     int32_t c = 0;
     for (uint32_t i = 0; i < pairs; ++i) c += slots[i] == (int32_t)e;
     counts[e] = c;
   }
   __syncthreads();
-  if (warp == 0) {  // experts in ascending order: position in the list and first pair
-    int32_t n = 0, first = 0;
+  if (warp == 0) {  // experts in ascending order: position in the list, first pair, first turn
+    int32_t n = 0, first = 0, turn = 0;
     for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
       const uint32_t e = e0 + lane;
-      const int32_t c = e < p.experts ? counts[e] : 0;
+      const int32_t c = e < p.experts ? counts[e] : 0, q = (c + (int32_t)p.per_pass - 1) / (int32_t)p.per_pass;
       const uint32_t met = __ballot_sync(0xFFFFFFFFu, c > 0);
-      int32_t incl = c;
+      int32_t ci = c, qi = q;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, incl, off);
-        if (lane >= off) incl += o;
+        const int32_t a = __shfl_up_sync(0xFFFFFFFFu, ci, off), b = __shfl_up_sync(0xFFFFFFFFu, qi, off);
+        if (lane >= off) ci += a, qi += b;
       }
       if (c > 0) {
         const int32_t a = n + __popc(met & ((1u << lane) - 1u));
-        p.list.expert[a] = (int32_t)e;
-        p.list.first[a] = first + incl - c;
+        out.expert[a] = (int32_t)e;
+        out.first[a] = first + ci - c;
+        out.turn[a] = turn + qi - q;
       }
-      if (e < p.experts) counts[e] = first + incl - c;
+      if (e < p.experts) counts[e] = first + ci - c;
       n += __popc(met);
-      first += __shfl_sync(0xFFFFFFFFu, incl, 31);
+      first += __shfl_sync(0xFFFFFFFFu, ci, 31);
+      turn += __shfl_sync(0xFFFFFFFFu, qi, 31);
     }
     if (lane == 0) {
-      *p.list.n = n;
-      p.list.first[n] = first;
+      *out.n = n;
+      out.first[n] = first;
+      out.turn[n] = turn;
     }
   }
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < p.experts; e += blockDim.x) {
+  for (uint32_t e = threadIdx.x; e < p.experts; e += THREADS) {
     int32_t at = counts[e];
     for (uint32_t i = 0; i < pairs; ++i)
-      if (slots[i] == (int32_t)e) p.list.pairs[at++] = (int32_t)i;
+      if (slots[i] == (int32_t)e) out.pairs[at++] = (int32_t)i;
+  }
+  __syncthreads();
+  if (write) {
+    const int32_t n = *out.n;
+    if (threadIdx.x == 0) *p.list.n = n;
+    for (int32_t i = threadIdx.x; i < n; i += THREADS) p.list.expert[i] = out.expert[i];
+    for (int32_t i = threadIdx.x; i <= n; i += THREADS) p.list.first[i] = out.first[i], p.list.turn[i] = out.turn[i];
+    for (int32_t i = threadIdx.x; i < out.first[n]; i += THREADS) p.list.pairs[i] = out.pairs[i];
   }
 }
 
@@ -164,41 +190,19 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Lane (g, t) holds 8 consecutive elements of rows g and g + 8 in each 32-element piece of the step: the order of k inside
-// an mma does not matter as long as both operands use the same one.
-struct Wide {
-  uint4 v[2][4];
-};
-template <bool VEC>
-__device__ __forceinline__ void load_wide(Wide &w, const uint16_t *const (&rows)[2], uint32_t step, uint32_t cols, int t) {
+// Lane (g, t)'s pieces are 8 consecutive elements of rows g and g + 8 in each 32-element chunk: the order of k inside an mma
+// does not matter as long as both operands use the same one.  x: shared address of column 0 at the step's first element;
+// columns behind `last` repeat it and are ignored by the caller.
+__device__ __forceinline__ void multiply_wide(uint32_t slot, uint32_t x, uint32_t pitch, uint32_t last, int lane, float (&acc)[4]) {
+  const uint32_t at = x + min((uint32_t)(lane >> 2), last) * pitch + (lane & 3) * 16u;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t e = step * BSTEP + c * 32u + t * 8u;
-      w.v[h][c] = make_uint4(0u, 0u, 0u, 0u);
-      if (VEC) {  // cols is a multiple of 8
-        if (e < cols) w.v[h][c] = ld_stream_v4(rows[h] + e);
-      } else {
-        uint32_t q[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (e + i < cols) q[i >> 1] |= ld_u16(rows[h] + e + i) << (16 * (i & 1));
-        w.v[h][c] = make_uint4(q[0], q[1], q[2], q[3]);
-      }
-    }
-  }
-}
-// x: shared address of column 0 at the step's first element; columns behind `last` repeat it and are ignored by the caller
-__device__ __forceinline__ void multiply_wide(const Wide &w, uint32_t x, uint32_t pitch, uint32_t last, int g, int t,
-                                              float (&acc)[4]) {
-  const uint32_t at = x + min((uint32_t)g, last) * pitch + t * 16u;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t b[4];
+  for (int c = 0; c < 2; ++c) {
+    uint32_t lo[4], hi[4], b[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(slot + c * 512 + lane * 16));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(slot + (2 + c) * 512 + lane * 16));
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(at + 64u * c));
-    mma_bf16(acc, w.v[0][c].x, w.v[1][c].x, w.v[0][c].y, w.v[1][c].y, b[0], b[1]);
-    mma_bf16(acc, w.v[0][c].z, w.v[1][c].z, w.v[0][c].w, w.v[1][c].w, b[2], b[3]);
+    mma_bf16(acc, lo[0], hi[0], lo[1], hi[1], b[0], b[1]);
+    mma_bf16(acc, lo[2], hi[2], lo[3], hi[3], b[2], b[3]);
   }
 }
 
@@ -219,21 +223,44 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// sums[token][16 rows] = this warp's part of the products of up to 2 TG tokens: its steps of d
-template <int TG, bool VEC>
-__device__ __forceinline__ void up_steps_mx(const RowPair &rows, Weights w, uint32_t step, uint32_t steps, uint32_t kblocks,
-                                            uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch, uint32_t last,
-                                            uint32_t zeros, int g, int t, float *sums) {
+constexpr uint32_t UP_DEPTH = 4;   // slots of a ring
+constexpr uint32_t UP_ROUND = 4;   // tiles of a warp between two barriers
+
+// Shared memory: 64 bytes of zeros | rings (before them, for a moment, the routing's scratch) | x and factors of a pass |
+// sums [2][round][warps along d][PASS][16] | lists
+template <bool MX>
+struct UpLayout {
+  uint32_t rings, x, f, sums, sums_half, lists, total;
+  __host__ __device__ UpLayout(const MoeParams &p) {
+    using F = Format<MX>;
+    const uint32_t steps = F::steps(p.d), pairs = p.m * p.topk;
+    const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (WARPS * p.experts + pairs + p.experts) * 4u;
+    rings = 64u;
+    x = rings + ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
+    f = x + p.per_pass * F::x_pitch(steps);
+    sums = f + p.per_pass * F::f_pitch(steps);
+    sums_half = UP_ROUND * WARPS * PASS * 16u;
+    lists = sums + 2u * sums_half * 4u;
+    total = lists + (1u + p.met + 2u * (p.met + 1u) + pairs) * 4u;
+  }
+};
+
+// One tile of a warp, all its steps: sums[token][16] are this warp's part.  `fill` loads the next slot of the ring.
+template <int TG, typename Fill>
+__device__ __forceinline__ void up_tile_mx(uint32_t ring, uint32_t &slot, uint32_t first, uint32_t by, uint32_t steps, uint32_t x,
+                                           uint32_t x_pitch, uint32_t f, uint32_t f_pitch, uint32_t last, uint32_t zeros, int lane,
+                                           float *sums, Fill &fill) {
+  const int g = lane >> 2, t = lane & 3;
   float y[TG][2];
 #pragma unroll
   for (int q = 0; q < TG; ++q) y[q][0] = y[q][1] = 0.0f;
-  while (step < steps) {
-    const uint32_t next = step + UP_PARTS;
-    Weights wn;
-    if (next < steps) load_step<VEC>(wn, rows, next, kblocks, t);
-    multiply_step<TG, true>(w, x + step * (STEP * 2), x_pitch, f + step * (STEP / 8), f_pitch, last, zeros, g, t, y);
-    w = wn;
-    step = next;
+  for (uint32_t step = first; step < steps; step += by) {
+    cp_wait<UP_DEPTH - 2>();
+    __syncwarp();  // the slot's scales came through other lanes, and the slot filled next has been read by all
+    fill();
+    multiply_step<TG, true>(ring + slot * SLOT_BYTES, x + step * (STEP * 2), x_pitch, f + step * (STEP / 8), f_pitch, last, zeros,
+                            lane, y);
+    slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
   }
 #pragma unroll
   for (int q = 0; q < TG; ++q) {
@@ -245,55 +272,80 @@ __device__ __forceinline__ void up_steps_mx(const RowPair &rows, Weights w, uint
   }
 }
 
-// Shared memory: 64 bytes of zeros | sums [8 warps][8 tokens][16] | x (4-bit: fp16 [8][steps * 256], then factors
-// [8][steps * 8]; 16-bit: bf16 [8][pitch], the pitch 64 bytes more than a multiple of 128 so that the eight rows of an mma
-// operand are read without bank conflicts).  A pass takes up to `per_pass` tokens of the expert.
-template <bool MX, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) up_kernel(const MoeParams p, uint32_t per_pass) {
+template <bool MX, bool VEC, bool SVEC>
+__global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
+  using F = Format<MX>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile = warp % UP_TILES, part = warp / UP_TILES;
-  const uint32_t steps = MX ? (p.d + STEP - 1) / STEP : (p.d + BSTEP - 1) / BSTEP, kblocks = (p.d + 31u) / 32u;
-  const uint32_t x_pitch = MX ? steps * (STEP * 2) : steps * (BSTEP * 2) + 64u, f_pitch = steps * (STEP / 8);
-  float *sums = reinterpret_cast<float *>(smem + 64);
-  const uint32_t zeros = smem_addr(smem), x = zeros + 64u + WARPS * 8 * 16 * 4, f = x + per_pass * x_pitch;
-  const uint32_t feature0 = blockIdx.x * (8u * UP_TILES);
+  const UpLayout<MX> at(p);
+  const uint32_t steps = F::steps(p.d), row_bytes = F::row_bytes(p.d), kblocks = (p.d + 31u) / 32u, tiles = (p.f + 7u) / 8u;
+  const uint32_t x_pitch = F::x_pitch(steps), f_pitch = F::f_pitch(steps);
+  const uint32_t zeros = smem_addr(smem), x = zeros + at.x, f = zeros + at.f, ring = zeros + at.rings + warp * (UP_DEPTH * F::SLOT);
+  float *sums = reinterpret_cast<float *>(smem + at.sums);
+  Lists list;
+  list.n = reinterpret_cast<int32_t *>(smem + at.lists);
+  list.expert = list.n + 1;
+  list.first = list.expert + p.met;
+  list.turn = list.first + p.met + 1;
+  list.pairs = list.turn + p.met + 1;
   if (threadIdx.x < 16) reinterpret_cast<uint32_t *>(smem)[threadIdx.x] = 0u;
 
   dep_wait();
-  if ((int32_t)blockIdx.y >= *p.list.n) return;
-  const uint32_t e = (uint32_t)p.list.expert[blockIdx.y];
-  const int32_t first = p.list.first[blockIdx.y], last = p.list.first[blockIdx.y + 1];
+  route(p, reinterpret_cast<uint32_t *>(smem + at.rings), list, blockIdx.x == 0);
+  const int32_t n = *list.n;
+  const uint64_t total = (uint64_t)list.turn[n] * tiles;  // every pass over an expert counts
+  const uint32_t u0 = (uint32_t)(total * blockIdx.x / gridDim.x), u1 = (uint32_t)(total * (blockIdx.x + 1) / gridDim.x);
+  __syncthreads();  // the routing's scratch becomes the rings
 
-  const uint32_t feat = min(feature0 + 8u * tile + g, p.f - 1u);  // features behind the last are not stored
-  RowPair rows;
-  const uint16_t *wide[2];
+  // this warp's items: steps kw, kw + KW, ... of tiles u0 + tw, u0 + tw + TW, ...
+  const uint32_t KW = p.k_warps, TW = WARPS / KW, kw = warp % KW, tw = warp / KW;
+  TileRows rows;
+  int32_t aim_a = 0;
+  auto aim = [&](uint32_t u) {
+    const uint32_t turn = u / tiles, feature0 = (u - turn * tiles) * 8u;
+    while ((int32_t)turn >= list.turn[aim_a + 1]) ++aim_a;
+    const uint64_t base = (uint64_t)list.expert[aim_a] * 2u * p.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint64_t r = (uint64_t)e * 2u * p.f + (h ? p.f : 0u) + feat;
+    for (int h = 0; h < 2; ++h)
+      rows.code[h] = feature0 + g < p.f ? p.w1 + (base + (h ? p.f : 0u) + feature0 + g) * row_bytes : nullptr;
     if (MX) {
-      rows.code[h] = p.w1 + r * kblocks * 16u;
-      rows.scale[h] = p.s1 + r * kblocks;
-    } else {
-      wide[h] = reinterpret_cast<const uint16_t *>(p.w1) + r * p.d;
+      const uint32_t r = lane >> 1;
+      rows.scale = feature0 + (r & 7u) < p.f ? p.s1 + (base + (r >= 8u ? p.f : 0u) + feature0 + (r & 7u)) * kblocks : nullptr;
     }
-  }
-  for (int32_t at = first; at < last; at += (int32_t)per_pass) {
-    const uint32_t cnt = min((uint32_t)(last - at), per_pass);
-    Weights w;
-    Wide wb;
-    if ((uint32_t)part < steps) {
-      if (MX) load_step<VEC>(w, rows, part, kblocks, t);
-      else load_wide<VEC>(wb, wide, part, p.d, t);
+  };
+  uint32_t fill_u = u0 + tw, fill_step = kw, fill_at = 0;
+  auto fill = [&]() {
+    if (fill_u < u1) {
+      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, fill_step, row_bytes, lane);
+      fill_step += KW;
+      if (fill_step >= steps) {
+        fill_step = kw;
+        fill_u += TW;
+        if (fill_u < u1) aim(fill_u);
+      }
     }
-    // the tokens' activations; four lanes share a block of 32
-    const uint32_t groups = steps * (MX ? STEP / 8 : BSTEP / 8), total = cnt * groups;
-    for (uint32_t i0 = 0; i0 < total; i0 += THREADS) {
+    cp_commit();
+    fill_at = fill_at + 1 == UP_DEPTH ? 0 : fill_at + 1;
+  };
+  if (fill_u < u1) aim(fill_u);
+#pragma unroll
+  for (uint32_t i = 0; i < UP_DEPTH - 1; ++i) fill();
+
+  uint32_t slot = 0, half = 0;
+  int32_t a = 0;
+  for (uint32_t u = u0; u < u1;) {  // a segment: this CTA's tiles of one pass over one expert
+    const uint32_t turn = u / tiles, seg_end = (uint32_t)min((uint64_t)u1, (uint64_t)(turn + 1u) * tiles);
+    while ((int32_t)turn >= list.turn[a + 1]) ++a;
+    const uint32_t pair0 = (uint32_t)list.first[a] + (turn - (uint32_t)list.turn[a]) * p.per_pass;
+    const uint32_t cnt = min(p.per_pass, (uint32_t)list.first[a + 1] - pair0);
+    // the tokens' activations (the last segment's were read before the barrier of its last round); four lanes share a block
+    const uint32_t groups = steps * (F::K / 8u), all = cnt * groups;
+    for (uint32_t i0 = 0; i0 < all; i0 += THREADS) {
       const uint32_t i = i0 + threadIdx.x;
-      const bool in = i < total;
+      const bool in = i < all;
       const uint32_t j = in ? i / groups : 0u, gr = in ? i - j * groups : 0u;
       uint32_t v[4];
-      const uint32_t tok = (uint32_t)p.list.pairs[at + j] / p.topk;
+      const uint32_t tok = (uint32_t)list.pairs[pair0 + j] / p.topk;
       load_x8(v, p.x + (int64_t)tok * p.rsx, gr * 8u, in ? p.d : 0u, p.x_vec);
       if (MX) {
         uint32_t top = 0;
@@ -310,258 +362,274 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const MoeParams p, uint3
       if (in) st_shared_v4(x + j * x_pitch + gr * 16u, v[0], v[1], v[2], v[3]);
     }
     __syncthreads();
-    float *own = sums + warp * (8 * 16);
-    if (MX) {
-      if (cnt <= 2) up_steps_mx<1, VEC>(rows, w, part, steps, kblocks, x, x_pitch, f, f_pitch, cnt - 1u, zeros, g, t, own);
-      else if (cnt <= 4) up_steps_mx<2, VEC>(rows, w, part, steps, kblocks, x, x_pitch, f, f_pitch, cnt - 1u, zeros, g, t, own);
-      else up_steps_mx<4, VEC>(rows, w, part, steps, kblocks, x, x_pitch, f, f_pitch, cnt - 1u, zeros, g, t, own);
-    } else {
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (uint32_t step = part; step < steps;) {
-        const uint32_t next = step + UP_PARTS;
-        Wide wn;
-        if (next < steps) load_wide<VEC>(wn, wide, next, p.d, t);
-        multiply_wide(wb, x + step * (BSTEP * 2), x_pitch, cnt - 1u, g, t, acc);
-        wb = wn;
-        step = next;
-      }
+    for (uint32_t r0 = u; r0 < seg_end; r0 += UP_ROUND * TW) {
+      const uint32_t r1 = min(seg_end, r0 + UP_ROUND * TW);
+      float *round = sums + half * at.sums_half;
+      for (uint32_t v = r0 + (tw + TW - (r0 - u0) % TW) % TW; v < r1; v += TW) {
+        float *own = round + ((v - r0) * KW + kw) * (PASS * 16);
+        if (MX) {
+          if (cnt <= 2) up_tile_mx<1>(ring, slot, kw, KW, steps, x, x_pitch, f, f_pitch, cnt - 1u, zeros, lane, own, fill);
+          else up_tile_mx<2>(ring, slot, kw, KW, steps, x, x_pitch, f, f_pitch, cnt - 1u, zeros, lane, own, fill);
+        } else {
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (uint32_t step = kw; step < steps; step += KW) {
+            cp_wait<UP_DEPTH - 2>();
+            __syncwarp();
+            fill();
+            multiply_wide(ring + slot * F::SLOT, x + step * (F::K * 2u), x_pitch, cnt - 1u, lane, acc);
+            slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
+          }
+          if (t < 2) {  // columns 2 t and 2 t + 1 of the four tokens
 #pragma unroll
-      for (int q = 0; q < 4; ++q) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
-    }
-    __syncthreads();
-    {  // one (token, feature) per thread: h = silu(gate) * up
-      const uint32_t j = threadIdx.x / 32u, c = threadIdx.x & 31u, feature = feature0 + c;
-      if (j < cnt && feature < p.f) {
-        const float *s = sums + (c / 8u) * (8 * 16) + j * 16 + (c & 7u);
-        float gate = 0.0f, up = 0.0f;
-#pragma unroll
-        for (int q = 0; q < UP_PARTS; ++q) {
-          gate += s[q * UP_TILES * (8 * 16)];
-          up += s[q * UP_TILES * (8 * 16) + 8];
+            for (int q = 0; q < 4; ++q) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
+          }
         }
-        p.h[(uint64_t)p.list.pairs[at + j] * p.f + feature] = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
       }
+      __syncthreads();
+      // h = silu(gate) * up; the other half of the sums is written meanwhile
+      const uint32_t outs = (r1 - r0) * 8u * cnt;
+      for (uint32_t i = threadIdx.x; i < outs; i += THREADS) {
+        const uint32_t c = i % (8u * (r1 - r0)), j = i / (8u * (r1 - r0));
+        const uint32_t feature = (r0 - turn * tiles) * 8u + c;
+        if (feature < p.f) {
+          const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
+          float gate = 0.0f, up = 0.0f;
+          for (uint32_t q = 0; q < KW; ++q) {
+            gate += s[q * (PASS * 16)];
+            up += s[q * (PASS * 16) + 8];
+          }
+          p.h[(uint64_t)list.pairs[pair0 + j] * p.f + feature] = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
+        }
+      }
+      half ^= 1u;
     }
-    // the next pass writes x and sums again: x only after this pass's multiplications, which the barrier above ended; the
-    // sums only after its own first barrier
+    u = seg_end;
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------- down
-constexpr int DOWN_K = 256;  // elements of f of one item
-
-// Shared memory: 64 bytes of zeros | per warp: h of the item (4-bit: fp16 [4][256], factors [4][8]; 16-bit: bf16 hi of four
-// tokens, then lo, [8][256] with a pitch of 576 bytes) | per warp: sums [m][rows]
-template <bool MX>
-struct Down {
-  static constexpr int RT = MX ? 2 : 1;  // 16-row tiles of a warp
-  static constexpr int ROWS = 16 * RT;
-  static constexpr int PASS = 4;         // tokens at a time
-  static constexpr int PITCH = MX ? DOWN_K * 2 : DOWN_K * 2 + 64;
-  static constexpr int STAGE = MX ? PASS * PITCH + PASS * (DOWN_K / 32) * 4 : 2 * PASS * PITCH;
-  static constexpr size_t smem(uint32_t m) { return 64 + (size_t)WARPS * STAGE + (size_t)WARPS * m * ROWS * 4; }
+// Shared memory: 64 bytes of zeros | rings | per warp: h of an item (4-bit: fp16 [4][256] and factors [4][8]; 16-bit: bf16, the
+// first parts of four tokens, then the second parts, [8][128] with a pitch of 320 bytes) | per warp: sums [m][16]
+template <bool MX, int DEPTH>
+struct DownLayout {
+  static constexpr uint32_t PITCH = MX ? 512 : 320;
+  static constexpr uint32_t STAGE = MX ? PASS * PITCH + PASS * 32 : 2 * PASS * PITCH;
+  static constexpr uint32_t RINGS = 64, STAGES = RINGS + WARPS * DEPTH * Format<MX>::SLOT, SUMS = STAGES + WARPS * STAGE;
+  static size_t total(uint32_t m) { return SUMS + (size_t)WARPS * m * 16 * 4; }
 };
 
-template <bool MX, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) down_kernel(const MoeParams p) {
-  using D = Down<MX>;
+template <bool MX, bool VEC, bool SVEC, int DEPTH>
+__global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
+  using F = Format<MX>;
+  using L = DownLayout<MX, DEPTH>;
+  constexpr int PER = F::ITEM / 32;  // elements of an item that a lane converts
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint32_t rank, ranks;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  const uint32_t row0 = (blockIdx.x / ranks) * D::ROWS;
-  const uint32_t zeros = smem_addr(smem), stage = zeros + 64u + warp * D::STAGE, factors = stage + D::PASS * D::PITCH;
-  float *all = reinterpret_cast<float *>(smem + 64 + WARPS * D::STAGE);  // [warp][m][ROWS]
-  float *own = all + (size_t)warp * p.m * D::ROWS;
+  const uint32_t row0 = blockIdx.x * p.down_rows, nrows = min(p.down_rows, p.d - row0);
+  const uint32_t row_bytes = F::row_bytes(p.f), kblocks = (p.f + 31u) / 32u;
+  const uint32_t zeros = smem_addr(smem), ring = zeros + L::RINGS + warp * (DEPTH * F::SLOT);
+  const uint32_t stage = zeros + L::STAGES + warp * L::STAGE, factors = stage + PASS * L::PITCH;
+  float *sums = reinterpret_cast<float *>(smem + L::SUMS), *own = sums + (size_t)warp * p.m * 16;
   if (threadIdx.x < 16) reinterpret_cast<uint32_t *>(smem)[threadIdx.x] = 0u;
-  for (uint32_t i = lane; i < p.m * D::ROWS; i += 32u) own[i] = 0.0f;
+  for (uint32_t i = lane; i < p.m * 16u; i += 32u) own[i] = 0.0f;
   __syncthreads();
   dep_wait();
 
-  const uint32_t kblocks = (p.f + 31u) / 32u, parts = (p.f + DOWN_K - 1) / DOWN_K;
-  const uint32_t items = (uint32_t)*p.list.n * parts;
-  for (uint32_t item = rank * WARPS + warp; item < items; item += ranks * WARPS) {
-    const uint32_t a = item / parts, k0 = (item - a * parts) * DOWN_K;
-    const uint32_t e = (uint32_t)p.list.expert[a];
-    const int32_t first = p.list.first[a], last = p.list.first[a + 1];
-    Weights w[D::RT];
-    Wide wb[2];
+  const uint32_t parts = (p.f + F::ITEM - 1u) / F::ITEM, items = (uint32_t)*p.list.n * parts;
+  TileRows rows;
+  auto aim = [&](uint32_t item) {
+    const uint64_t base = (uint64_t)p.list.expert[item / parts] * p.d + row0;
 #pragma unroll
-    for (int r = 0; r < D::RT; ++r) {
-      RowPair rows;
-      const uint16_t *wide[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t row = min(row0 + 16u * r + g + 8u * h, p.d - 1u);
-        const uint64_t at = (uint64_t)e * p.d + row;
-        if (MX) {
-          rows.code[h] = p.w2 + at * kblocks * 16u;
-          rows.scale[h] = p.s2 + at * kblocks;
-        } else {
-          wide[h] = reinterpret_cast<const uint16_t *>(p.w2) + at * p.f;
-        }
-      }
-      if (MX) {
-        load_step<VEC>(w[r], rows, k0 / STEP, kblocks, t);
-      } else {
-        load_wide<VEC>(wb[0], wide, k0 / BSTEP, p.f, t);
-        load_wide<VEC>(wb[1], wide, k0 / BSTEP + 1u, p.f, t);
+    for (int h = 0; h < 2; ++h) rows.code[h] = g + 8u * h < nrows ? p.w2 + (base + g + 8u * h) * row_bytes : nullptr;
+    if (MX) rows.scale = (uint32_t)(lane >> 1) < nrows ? p.s2 + (base + (lane >> 1)) * kblocks : nullptr;
+  };
+  uint32_t fill_item = warp, fill_sub = 0, fill_at = 0;
+  auto fill = [&]() {
+    if (fill_item < items) {
+      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, (fill_item % parts) * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
+      if (++fill_sub == F::ITEM_SLOTS) {
+        fill_sub = 0;
+        fill_item += WARPS;
+        if (fill_item < items) aim(fill_item);
       }
     }
-    for (int32_t at = first; at < last; at += D::PASS) {
-      const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)D::PASS);
-      __syncwarp();  // the pass before has read its h
-      for (uint32_t j = 0; j < cnt; ++j) {  // lane: 8 consecutive elements of f
-        const float *src = p.h + (uint64_t)p.list.pairs[at + j] * p.f;
-        const uint32_t col = k0 + lane * 8u;
-        float v[8];
-        if (p.h_vec && col + 8u <= p.f) {
-          const float4 v0 = __ldcg(reinterpret_cast<const float4 *>(src + col)), v1 = __ldcg(reinterpret_cast<const float4 *>(src + col) + 1);
-          v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
-        } else {
+    cp_commit();
+    fill_at = fill_at + 1 == DEPTH ? 0 : fill_at + 1;
+  };
+  // h of up to PASS pairs from `at` on: PER elements of each to a lane
+  auto load_h = [&](float (&v)[PASS][PER], int32_t at, int32_t last, uint32_t k0) {
+    const uint32_t col = k0 + lane * PER;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = col + q < p.f ? __ldcg(src + col + q) : 0.0f;
-        }
-        if (MX) {
-          uint32_t top = 0;
+    for (int j = 0; j < PASS; ++j) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) top = max(top, f2u(v[q]) & 0x7FFFFFFFu);
-          top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-          top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-          float back;
-          const float factor = block_factor(top, back);
-          st_shared_v4(stage + j * D::PITCH + lane * 16u, pack_f16x2_no_nan(v[0] * factor, v[1] * factor),
-                       pack_f16x2_no_nan(v[2] * factor, v[3] * factor), pack_f16x2_no_nan(v[4] * factor, v[5] * factor),
-                       pack_f16x2_no_nan(v[6] * factor, v[7] * factor));
-          if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(factors + j * (DOWN_K / 32) * 4u + g * 4u), "f"(back) : "memory");
-        } else {
-          uint32_t hi[4], lo[4];
+      for (int q = 0; q < PER; ++q) v[j][q] = 0.0f;
+      if (at + j < last) {
+        const float *src = p.h + (uint64_t)p.list.pairs[at + j] * p.f + col;
+        if (p.h_vec && col + PER <= p.f) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            hi[q] = pack_bf16x2_no_nan(v[2 * q], v[2 * q + 1]);
-            const float a0 = u2f(hi[q] << 16), a1 = u2f(hi[q] & 0xFFFF0000u);
-            // an infinity or NaN stays in the first part
-            lo[q] = pack_bf16x2_no_nan(fabsf(a0) < INFINITY ? v[2 * q] - a0 : 0.0f, fabsf(a1) < INFINITY ? v[2 * q + 1] - a1 : 0.0f);
+          for (int q = 0; q < PER; q += 4) {
+            const float4 w = __ldcg(reinterpret_cast<const float4 *>(src + q));
+            v[j][q] = w.x, v[j][q + 1] = w.y, v[j][q + 2] = w.z, v[j][q + 3] = w.w;
           }
-          st_shared_v4(stage + j * D::PITCH + lane * 16u, hi[0], hi[1], hi[2], hi[3]);
-          st_shared_v4(stage + (j + D::PASS) * D::PITCH + lane * 16u, lo[0], lo[1], lo[2], lo[3]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < PER; ++q)
+            if (col + q < p.f) v[j][q] = __ldcg(src + q);
         }
       }
+    }
+  };
+  auto store_h = [&](const float (&v)[PASS][PER], uint32_t cnt) {
+#pragma unroll
+    for (int j = 0; j < PASS; ++j) {
+      if ((uint32_t)j >= cnt) break;
+      if (MX) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) top = max(top, f2u(v[j][q]) & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        float back;
+        const float c = block_factor(top, back);
+        st_shared_v4(stage + j * L::PITCH + lane * 16u, pack_f16x2_no_nan(v[j][0] * c, v[j][1] * c), pack_f16x2_no_nan(v[j][2] * c, v[j][3] * c),
+                     pack_f16x2_no_nan(v[j][4 % PER] * c, v[j][5 % PER] * c), pack_f16x2_no_nan(v[j][6 % PER] * c, v[j][7 % PER] * c));
+        if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(factors + j * 32u + g * 4u), "f"(back) : "memory");
+      } else {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float a = v[j][2 * q], b = v[j][2 * q + 1];
+          hi[q] = pack_bf16x2_no_nan(a, b);
+          const float a0 = u2f(hi[q] << 16), b0 = u2f(hi[q] & 0xFFFF0000u);
+          // an infinity or NaN stays in the first part
+          lo[q] = pack_bf16x2_no_nan(fabsf(a0) < INFINITY ? a - a0 : 0.0f, fabsf(b0) < INFINITY ? b - b0 : 0.0f);
+        }
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + j * L::PITCH + lane * 8u), "r"(hi[0]), "r"(hi[1]) : "memory");
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + (j + PASS) * L::PITCH + lane * 8u), "r"(lo[0]), "r"(lo[1]) : "memory");
+      }
+    }
+  };
+  if (fill_item < items) aim(fill_item);
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; ++i) fill();
+
+  float v[PASS][PER];
+  if ((uint32_t)warp < items) {
+    const uint32_t e = warp / parts;
+    load_h(v, p.list.first[e], p.list.first[e + 1], (warp % parts) * F::ITEM);
+  }
+  uint32_t slot = 0;
+  for (uint32_t item = warp; item < items; item += WARPS) {
+    const uint32_t a = item / parts, k0 = (item - a * parts) * F::ITEM, next = item + WARPS;
+    const int32_t first = p.list.first[a], last = p.list.first[a + 1];
+#pragma unroll
+    for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) {
+      cp_wait<DEPTH - 1 - (int)F::ITEM_SLOTS>();  // all slots of the item
+      if (s == 0) __syncwarp();
+    }
+    for (int32_t at = first; at < last; at += PASS) {
+      const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)PASS);
+      if (at != first) load_h(v, at, last, k0);
+      __syncwarp();  // the h before has been read
+      store_h(v, cnt);
+      if (at + PASS >= last && next < items) load_h(v, p.list.first[next / parts], p.list.first[next / parts + 1], (next % parts) * F::ITEM);
       __syncwarp();
       if (MX) {
+        float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+        if (cnt <= 2) {
+          float y1[1][2] = {{0.0f, 0.0f}};
+          multiply_step<1, true>(ring + slot * F::SLOT, stage, L::PITCH, factors, 32, cnt - 1u, zeros, lane, y1);
+          y[0][0] = y1[0][0], y[0][1] = y1[0][1];
+        } else {
+          multiply_step<2, true>(ring + slot * F::SLOT, stage, L::PITCH, factors, 32, cnt - 1u, zeros, lane, y);
+        }
 #pragma unroll
-        for (int r = 0; r < D::RT; ++r) {
-          float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-          if (cnt <= 2) {
-            float(&y1)[1][2] = reinterpret_cast<float(&)[1][2]>(y);
-            multiply_step<1, true>(w[r], stage, D::PITCH, factors, DOWN_K / 32 * 4, cnt - 1u, zeros, g, t, y1);
-          } else {
-            multiply_step<2, true>(w[r], stage, D::PITCH, factors, DOWN_K / 32 * 4, cnt - 1u, zeros, g, t, y);
-          }
+        for (int q = 0; q < 2; ++q) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float v = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
-              const uint32_t j = 2u * q + (uint32_t)(t >> 1);
-              if ((t & 1) == 0 && j < cnt) {
-                const uint32_t pair = (uint32_t)p.list.pairs[at + j];
-                float *o = own + (pair / p.topk) * D::ROWS + 16 * r + g + 8 * h;
-                *o = __fmaf_rn(p.gates[pair], v, *o);
-              }
+          for (int h = 0; h < 2; ++h) {
+            const float s = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
+            const uint32_t j = 2u * q + (uint32_t)(t >> 1);
+            if ((t & 1) == 0 && j < cnt) {
+              const uint32_t pair = (uint32_t)p.list.pairs[at + j];
+              float *o = own + (pair / p.topk) * 16 + g + 8 * h;
+              *o = __fmaf_rn(p.gates[pair], s, *o);
             }
           }
         }
       } else {
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        multiply_wide(wb[0], stage, D::PITCH, 7u, g, t, acc);
-        multiply_wide(wb[1], stage + BSTEP * 2, D::PITCH, 7u, g, t, acc);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // columns 2 t, 2 t + 1: the first part of tokens 0..3 in lanes t = 0, 1, the second in 2, 3
-          const float v = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
+        for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) {
+          const uint32_t i = slot + s >= DEPTH ? slot + s - DEPTH : slot + s;
+          multiply_wide(ring + i * F::SLOT, stage + s * (F::K * 2u), L::PITCH, 7u, lane, acc);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // columns 2 t, 2 t + 1: the first parts of the four tokens in lanes t = 0, 1, the second in 2, 3
+          const float s = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
           const uint32_t j = 2u * t + (q & 1);
           if (t < 2 && j < cnt) {
             const uint32_t pair = (uint32_t)p.list.pairs[at + j];
-            float *o = own + (pair / p.topk) * D::ROWS + g + 8 * (q >> 1);
-            *o = __fmaf_rn(p.gates[pair], v, *o);
+            float *o = own + (pair / p.topk) * 16 + g + 8 * (q >> 1);
+            *o = __fmaf_rn(p.gates[pair], s, *o);
           }
         }
       }
     }
+    __syncwarp();  // every lane has read the item's slots
+#pragma unroll
+    for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) fill();
+    slot += F::ITEM_SLOTS;
+    if (slot >= DEPTH) slot -= DEPTH;
   }
   __syncthreads();
-  // over the warps, then over the cluster's CTAs, in order
-  const uint32_t outs = p.m * D::ROWS;
-  for (uint32_t i = threadIdx.x; i < outs; i += THREADS) {
-    float v = all[i];
+  for (uint32_t i = threadIdx.x; i < p.m * 16u; i += THREADS) {
+    const uint32_t tok = i >> 4, r = i & 15u;
+    float s = sums[i];
 #pragma unroll
-    for (int q = 1; q < WARPS; ++q) v += all[(size_t)q * outs + i];
-    all[i] = v;
+    for (int q = 1; q < WARPS; ++q) s += sums[(size_t)q * p.m * 16 + i];
+    if (r < nrows) p.y[(int64_t)tok * p.rsy + row0 + r] = (uint16_t)enc_bf16(s);
   }
-  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else __syncthreads();
-  for (uint32_t i = rank * THREADS + threadIdx.x; i < outs; i += ranks * THREADS) {
-    float v = 0.0f;
-    const uint32_t at = smem_addr(all + i);
-    for (uint32_t r = 0; r < ranks; ++r) {
-      uint32_t remote;
-      float part;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(remote) : "memory");
-      v += part;
-    }
-    const uint32_t tok = i / D::ROWS, row = row0 + i % D::ROWS;
-    if (row < p.d) p.y[(int64_t)tok * p.rsy + row] = (uint16_t)enc_bf16(v);
-  }
-  // no CTA leaves while its shared memory may still be read
-  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, unsigned ranks, cudaStream_t s, A... args) {
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+cudaError_t launch(void (*kernel)(P...), unsigned grid, size_t smem, cudaStream_t s, A... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ranks;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = 1;
   SKLB_COUNT_LAUNCH();
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-constexpr size_t UP_BUDGET = 96 * 1024;  // activations of one pass: two CTAs on an SM
-
-template <bool MX, bool VEC>
-cudaError_t launch_moe(const MoeParams &p, cudaStream_t s) {
-  const uint32_t pairs = p.m * p.topk, met = pairs < p.experts ? pairs : p.experts;
-  const unsigned warps = p.m < 16 ? p.m : 16;
-  cudaError_t e = launch(route_kernel, dim3(1), 32 * warps, ((size_t)warps * p.experts + pairs + p.experts) * 4, 1, s, p);
+template <bool MX, bool VEC, bool SVEC>
+cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
+  using F = Format<MX>;
+  const uint32_t pairs = p.m * p.topk;
+  p.met = pairs < p.experts ? pairs : p.experts;
+  const uint32_t steps = F::steps(p.d);
+  p.k_warps = 1;
+  while (p.k_warps < (uint32_t)WARPS && p.k_warps * 2u <= steps) p.k_warps *= 2u;
+  p.per_pass = p.m < PASS ? p.m : PASS;
+  while (p.per_pass > 1 && UpLayout<MX>(p).total > MAX_SMEM) --p.per_pass;
+  const UpLayout<MX> up(p);
+  if (up.total > MAX_SMEM) return cudaErrorInvalidConfiguration;
+  // an SM has room for one CTA; never more CTAs than tiles that can exist
+  const uint64_t most = (uint64_t)p.met * ((p.m + p.per_pass - 1) / p.per_pass) * ((p.f + 7) / 8);
+  cudaError_t e = launch(up_kernel<MX, VEC, SVEC>, (unsigned)(most < 148 ? most : 148), up.total, s, (const MoeParams)p);
   if (e != cudaSuccess) return e;
-  const uint32_t steps = MX ? (p.d + STEP - 1) / STEP : (p.d + BSTEP - 1) / BSTEP;
-  const size_t per_token = MX ? (size_t)steps * (STEP * 2 + STEP / 8) : (size_t)steps * (BSTEP * 2) + 64;
-  uint32_t per_pass = p.m < 8 ? p.m : 8;
-  while (per_pass > 1 && per_pass * per_token > UP_BUDGET) --per_pass;
-  e = launch(up_kernel<MX, VEC>, dim3((p.f + 31) / 32, met), THREADS, 64 + WARPS * 8 * 16 * 4 + per_pass * per_token, 1, s, p,
-             per_pass);
-  if (e != cudaSuccess) return e;
-  // CTAs of a cluster: as many as find an item for each warp, at most 8
-  const uint32_t items = met * ((p.f + DOWN_K - 1) / DOWN_K);
-  unsigned ranks = 1;
-  while (ranks < 8 && items > ranks * WARPS) ranks *= 2;
-  const uint32_t tiles = (p.d + Down<MX>::ROWS - 1) / Down<MX>::ROWS;
-  return launch(down_kernel<MX, VEC>, dim3(tiles * ranks), THREADS, Down<MX>::smem(p.m), ranks, s, p);
+  const uint32_t rounds = (p.d + 148u * 16u - 1u) / (148u * 16u), ctas = 148u * rounds;
+  p.down_rows = (p.d + ctas - 1u) / ctas;
+  const unsigned grid = (p.d + p.down_rows - 1u) / p.down_rows;
+  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch(down_kernel<MX, VEC, SVEC, 4>, grid, DownLayout<MX, 4>::total(p.m), s, (const MoeParams)p);
+  return launch(down_kernel<MX, VEC, SVEC, 3>, grid, DownLayout<MX, 3>::total(p.m), s, (const MoeParams)p);
 }
 
 }  // namespace
@@ -573,10 +641,10 @@ extern "C" int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64
   return m <= MAX_TOKENS && d <= 32768 && f <= 32768 && experts <= MAX_EXPERTS && topk <= MAX_TOPK;
 }
 
-// h [m * topk][f] fp32, then n, expert[], first[], pairs[]
+// h [m * topk][f] fp32, then n, expert[], first[], turn[], pairs[]
 extern "C" size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk) {
   const size_t pairs = (size_t)(m * topk), met = pairs < experts ? pairs : (size_t)experts;
-  return (pairs * (size_t)f + 1 + met + met + 1 + pairs) * 4;
+  return (pairs * (size_t)f + 1 + met + 2 * (met + 1) + pairs) * 4;
 }
 
 extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
@@ -594,15 +662,17 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.list.n = (int32_t *)(p.h + pairs * p.f);
   p.list.expert = p.list.n + 1;
   p.list.first = p.list.expert + met;
-  p.list.pairs = p.list.first + met + 1;
+  p.list.turn = p.list.first + met + 1;
+  p.list.pairs = p.list.turn + met + 1;
   cudaStream_t s = (cudaStream_t)stream;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(p.w1) | reinterpret_cast<uintptr_t>(p.w2);
   if (q->mx) {
-    // 16-byte loads of codes, 8-byte loads of scales: packed rows are always whole blocks of 16 bytes
-    const bool vec = (bases & 15u) == 0 && ((reinterpret_cast<uintptr_t>(p.s1) | reinterpret_cast<uintptr_t>(p.s2)) & 7u) == 0 &&
-                     (p.d + 31) / 32 % 8 == 0 && (p.f + 31) / 32 % 8 == 0;
-    return (int)(vec ? launch_moe<true, true>(p, s) : launch_moe<true, false>(p, s));
+    // packed rows are whole blocks of 16 bytes; the rows of scales start on 8 bytes if their lengths are multiples of 8
+    const bool vec = (bases & 15u) == 0, svec = ((reinterpret_cast<uintptr_t>(p.s1) | reinterpret_cast<uintptr_t>(p.s2)) & 7u) == 0 &&
+                                                (p.d + 31) / 32 % 8 == 0 && (p.f + 31) / 32 % 8 == 0;
+    if (vec && svec) return (int)launch_moe<true, true, true>(p, s);
+    return (int)(vec ? launch_moe<true, true, false>(p, s) : launch_moe<true, false, false>(p, s));
   }
   const bool vec = (bases & 15u) == 0 && p.d % 8 == 0 && p.f % 8 == 0;
-  return (int)(vec ? launch_moe<false, true>(p, s) : launch_moe<false, false>(p, s));
+  return (int)(vec ? launch_moe<false, true, false>(p, s) : launch_moe<false, false, false>(p, s));
 }

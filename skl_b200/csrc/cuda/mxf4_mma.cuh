@@ -27,11 +27,6 @@ namespace mxmma {
 
 constexpr int STEP = 256;  // elements of k that a warp takes at a time: two chunks, 128 bytes of each of its 16 rows
 
-// the E8M0 scale of byte b: 2^(b - 127); 0 is the subnormal 2^-127, 255 NaN
-__device__ __forceinline__ float e8m0(uint32_t b) {
-  return u2f(max(b << 23, 0x00400000u) | ((b + 1u) >> 8) << 22);
-}
-
 // 8 E2M1 codes of a word as 4 fp16 pairs
 __device__ __forceinline__ void e2m1_to_f16(uint32_t w, uint32_t (&r)[4]) {
   asm("{.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
@@ -46,50 +41,81 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The weights of one step as a lane holds them: blocks t and t + 4 of rows g and g + 8, and the 8 scale bytes of each row.
-struct Weights {
-  uint4 code[2][2];   // [row half][chunk]
-  uint2 scale[2];     // [row half]
+// Two E8M0 scale bytes as fp32 (0 is the subnormal 2^-127, 255 NaN): the hardware widens them to bf16 exactly.
+__device__ __forceinline__ void e8m0x2(uint32_t two, float &lo, float &hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  lo = u2f(r << 16);
+  hi = u2f(r & 0xFFFF0000u);
+}
+
+// A warp's ring of steps in shared memory, filled with cp.async so that loads in flight cost no registers: a slot holds the
+// 16-byte pieces of its 16 rows in the order of the lanes (lane l's pieces [row half][chunk] at (2 half + chunk) * 512 +
+// 16 l, written and read by the same lane without bank conflicts) and the 16 rows' 8 scale bytes of the step.  The experts'
+// layer uses the same rings for 16-bit weights, without scales.
+constexpr int CODE_BYTES = 4 * 512, SLOT_BYTES = CODE_BYTES + 128;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// How a lane addresses the 16 rows of a tile: rows g and g + 8 for the codes, row lane / 2 for the scales.  A row that does
+// not exist has null pointers; its codes count as zeros.
+struct TileRows {
+  const uint8_t *code[2];
+  const uint8_t *scale;
 };
 
-// How a warp addresses its 16 rows.
-struct RowPair {
-  const uint8_t *code[2];   // row g, row g + 8: first byte of the row
-  const uint8_t *scale[2];  // first scale byte
-};
+__device__ __forceinline__ void st_zero16(uint32_t at) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+}
 
-// VEC: 16-byte aligned packed rows and 8-byte aligned scale rows; otherwise single bytes.
-// Blocks behind the last one count as zeros with scale 1.
-template <bool VEC>
-__device__ __forceinline__ void load_step(Weights &w, const RowPair &rows, uint32_t step, uint32_t kblocks, int t) {
-  const uint32_t b0 = step * 8u;
+// Bytes [128 step, 128 step + 128) of a tile's 16 rows into a slot, and with SCALES the 8 scale bytes of each row.
+// `row_bytes`: length of a row (MX-FP4: 16 bytes to a block); what lies behind it, and rows that do not exist, are zeros with
+// scale 1.  VEC: rows start on 16 bytes and are whole units of 16; SVEC: scale rows start on 8 bytes.  Without them single
+// bytes are loaded, which are in place when the call returns.
+template <bool SCALES, bool VEC, bool SVEC>
+__device__ __forceinline__ void fill_slot(uint32_t slot, const TileRows &rows, uint32_t step, uint32_t row_bytes, int lane) {
+  const int t = lane & 3;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const uint32_t b = b0 + 4u * c + t;
-      w.code[h][c] = make_uint4(0u, 0u, 0u, 0u);
-      if (b < kblocks) {
-        const uint8_t *p = rows.code[h] + (size_t)b * 16;
+      const uint32_t b = step * 128u + 64u * c + 16u * t, dst = slot + (2 * h + c) * 512 + lane * 16;
+      if (rows.code[h] && b < row_bytes) {
+        const uint8_t *p = rows.code[h] + b;
         if (VEC) {
-          w.code[h][c] = ld_stream_v4(p);
+          cp_async16(dst, p);
         } else {
-          uint32_t q[4];
+          uint32_t q[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            q[i] = ld_u8(p + 4 * i) | ld_u8(p + 4 * i + 1) << 8 | ld_u8(p + 4 * i + 2) << 16 | ld_u8(p + 4 * i + 3) << 24;
-          w.code[h][c] = make_uint4(q[0], q[1], q[2], q[3]);
+          for (int i = 0; i < 16; ++i)
+            if (b + i < row_bytes) q[i >> 2] |= ld_u8(p + i) << (8 * (i & 3));
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
         }
+      } else {
+        st_zero16(dst);
       }
     }
-    if (VEC && b0 + 8u <= kblocks) {
-      w.scale[h] = ld_v2(rows.scale[h] + b0);
+  }
+  if (SCALES && (lane & 1) == 0) {
+    const uint32_t dst = slot + 4 * 512 + lane * 4, b0 = step * 8u, kblocks = row_bytes / 16u;
+    if (SVEC && rows.scale && b0 + 8u <= kblocks) {
+      cp_async8(dst, rows.scale + b0);
     } else {
       uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (b0 + i < kblocks) q[i >> 2] = (q[i >> 2] & ~(0xFFu << (8 * (i & 3)))) | ld_u8(rows.scale[h] + b0 + i) << (8 * (i & 3));
-      w.scale[h] = make_uint2(q[0], q[1]);
+        if (rows.scale && b0 + i < kblocks) q[i >> 2] = (q[i >> 2] & ~(0xFFu << (8 * (i & 3)))) | ld_u8(rows.scale + b0 + i) << (8 * (i & 3));
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(dst), "r"(q[0]), "r"(q[1]) : "memory");
     }
   }
 }
@@ -100,8 +126,9 @@ __device__ __forceinline__ void load_step(Weights &w, const RowPair &rows, uint3
 // y[group][row half]: the running sums of this lane's token (2 * group + t / 2), over blocks 2 (t % 2) and 2 (t % 2) + 1
 // of every chunk: the lanes t and t ^ 1 hold the two halves of a sum.
 template <int TG, bool FACTORS>
-__device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch,
-                                              uint32_t last, uint32_t zeros, int g, int t, float (&y)[TG][2]) {
+__device__ __forceinline__ void multiply_step(uint32_t slot, uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch,
+                                              uint32_t last, uint32_t zeros, int lane, float (&y)[TG][2]) {
+  const int g = lane >> 2, t = lane & 3;
   const bool mine = (g & 3) == t;
   uint32_t xrow[TG], frow[TG];
 #pragma unroll
@@ -109,13 +136,22 @@ __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint
     xrow[q] = mine ? x + min(2u * q + (uint32_t)(g >> 2), last) * x_pitch + t * 64u : zeros;
     frow[q] = f + min(2u * q + (uint32_t)(t >> 1), last) * f_pitch + (uint32_t)(t & 1) * 8u;
   }
+  uint32_t sc[2][2];  // [row half][chunk]: the scale bytes of the chunk's four blocks
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[h][0]), "=r"(sc[h][1]) : "r"(slot + 4 * 512 + (g + 8 * h) * 8));
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float acc[TG][4];
 #pragma unroll
     for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
-    const uint32_t lo[4] = {w.code[0][c].x, w.code[0][c].y, w.code[0][c].z, w.code[0][c].w};
-    const uint32_t hi[4] = {w.code[1][c].x, w.code[1][c].y, w.code[1][c].z, w.code[1][c].w};
+    uint32_t lo[4], hi[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3])
+                 : "r"(slot + c * 512 + lane * 16));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3])
+                 : "r"(slot + (2 + c) * 512 + lane * 16));
     const uint32_t skip = mine ? c * 256u : 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -134,11 +170,7 @@ __device__ __forceinline__ void multiply_step(const Weights &w, uint32_t x, uint
     }
     float s[2][2];  // [row half][block of this lane's pair]
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t word = (c ? w.scale[h].y : w.scale[h].x) >> (16 * (t & 1));
-      s[h][0] = e8m0(word & 0xFFu);
-      s[h][1] = e8m0((word >> 8) & 0xFFu);
-    }
+    for (int h = 0; h < 2; ++h) e8m0x2(sc[h][c] >> (16 * (t & 1)), s[h][0], s[h][1]);
 #pragma unroll
     for (int q = 0; q < TG; ++q) {
       float f0 = 1.0f, f1 = 1.0f;
