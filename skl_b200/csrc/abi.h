@@ -141,8 +141,8 @@ int skl_b200_launch_widen_mxf4(void *dst, int dst_type, int64_t rsd, const void 
 /* An fp16 matrix as the exact sum of two bf16 ones: dst rows of 2 * ld elements, [hi | lo], zeros behind column k (ld >= k) */
 int skl_b200_launch_split_f16(void *dst, uint32_t ld, const void *src, int64_t rs, uint32_t m, uint32_t k, void *stream);
 
-/* C = alpha * A W^T + beta * C, A m x k (ta = BF16 / F16, unit column stride), W n x k MX-FP4, for m <= 8 */
-int skl_b200_mxf4_skinny_supported(uint64_t m, uint64_t n, uint64_t k, int ta);
+/* C = alpha * A W^T + beta * C, A m x k (ta = BF16 / F16, unit column stride), W n x k MX-FP4, for m <= 4 */
+int skl_b200_mxf4_skinny_supported(uint64_t m, uint64_t n, uint64_t k);
 int skl_b200_launch_mxf4_skinny(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                 const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
                                 int64_t rsc, int static_b, void *stream);

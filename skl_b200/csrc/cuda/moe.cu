@@ -29,8 +29,10 @@ constexpr size_t MAX_SMEM = 226 * 1024;
 
 // The routed pairs (token * topk + j) sorted by expert: n experts met, in ascending order, expert[a] with the pairs
 // pairs[first[a]] .. pairs[first[a + 1] - 1], in token order; they are taken `per_pass` at a time, passes before expert a: turn[a].
+// token[], gate[]: of the pairs, in the same order (only in the workspace, for the second kernel).
 struct Lists {
-  int32_t *n, *expert, *first, *turn, *pairs;
+  int32_t *n, *expert, *first, *turn, *pairs, *token;
+  float *gate;
 };
 struct MoeParams {
   const float *logits;
@@ -58,10 +60,9 @@ struct Format {
   static constexpr uint32_t ITEM_SLOTS = ITEM / K;
   static __host__ __device__ uint32_t row_bytes(uint32_t cols) { return MX ? (cols + 31u) / 32u * 16u : cols * 2u; }
   static __host__ __device__ uint32_t steps(uint32_t cols) { return (cols + K - 1u) / K; }
-  // a token's activations in shared memory: fp16 and a factor per block, or bf16 with a pitch 64 bytes more than a multiple
-  // of 128, so that the eight rows of an mma operand are read without bank conflicts
-  static __host__ __device__ uint32_t x_pitch(uint32_t steps) { return MX ? steps * (K * 2u) : steps * (K * 2u) + 64u; }
-  static __host__ __device__ uint32_t f_pitch(uint32_t steps) { return MX ? steps * (K / 8u) : 0u; }
+  // a token's bf16 activations in shared memory: a pitch 64 bytes more than a multiple of 128, so that the rows of an mma
+  // operand are read without bank conflicts
+  static __host__ __device__ uint32_t x_pitch(uint32_t steps) { return steps * (K * 2u) + 64u; }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -179,7 +180,12 @@ __device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, b
     if (threadIdx.x == 0) *p.list.n = n;
     for (int32_t i = threadIdx.x; i < n; i += THREADS) p.list.expert[i] = out.expert[i];
     for (int32_t i = threadIdx.x; i <= n; i += THREADS) p.list.first[i] = out.first[i], p.list.turn[i] = out.turn[i];
-    for (int32_t i = threadIdx.x; i < out.first[n]; i += THREADS) p.list.pairs[i] = out.pairs[i];
+    for (int32_t i = threadIdx.x; i < out.first[n]; i += THREADS) {
+      const int32_t pair = out.pairs[i];
+      p.list.pairs[i] = pair;
+      p.list.token[i] = pair / (int32_t)p.topk;
+      p.list.gate[i] = p.gates[pair];  // written by this CTA, before a barrier
+    }
   }
 }
 
@@ -226,49 +232,82 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
 constexpr uint32_t UP_DEPTH = 4;   // slots of a ring
 constexpr uint32_t UP_ROUND = 4;   // tiles of a warp between two barriers
 
-// Shared memory: 64 bytes of zeros | rings (before them, for a moment, the routing's scratch) | x and factors of a pass |
-// sums [2][round][warps along d][PASS][16] | lists
+// Shared memory: rings (before them, for a moment, the routing's scratch) | 16-bit weights: x of a pass, bf16 [tokens][pitch]
+// | sums [2][round][warps along d][PASS][16] | lists
 template <bool MX>
 struct UpLayout {
-  uint32_t rings, x, f, sums, sums_half, lists, total;
+  uint32_t x, sums, sums_half, lists, total;
   __host__ __device__ UpLayout(const MoeParams &p) {
     using F = Format<MX>;
     const uint32_t steps = F::steps(p.d), pairs = p.m * p.topk;
     const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (WARPS * p.experts + pairs + p.experts) * 4u;
-    rings = 64u;
-    x = rings + ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
-    f = x + p.per_pass * F::x_pitch(steps);
-    sums = f + p.per_pass * F::f_pitch(steps);
+    x = ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
+    sums = x + (MX ? 0u : p.per_pass * F::x_pitch(steps));
     sums_half = UP_ROUND * WARPS * PASS * 16u;
     lists = sums + 2u * sums_half * 4u;
     total = lists + (1u + p.met + 2u * (p.met + 1u) + pairs) * 4u;
   }
 };
 
-// One tile of a warp, all its steps: sums[token][16] are this warp's part.  `fill` loads the next slot of the ring.
-template <int TG, typename Fill>
-__device__ __forceinline__ void up_tile_mx(uint32_t ring, uint32_t &slot, uint32_t first, uint32_t by, uint32_t steps, uint32_t x,
-                                           uint32_t x_pitch, uint32_t f, uint32_t f_pitch, uint32_t last, uint32_t zeros, int lane,
-                                           float *sums, Fill &fill) {
-  const int g = lane >> 2, t = lane & 3;
-  float y[TG][2];
-#pragma unroll
-  for (int q = 0; q < TG; ++q) y[q][0] = y[q][1] = 0.0f;
-  for (uint32_t step = first; step < steps; step += by) {
-    cp_wait<UP_DEPTH - 2>();
-    __syncwarp();  // the slot's scales came through other lanes, and the slot filled next has been read by all
-    fill();
-    multiply_step<TG, true>(ring + slot * SLOT_BYTES, x + step * (STEP * 2), x_pitch, f + step * (STEP / 8), f_pitch, last, zeros,
-                            lane, y);
-    slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
+// This CTA's run of tiles [u0, u1), tile = pass over an expert * tiles of an expert + tile.  It is taken in rounds that do not
+// leave a pass, of UP_ROUND tiles of each group of warps; 4-bit weights: in a round a warp goes through its steps and for
+// each through its tiles, so that its activations stay in registers; 16-bit weights: through its tiles and for each through
+// its steps, so that the sums do.  The cursor names the warp's next item in that order, for the loads that run ahead.
+template <bool MX>
+struct Cursor {
+  uint32_t r0, r1, step, v;
+  __device__ __forceinline__ void round(const uint32_t start, uint32_t u0, uint32_t u1, uint32_t tiles, uint32_t TW, uint32_t tw, uint32_t kw) {
+    r0 = start;
+    r1 = min(min(u1, r0 + UP_ROUND * TW), (r0 / tiles + 1u) * tiles);
+    v = r0 + (tw + TW - (r0 - u0) % TW) % TW;
+    step = kw;
   }
+  __device__ __forceinline__ void next(uint32_t u0, uint32_t u1, uint32_t tiles, uint32_t steps, uint32_t KW, uint32_t TW, uint32_t kw, uint32_t tw) {
+    if (MX) {
+      v += TW;
+      if (v < r1) return;
+      v = r0 + (tw + TW - (r0 - u0) % TW) % TW;
+      step += KW;
+      if (step < steps) return;
+    } else {
+      step += KW;
+      if (step < steps) return;
+      step = kw;
+      v += TW;
+      if (v < r1) return;
+    }
+    do round(r1, u0, u1, tiles, TW, tw, kw);
+    while (r0 < u1 && v >= r1);
+  }
+};
+
+template <int TG>
+__device__ __forceinline__ void up_columns(const MoeParams &p, const int32_t *pairs, uint32_t cnt, uint32_t step, int lane, Columns (&x)[TG]) {
+  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int q = 0; q < TG; ++q) {
+    const uint32_t j = 2u * q + (uint32_t)(g >> 2);
+    float back[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      y[q][h] += __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
-      if ((t & 1) == 0) sums[(2 * q + (t >> 1)) * 16 + g + 8 * h] = y[q][h];
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t k0 = step * STEP + 128u * c + 32u * t;
+      if ((g & 3) == t && j < cnt && k0 < p.d) {
+        const uint16_t *row = p.x + (int64_t)((uint32_t)pairs[j] / p.topk) * p.rsx;
+        float e[32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[4];
+          load_x8(w, row, k0 + 8u * i, p.d, p.x_vec);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) e[8 * i + 2 * h] = dec_bf16(w[h] & 0xFFFFu), e[8 * i + 2 * h + 1] = u2f(w[h] & 0xFFFF0000u);
+        }
+        pack_block(x[q], c, e, back[c]);
+      } else {
+        no_block(x[q], c, back[c]);
+      }
     }
+    __syncwarp();
+    spread_factors(x[q], back, lane);
   }
 }
 
@@ -279,8 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const UpLayout<MX> at(p);
   const uint32_t steps = F::steps(p.d), row_bytes = F::row_bytes(p.d), kblocks = (p.d + 31u) / 32u, tiles = (p.f + 7u) / 8u;
-  const uint32_t x_pitch = F::x_pitch(steps), f_pitch = F::f_pitch(steps);
-  const uint32_t zeros = smem_addr(smem), x = zeros + at.x, f = zeros + at.f, ring = zeros + at.rings + warp * (UP_DEPTH * F::SLOT);
+  const uint32_t x = smem_addr(smem) + at.x, x_pitch = F::x_pitch(steps), ring = smem_addr(smem) + warp * (UP_DEPTH * F::SLOT);
   float *sums = reinterpret_cast<float *>(smem + at.sums);
   Lists list;
   list.n = reinterpret_cast<int32_t *>(smem + at.lists);
@@ -288,133 +326,162 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   list.first = list.expert + p.met;
   list.turn = list.first + p.met + 1;
   list.pairs = list.turn + p.met + 1;
-  if (threadIdx.x < 16) reinterpret_cast<uint32_t *>(smem)[threadIdx.x] = 0u;
 
   dep_wait();
-  route(p, reinterpret_cast<uint32_t *>(smem + at.rings), list, blockIdx.x == 0);
+  route(p, reinterpret_cast<uint32_t *>(smem), list, blockIdx.x == 0);
   const int32_t n = *list.n;
   const uint64_t total = (uint64_t)list.turn[n] * tiles;  // every pass over an expert counts
   const uint32_t u0 = (uint32_t)(total * blockIdx.x / gridDim.x), u1 = (uint32_t)(total * (blockIdx.x + 1) / gridDim.x);
   __syncthreads();  // the routing's scratch becomes the rings
 
-  // this warp's items: steps kw, kw + KW, ... of tiles u0 + tw, u0 + tw + TW, ...
   const uint32_t KW = p.k_warps, TW = WARPS / KW, kw = warp % KW, tw = warp / KW;
   TileRows rows;
   int32_t aim_a = 0;
-  auto aim = [&](uint32_t u) {
-    const uint32_t turn = u / tiles, feature0 = (u - turn * tiles) * 8u;
-    while ((int32_t)turn >= list.turn[aim_a + 1]) ++aim_a;
-    const uint64_t base = (uint64_t)list.expert[aim_a] * 2u * p.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      rows.code[h] = feature0 + g < p.f ? p.w1 + (base + (h ? p.f : 0u) + feature0 + g) * row_bytes : nullptr;
-    if (MX) {
-      const uint32_t r = lane >> 1;
-      rows.scale = feature0 + (r & 7u) < p.f ? p.s1 + (base + (r >= 8u ? p.f : 0u) + feature0 + (r & 7u)) * kblocks : nullptr;
-    }
+  // a row that does not exist may lie outside the matrix, its pointer is never followed
+  const uint64_t tile_by = (uint64_t)(8u * TW) * row_bytes, up_by = (uint64_t)p.f * row_bytes;
+  const uint32_t srow = lane >> 1;
+  uint32_t feature0 = 0;
+  auto mark = [&]() {
+    rows.has[0] = rows.has[1] = feature0 + g < p.f;
+    if (MX) rows.has_scale = feature0 + (srow & 7u) < p.f;
   };
-  uint32_t fill_u = u0 + tw, fill_step = kw, fill_at = 0;
+  auto aim = [&](uint32_t u) {
+    const uint32_t turn = u / tiles;
+    feature0 = (u - turn * tiles) * 8u;
+    while ((int32_t)turn >= list.turn[aim_a + 1]) ++aim_a;
+    const uint64_t base = (uint64_t)list.expert[aim_a] * 2u * p.f + feature0;
+    rows.code[0] = p.w1 + (base + g) * row_bytes + 16 * t;
+    rows.code[1] = rows.code[0] + up_by;
+    if (MX) rows.scale = p.s1 + (base + (srow >= 8u ? p.f : 0u) + (srow & 7u)) * kblocks;
+    mark();
+  };
+  Cursor<MX> ahead = {};
+  uint32_t fill_at = 0;
   auto fill = [&]() {
-    if (fill_u < u1) {
-      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, fill_step, row_bytes, lane);
-      fill_step += KW;
-      if (fill_step >= steps) {
-        fill_step = kw;
-        fill_u += TW;
-        if (fill_u < u1) aim(fill_u);
+    if (ahead.r0 < u1) {
+      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, ahead.step, row_bytes, lane);
+      const uint32_t v = ahead.v, r0 = ahead.r0;
+      ahead.next(u0, u1, tiles, steps, KW, TW, kw, tw);
+      if (ahead.v != v) {
+        if (ahead.r0 == r0 && ahead.v > v) {  // the group's next tile of the same expert
+          rows.code[0] += tile_by, rows.code[1] += tile_by, feature0 += 8u * TW;
+          if (MX) rows.scale += (uint64_t)(8u * TW) * kblocks;
+          mark();
+        } else if (ahead.r0 < u1) {
+          aim(ahead.v);
+        }
       }
     }
     cp_commit();
     fill_at = fill_at + 1 == UP_DEPTH ? 0 : fill_at + 1;
   };
-  if (fill_u < u1) aim(fill_u);
+  ahead.round(u0, u0, u1, tiles, TW, tw, kw);
+  while (ahead.r0 < u1 && ahead.v >= ahead.r1) ahead.round(ahead.r1, u0, u1, tiles, TW, tw, kw);
+  if (ahead.r0 < u1) aim(ahead.v);
 #pragma unroll
   for (uint32_t i = 0; i < UP_DEPTH - 1; ++i) fill();
 
   uint32_t slot = 0, half = 0;
   int32_t a = 0;
-  for (uint32_t u = u0; u < u1;) {  // a segment: this CTA's tiles of one pass over one expert
-    const uint32_t turn = u / tiles, seg_end = (uint32_t)min((uint64_t)u1, (uint64_t)(turn + 1u) * tiles);
+  uint32_t held = 0xFFFFFFFFu;  // the pass whose x is at hand
+  Columns cols[2];
+  for (uint32_t r0 = u0; r0 < u1;) {
+    Cursor<MX> now;
+    now.round(r0, u0, u1, tiles, TW, tw, kw);
+    const uint32_t r1 = now.r1, turn = r0 / tiles;
     while ((int32_t)turn >= list.turn[a + 1]) ++a;
     const uint32_t pair0 = (uint32_t)list.first[a] + (turn - (uint32_t)list.turn[a]) * p.per_pass;
     const uint32_t cnt = min(p.per_pass, (uint32_t)list.first[a + 1] - pair0);
-    // the tokens' activations (the last segment's were read before the barrier of its last round); four lanes share a block
-    const uint32_t groups = steps * (F::K / 8u), all = cnt * groups;
-    for (uint32_t i0 = 0; i0 < all; i0 += THREADS) {
-      const uint32_t i = i0 + threadIdx.x;
-      const bool in = i < all;
-      const uint32_t j = in ? i / groups : 0u, gr = in ? i - j * groups : 0u;
-      uint32_t v[4];
-      const uint32_t tok = (uint32_t)list.pairs[pair0 + j] / p.topk;
-      load_x8(v, p.x + (int64_t)tok * p.rsx, gr * 8u, in ? p.d : 0u, p.x_vec);
-      if (MX) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) top = max(top, max(v[q] << 16 & 0x7FFFFFFFu, v[q] & 0x7FFF0000u));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        float back;
-        const float factor = block_factor(top, back);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = pack_f16x2_no_nan(dec_bf16(v[q] & 0xFFFFu) * factor, u2f(v[q] & 0xFFFF0000u) * factor);
-        if (in && (gr & 3u) == 0u) asm volatile("st.shared.f32 [%0], %1;" ::"r"(f + j * f_pitch + gr), "f"(back) : "memory");
+    float *round = sums + half * at.sums_half;
+    if (MX) {
+      if (now.v < r1) {
+        for (uint32_t step = kw; step < steps; step += KW) {
+          // the activations of this step, unless they are the same as in the round before
+          const bool fresh = held != turn || steps > KW;
+          if (cnt <= 2) {
+            Columns(&one)[1] = reinterpret_cast<Columns(&)[1]>(cols);
+            if (fresh) up_columns<1>(p, list.pairs + pair0, cnt, step, lane, one);
+            for (uint32_t v = now.v; v < r1; v += TW) {
+              float y[1][2] = {{0.0f, 0.0f}};
+              cp_wait<UP_DEPTH - 2>();
+              __syncwarp();  // the slot's scales came through other lanes, and the slot filled next has been read by all
+              fill();
+              multiply_step<1>(ring + slot * F::SLOT, one, lane, y);
+              slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
+              keep_sums<1>(round + ((v - r0) * KW + kw) * (PASS * 16), y, step == kw, lane);
+            }
+          } else {
+            if (fresh) up_columns<2>(p, list.pairs + pair0, cnt, step, lane, cols);
+            for (uint32_t v = now.v; v < r1; v += TW) {
+              float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+              cp_wait<UP_DEPTH - 2>();
+              __syncwarp();
+              fill();
+              multiply_step<2>(ring + slot * F::SLOT, cols, lane, y);
+              slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
+              keep_sums<2>(round + ((v - r0) * KW + kw) * (PASS * 16), y, step == kw, lane);
+            }
+          }
+        }
+        held = turn;
       }
-      if (in) st_shared_v4(x + j * x_pitch + gr * 16u, v[0], v[1], v[2], v[3]);
+    } else {
+      if (held != turn) {  // x of the pass (the one before was last read before the barrier of its last round)
+        const uint32_t groups = steps * (F::K / 8u), all = cnt * groups;
+        for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
+          const uint32_t j = i / groups, gr = i - j * groups;
+          uint32_t v[4];
+          load_x8(v, p.x + (int64_t)((uint32_t)list.pairs[pair0 + j] / p.topk) * p.rsx, gr * 8u, p.d, p.x_vec);
+          st_shared_v4(x + j * x_pitch + gr * 16u, v[0], v[1], v[2], v[3]);
+        }
+        held = turn;
+        __syncthreads();
+      }
+      for (uint32_t v = now.v; v < r1; v += TW) {
+        float *own = round + ((v - r0) * KW + kw) * (PASS * 16);
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t step = kw; step < steps; step += KW) {
+          cp_wait<UP_DEPTH - 2>();
+          __syncwarp();
+          fill();
+          multiply_wide(ring + slot * F::SLOT, x + step * (F::K * 2u), x_pitch, cnt - 1u, lane, acc);
+          slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
+        }
+        if (t < 2) {  // columns 2 t and 2 t + 1 of the four tokens
+#pragma unroll
+          for (int q = 0; q < 4; ++q) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
+        }
+      }
     }
     __syncthreads();
-    for (uint32_t r0 = u; r0 < seg_end; r0 += UP_ROUND * TW) {
-      const uint32_t r1 = min(seg_end, r0 + UP_ROUND * TW);
-      float *round = sums + half * at.sums_half;
-      for (uint32_t v = r0 + (tw + TW - (r0 - u0) % TW) % TW; v < r1; v += TW) {
-        float *own = round + ((v - r0) * KW + kw) * (PASS * 16);
-        if (MX) {
-          if (cnt <= 2) up_tile_mx<1>(ring, slot, kw, KW, steps, x, x_pitch, f, f_pitch, cnt - 1u, zeros, lane, own, fill);
-          else up_tile_mx<2>(ring, slot, kw, KW, steps, x, x_pitch, f, f_pitch, cnt - 1u, zeros, lane, own, fill);
-        } else {
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (uint32_t step = kw; step < steps; step += KW) {
-            cp_wait<UP_DEPTH - 2>();
-            __syncwarp();
-            fill();
-            multiply_wide(ring + slot * F::SLOT, x + step * (F::K * 2u), x_pitch, cnt - 1u, lane, acc);
-            slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
-          }
-          if (t < 2) {  // columns 2 t and 2 t + 1 of the four tokens
-#pragma unroll
-            for (int q = 0; q < 4; ++q) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
-          }
+    // h = silu(gate) * up; the other half of the sums is written meanwhile
+    const uint32_t outs = (r1 - r0) * 8u * cnt;
+    for (uint32_t i = threadIdx.x; i < outs; i += THREADS) {
+      const uint32_t c = i % (8u * (r1 - r0)), j = i / (8u * (r1 - r0));
+      const uint32_t feature = (r0 - turn * tiles) * 8u + c;
+      if (feature < p.f) {
+        const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
+        float gate = 0.0f, up = 0.0f;
+        for (uint32_t q = 0; q < KW; ++q) {
+          gate += s[q * (PASS * 16)];
+          up += s[q * (PASS * 16) + 8];
         }
+        p.h[(uint64_t)list.pairs[pair0 + j] * p.f + feature] = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
       }
-      __syncthreads();
-      // h = silu(gate) * up; the other half of the sums is written meanwhile
-      const uint32_t outs = (r1 - r0) * 8u * cnt;
-      for (uint32_t i = threadIdx.x; i < outs; i += THREADS) {
-        const uint32_t c = i % (8u * (r1 - r0)), j = i / (8u * (r1 - r0));
-        const uint32_t feature = (r0 - turn * tiles) * 8u + c;
-        if (feature < p.f) {
-          const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
-          float gate = 0.0f, up = 0.0f;
-          for (uint32_t q = 0; q < KW; ++q) {
-            gate += s[q * (PASS * 16)];
-            up += s[q * (PASS * 16) + 8];
-          }
-          p.h[(uint64_t)list.pairs[pair0 + j] * p.f + feature] = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
-        }
-      }
-      half ^= 1u;
     }
-    u = seg_end;
+    half ^= 1u;
+    r0 = r1;
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------- down
-// Shared memory: 64 bytes of zeros | rings | per warp: h of an item (4-bit: fp16 [4][256] and factors [4][8]; 16-bit: bf16, the
+// Shared memory: rings | per warp: h of an item (4-bit: fp16 [4][256] and factors [4][8]; 16-bit: bf16, the
 // first parts of four tokens, then the second parts, [8][128] with a pitch of 320 bytes) | per warp: sums [m][16]
 template <bool MX, int DEPTH>
 struct DownLayout {
   static constexpr uint32_t PITCH = MX ? 512 : 320;
   static constexpr uint32_t STAGE = MX ? PASS * PITCH + PASS * 32 : 2 * PASS * PITCH;
-  static constexpr uint32_t RINGS = 64, STAGES = RINGS + WARPS * DEPTH * Format<MX>::SLOT, SUMS = STAGES + WARPS * STAGE;
+  static constexpr uint32_t STAGES = WARPS * DEPTH * Format<MX>::SLOT, SUMS = STAGES + WARPS * STAGE;
   static size_t total(uint32_t m) { return SUMS + (size_t)WARPS * m * 16 * 4; }
 };
 
@@ -427,30 +494,34 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t row0 = blockIdx.x * p.down_rows, nrows = min(p.down_rows, p.d - row0);
   const uint32_t row_bytes = F::row_bytes(p.f), kblocks = (p.f + 31u) / 32u;
-  const uint32_t zeros = smem_addr(smem), ring = zeros + L::RINGS + warp * (DEPTH * F::SLOT);
-  const uint32_t stage = zeros + L::STAGES + warp * L::STAGE, factors = stage + PASS * L::PITCH;
+  const uint32_t ring = smem_addr(smem) + warp * (DEPTH * F::SLOT);
+  const uint32_t stage = smem_addr(smem) + L::STAGES + warp * L::STAGE, factors = stage + PASS * L::PITCH;
   float *sums = reinterpret_cast<float *>(smem + L::SUMS), *own = sums + (size_t)warp * p.m * 16;
-  if (threadIdx.x < 16) reinterpret_cast<uint32_t *>(smem)[threadIdx.x] = 0u;
   for (uint32_t i = lane; i < p.m * 16u; i += 32u) own[i] = 0.0f;
-  __syncthreads();
+  __syncwarp();
   dep_wait();
 
   const uint32_t parts = (p.f + F::ITEM - 1u) / F::ITEM, items = (uint32_t)*p.list.n * parts;
+  // a row that does not exist may lie outside the matrix, its pointer is never followed
   TileRows rows;
-  auto aim = [&](uint32_t item) {
-    const uint64_t base = (uint64_t)p.list.expert[item / parts] * p.d + row0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) rows.code[h] = g + 8u * h < nrows ? p.w2 + (base + g + 8u * h) * row_bytes : nullptr;
-    if (MX) rows.scale = (uint32_t)(lane >> 1) < nrows ? p.s2 + (base + (lane >> 1)) * kblocks : nullptr;
+  rows.has[0] = g < nrows, rows.has[1] = g + 8u < nrows, rows.has_scale = (uint32_t)(lane >> 1) < nrows;
+  const uint64_t expert_by = (uint64_t)p.d * row_bytes, first_row = (uint64_t)(row0 + g) * row_bytes + 16 * t;
+  auto aim = [&](uint32_t a) {
+    const uint64_t e = (uint64_t)p.list.expert[a];
+    rows.code[0] = p.w2 + e * expert_by + first_row;
+    rows.code[1] = rows.code[0] + 8u * row_bytes;
+    if (MX) rows.scale = p.s2 + (e * p.d + row0 + (lane >> 1)) * kblocks;
   };
-  uint32_t fill_item = warp, fill_sub = 0, fill_at = 0;
+  const uint32_t by_a = WARPS / parts, by_part = WARPS % parts;  // an item ahead: WARPS parts further
+  uint32_t fill_item = warp, fill_a = warp / parts, fill_part = warp % parts, fill_sub = 0, fill_at = 0;
   auto fill = [&]() {
     if (fill_item < items) {
-      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, (fill_item % parts) * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
+      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, fill_part * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
       if (++fill_sub == F::ITEM_SLOTS) {
         fill_sub = 0;
-        fill_item += WARPS;
-        if (fill_item < items) aim(fill_item);
+        fill_item += WARPS, fill_a += by_a, fill_part += by_part;
+        if (fill_part >= parts) fill_part -= parts, ++fill_a;
+        if (fill_item < items) aim(fill_a);
       }
     }
     cp_commit();
@@ -509,19 +580,41 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
       }
     }
   };
-  if (fill_item < items) aim(fill_item);
+  // tokens 2 q and 2 q + 1 of the staged h as the columns of a group (4-bit weights)
+  auto columns = [&](Columns &c, int q, uint32_t cnt) {
+    const uint32_t j = 2u * q + (uint32_t)(g >> 2);
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t *w = c.v[ch] + 4 * i;
+        w[0] = w[1] = w[2] = w[3] = 0u;
+        if ((g & 3) == t && j < cnt)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(stage + j * L::PITCH + ch * 256u + t * 64u + 16u * i));
+      }
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                   : "=f"(c.factor[ch][0]), "=f"(c.factor[ch][1])
+                   : "r"(factors + min(2u * q + (uint32_t)(t >> 1), cnt - 1u) * 32u + ch * 16u + (uint32_t)(t & 1) * 8u));
+    }
+  };
+  if (fill_item < items) aim(fill_a);
 #pragma unroll
   for (int i = 0; i < DEPTH - 1; ++i) fill();
 
   float v[PASS][PER];
+  uint32_t a = warp / parts, part = warp % parts, slot = 0;
+  int32_t first = 0, last = 0;
   if ((uint32_t)warp < items) {
-    const uint32_t e = warp / parts;
-    load_h(v, p.list.first[e], p.list.first[e + 1], (warp % parts) * F::ITEM);
+    first = p.list.first[a], last = p.list.first[a + 1];
+    load_h(v, first, last, part * F::ITEM);
   }
-  uint32_t slot = 0;
   for (uint32_t item = warp; item < items; item += WARPS) {
-    const uint32_t a = item / parts, k0 = (item - a * parts) * F::ITEM, next = item + WARPS;
-    const int32_t first = p.list.first[a], last = p.list.first[a + 1];
+    uint32_t next_a = a + by_a, next_part = part + by_part;
+    if (next_part >= parts) next_part -= parts, ++next_a;
+    const bool more = item + WARPS < items;
+    const int32_t next_first = more ? p.list.first[next_a] : 0, next_last = more ? p.list.first[next_a + 1] : 0;
 #pragma unroll
     for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) {
       cp_wait<DEPTH - 1 - (int)F::ITEM_SLOTS>();  // all slots of the item
@@ -529,19 +622,24 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
     }
     for (int32_t at = first; at < last; at += PASS) {
       const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)PASS);
-      if (at != first) load_h(v, at, last, k0);
+      if (at != first) load_h(v, at, last, part * F::ITEM);
       __syncwarp();  // the h before has been read
       store_h(v, cnt);
-      if (at + PASS >= last && next < items) load_h(v, p.list.first[next / parts], p.list.first[next / parts + 1], (next % parts) * F::ITEM);
+      if (at + PASS >= last && more) load_h(v, next_first, next_last, next_part * F::ITEM);
       __syncwarp();
       if (MX) {
         float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         if (cnt <= 2) {
+          Columns x[1];
           float y1[1][2] = {{0.0f, 0.0f}};
-          multiply_step<1, true>(ring + slot * F::SLOT, stage, L::PITCH, factors, 32, cnt - 1u, zeros, lane, y1);
+          columns(x[0], 0, cnt);
+          multiply_step<1>(ring + slot * F::SLOT, x, lane, y1);
           y[0][0] = y1[0][0], y[0][1] = y1[0][1];
         } else {
-          multiply_step<2, true>(ring + slot * F::SLOT, stage, L::PITCH, factors, 32, cnt - 1u, zeros, lane, y);
+          Columns x[2];
+          columns(x[0], 0, cnt);
+          columns(x[1], 1, cnt);
+          multiply_step<2>(ring + slot * F::SLOT, x, lane, y);
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -550,9 +648,8 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
             const float s = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
             const uint32_t j = 2u * q + (uint32_t)(t >> 1);
             if ((t & 1) == 0 && j < cnt) {
-              const uint32_t pair = (uint32_t)p.list.pairs[at + j];
-              float *o = own + (pair / p.topk) * 16 + g + 8 * h;
-              *o = __fmaf_rn(p.gates[pair], s, *o);
+              float *o = own + p.list.token[at + j] * 16 + g + 8 * h;
+              *o = __fmaf_rn(p.list.gate[at + j], s, *o);
             }
           }
         }
@@ -568,9 +665,8 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
           const float s = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
           const uint32_t j = 2u * t + (q & 1);
           if (t < 2 && j < cnt) {
-            const uint32_t pair = (uint32_t)p.list.pairs[at + j];
-            float *o = own + (pair / p.topk) * 16 + g + 8 * (q >> 1);
-            *o = __fmaf_rn(p.gates[pair], s, *o);
+            float *o = own + p.list.token[at + j] * 16 + g + 8 * (q >> 1);
+            *o = __fmaf_rn(p.list.gate[at + j], s, *o);
           }
         }
       }
@@ -580,6 +676,7 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
     for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) fill();
     slot += F::ITEM_SLOTS;
     if (slot >= DEPTH) slot -= DEPTH;
+    a = next_a, part = next_part, first = next_first, last = next_last;
   }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < p.m * 16u; i += THREADS) {
@@ -591,10 +688,17 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
   }
 }
 
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), unsigned grid, size_t smem, cudaStream_t s, A... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM);
+template <auto KERNEL>
+cudaError_t launch(unsigned grid, size_t smem, cudaStream_t s, const MoeParams &p) {
+  static bool ready[64];  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (!ready[dev & 63]) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM);
+    if (e != cudaSuccess) return e;
+    ready[dev & 63] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(grid);
@@ -606,7 +710,7 @@ cudaError_t launch(void (*kernel)(P...), unsigned grid, size_t smem, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   SKLB_COUNT_LAUNCH();
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return cudaLaunchKernelEx(&cfg, KERNEL, p);
 }
 
 template <bool MX, bool VEC, bool SVEC>
@@ -623,13 +727,13 @@ cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
   if (up.total > MAX_SMEM) return cudaErrorInvalidConfiguration;
   // an SM has room for one CTA; never more CTAs than tiles that can exist
   const uint64_t most = (uint64_t)p.met * ((p.m + p.per_pass - 1) / p.per_pass) * ((p.f + 7) / 8);
-  cudaError_t e = launch(up_kernel<MX, VEC, SVEC>, (unsigned)(most < 148 ? most : 148), up.total, s, (const MoeParams)p);
+  cudaError_t e = launch<up_kernel<MX, VEC, SVEC>>((unsigned)(most < 148 ? most : 148), up.total, s, p);
   if (e != cudaSuccess) return e;
   const uint32_t rounds = (p.d + 148u * 16u - 1u) / (148u * 16u), ctas = 148u * rounds;
   p.down_rows = (p.d + ctas - 1u) / ctas;
   const unsigned grid = (p.d + p.down_rows - 1u) / p.down_rows;
-  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch(down_kernel<MX, VEC, SVEC, 4>, grid, DownLayout<MX, 4>::total(p.m), s, (const MoeParams)p);
-  return launch(down_kernel<MX, VEC, SVEC, 3>, grid, DownLayout<MX, 3>::total(p.m), s, (const MoeParams)p);
+  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch<down_kernel<MX, VEC, SVEC, 4>>(grid, DownLayout<MX, 4>::total(p.m), s, p);
+  return launch<down_kernel<MX, VEC, SVEC, 3>>(grid, DownLayout<MX, 3>::total(p.m), s, p);
 }
 
 }  // namespace
@@ -641,10 +745,10 @@ extern "C" int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64
   return m <= MAX_TOKENS && d <= 32768 && f <= 32768 && experts <= MAX_EXPERTS && topk <= MAX_TOPK;
 }
 
-// h [m * topk][f] fp32, then n, expert[], first[], turn[], pairs[]
+// h [m * topk][f] fp32, then n, expert[], first[], turn[], pairs[], token[], gate[]
 extern "C" size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk) {
   const size_t pairs = (size_t)(m * topk), met = pairs < experts ? pairs : (size_t)experts;
-  return (pairs * (size_t)f + 1 + met + 2 * (met + 1) + pairs) * 4;
+  return (pairs * (size_t)f + 1 + met + 2 * (met + 1) + 3 * pairs) * 4;
 }
 
 extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
@@ -664,6 +768,8 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.list.first = p.list.expert + met;
   p.list.turn = p.list.first + met + 1;
   p.list.pairs = p.list.turn + met + 1;
+  p.list.token = p.list.pairs + pairs;
+  p.list.gate = (float *)(p.list.token + pairs);
   cudaStream_t s = (cudaStream_t)stream;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(p.w1) | reinterpret_cast<uintptr_t>(p.w2);
   if (q->mx) {

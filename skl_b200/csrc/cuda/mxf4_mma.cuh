@@ -8,7 +8,8 @@
 // token's activations in the k positions of lane b and zeros elsewhere.  After the eight mmas of a chunk the accumulator of
 // (row, 4 * token + b) is the unscaled sum of block b, which is multiplied by the weight block's and the activation block's
 // scale and added to the running fp32 sum: 4 multiply-adds for 64 weights per lane.  A group of columns thus serves two
-// tokens.  Measured: the conversion with the mma behind it runs at 22 T elements/s on the whole chip, against 12 T that HBM
+// tokens; it stays in registers while the warp goes through its tiles (read from shared memory for each, it kept the
+// shared-memory pipe busier than the weights did).  Measured: the conversion with the mma behind it runs at 22 T elements/s on the whole chip, against 12 T that HBM
 // delivers (17/32 byte per element at 6.4 TB/s); placing the bits of bf16 with integer instructions reached 12 T.
 //
 // fp16 activations are used as they are.  bf16 activations are brought into fp16's range with one power of two per block of
@@ -55,135 +56,70 @@ __device__ __forceinline__ void e8m0x2(uint32_t two, float &lo, float &hi) {
 // layer uses the same rings for 16-bit weights, without scales.
 constexpr int CODE_BYTES = 4 * 512, SLOT_BYTES = CODE_BYTES + 128;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// How a lane addresses the 16 rows of a tile: rows g and g + 8 for the codes, row lane / 2 for the scales.  A row that does
-// not exist has null pointers; its codes count as zeros.
+// `bytes`: how much of the 16 (8) is read, the rest is zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// How a lane addresses the 16 rows of a tile: rows g and g + 8 for the codes (from byte 16 t on), row lane / 2 for the scales;
+// a row that does not exist (has[] false) counts as zeros and its pointer is not followed.
 struct TileRows {
   const uint8_t *code[2];
   const uint8_t *scale;
+  bool has[2], has_scale;
 };
 
-__device__ __forceinline__ void st_zero16(uint32_t at) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-}
-
 // Bytes [128 step, 128 step + 128) of a tile's 16 rows into a slot, and with SCALES the 8 scale bytes of each row.
-// `row_bytes`: length of a row (MX-FP4: 16 bytes to a block); what lies behind it, and rows that do not exist, are zeros with
-// scale 1.  VEC: rows start on 16 bytes and are whole units of 16; SVEC: scale rows start on 8 bytes.  Without them single
-// bytes are loaded, which are in place when the call returns.
+// `row_bytes`: length of a row (MX-FP4: 16 bytes to a block); what lies behind it counts as zeros (blocks that do not exist
+// and rows that do not exist have codes of zero and a scale that is finite).  VEC: rows start on 16 bytes and are whole units
+// of 16; SVEC: scale rows start on 8 bytes.  Without them single bytes are loaded, which are in place when the call returns.
 template <bool SCALES, bool VEC, bool SVEC>
 __device__ __forceinline__ void fill_slot(uint32_t slot, const TileRows &rows, uint32_t step, uint32_t row_bytes, int lane) {
-  const int t = lane & 3;
+  const uint32_t at = step * 128u, dst = slot + lane * 16;
+  const bool whole = at + 128u <= row_bytes;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    const uint8_t *p = rows.code[h] + at;
+    if (VEC && whole) {  // the usual case first: a dozen instructions for a slot
+      const uint32_t bytes = rows.has[h] ? 16u : 0u;
+      cp_async16(dst + 2 * h * 512, p, bytes);
+      cp_async16(dst + 2 * h * 512 + 512, p + 64, bytes);
+    } else {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const uint32_t b = step * 128u + 64u * c + 16u * t, dst = slot + (2 * h + c) * 512 + lane * 16;
-      if (rows.code[h] && b < row_bytes) {
-        const uint8_t *p = rows.code[h] + b;
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t b = at + 64u * c + 16u * (lane & 3), d = dst + (2 * h + c) * 512;
         if (VEC) {
-          cp_async16(dst, p);
+          const bool in = rows.has[h] && b < row_bytes;
+          cp_async16(d, p + 64 * c, in ? 16u : 0u);
         } else {
           uint32_t q[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (b + i < row_bytes) q[i >> 2] |= ld_u8(p + i) << (8 * (i & 3));
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
+            if (rows.has[h] && b + i < row_bytes) q[i >> 2] |= ld_u8(p + 64 * c + i) << (8 * (i & 3));
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
         }
-      } else {
-        st_zero16(dst);
       }
     }
   }
   if (SCALES && (lane & 1) == 0) {
-    const uint32_t dst = slot + 4 * 512 + lane * 4, b0 = step * 8u, kblocks = row_bytes / 16u;
-    if (SVEC && rows.scale && b0 + 8u <= kblocks) {
-      cp_async8(dst, rows.scale + b0);
+    const uint32_t d = slot + CODE_BYTES + lane * 4, b0 = step * 8u, kblocks = row_bytes / 16u;
+    if (SVEC && whole) {
+      cp_async8(d, rows.scale + b0, rows.has_scale ? 8u : 0u);
     } else {
-      uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+      uint32_t q[2] = {0u, 0u};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (rows.scale && b0 + i < kblocks) q[i >> 2] = (q[i >> 2] & ~(0xFFu << (8 * (i & 3)))) | ld_u8(rows.scale + b0 + i) << (8 * (i & 3));
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(dst), "r"(q[0]), "r"(q[1]) : "memory");
-    }
-  }
-}
-
-// Activations in shared memory, for TG groups of two tokens: fp16 elements [token][elements] and one fp32 factor per block
-// [token][elements / 32].  `x` / `f`: shared addresses of token 0's element / block 0 of the step; the pitches are in bytes.
-// `last`: the last token there is; columns of further ones repeat it (columns do not mix) and are ignored by the caller.
-// y[group][row half]: the running sums of this lane's token (2 * group + t / 2), over blocks 2 (t % 2) and 2 (t % 2) + 1
-// of every chunk: the lanes t and t ^ 1 hold the two halves of a sum.
-template <int TG, bool FACTORS>
-__device__ __forceinline__ void multiply_step(uint32_t slot, uint32_t x, uint32_t x_pitch, uint32_t f, uint32_t f_pitch,
-                                              uint32_t last, uint32_t zeros, int lane, float (&y)[TG][2]) {
-  const int g = lane >> 2, t = lane & 3;
-  const bool mine = (g & 3) == t;
-  uint32_t xrow[TG], frow[TG];
-#pragma unroll
-  for (int q = 0; q < TG; ++q) {
-    xrow[q] = mine ? x + min(2u * q + (uint32_t)(g >> 2), last) * x_pitch + t * 64u : zeros;
-    frow[q] = f + min(2u * q + (uint32_t)(t >> 1), last) * f_pitch + (uint32_t)(t & 1) * 8u;
-  }
-  uint32_t sc[2][2];  // [row half][chunk]: the scale bytes of the chunk's four blocks
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[h][0]), "=r"(sc[h][1]) : "r"(slot + 4 * 512 + (g + 8 * h) * 8));
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    float acc[TG][4];
-#pragma unroll
-    for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
-    uint32_t lo[4], hi[4];
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3])
-                 : "r"(slot + c * 512 + lane * 16));
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3])
-                 : "r"(slot + (2 + c) * 512 + lane * 16));
-    const uint32_t skip = mine ? c * 256u : 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t a[4], b[4];
-      e2m1_to_f16(lo[j], a);
-      e2m1_to_f16(hi[j], b);
-#pragma unroll
-      for (int q = 0; q < TG; ++q) {
-        uint32_t v[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                     : "r"(xrow[q] + skip + 16u * j));
-        mma_f16(acc[q], a[0], b[0], a[1], b[1], v[0], v[1]);
-        mma_f16(acc[q], a[2], b[2], a[3], b[3], v[2], v[3]);
-      }
-    }
-    float s[2][2];  // [row half][block of this lane's pair]
-#pragma unroll
-    for (int h = 0; h < 2; ++h) e8m0x2(sc[h][c] >> (16 * (t & 1)), s[h][0], s[h][1]);
-#pragma unroll
-    for (int q = 0; q < TG; ++q) {
-      float f0 = 1.0f, f1 = 1.0f;
-      if (FACTORS)
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                     : "=f"(f0), "=f"(f1)
-                     : "r"(frow[q] + c * 16u));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float p0 = FACTORS ? acc[q][2 * h] * f0 : acc[q][2 * h], p1 = FACTORS ? acc[q][2 * h + 1] * f1 : acc[q][2 * h + 1];
-        y[q][h] = __fmaf_rn(p0, s[h][0], y[q][h]);
-        y[q][h] = __fmaf_rn(p1, s[h][1], y[q][h]);
-      }
+        if (rows.has_scale && b0 + i < kblocks) q[i >> 2] |= ld_u8(rows.scale + b0 + i) << (8 * (i & 3));
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(d), "r"(q[0]), "r"(q[1]) : "memory");
     }
   }
 }
@@ -196,6 +132,101 @@ __device__ __forceinline__ float block_factor(uint32_t top, float &back) {
   e = e > 126 ? 126 : e;
   back = u2f((uint32_t)(127 - e) << 23);
   return u2f((uint32_t)(127 + e) << 23);
+}
+
+// One group of two tokens as the mma's second operand, for one step, in registers: lane (g, t) with g % 4 == t holds block t of
+// both chunks of token g / 4 as fp16 pairs, every other lane zeros.  factor[chunk][i]: what undoes the block factors of the
+// sums this lane ends up with, token t / 2, blocks 2 (t % 2) + i.
+struct Columns {
+  uint32_t v[2][16];
+  float factor[2][2];
+};
+// a lane that holds no block, or a block that does not exist
+__device__ __forceinline__ void no_block(Columns &x, int c, float &back) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x.v[c][i] = 0u;
+  back = 1.0f;
+}
+// 32 fp32 values into the block of chunk c
+__device__ __forceinline__ void pack_block(Columns &x, int c, const float (&e)[32], float &back) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, f2u(e[i]) & 0x7FFFFFFFu);
+  const float factor = block_factor(top, back);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x.v[c][i] = pack_f16x2_no_nan(e[2 * i] * factor, e[2 * i + 1] * factor);
+}
+// the factors travel to the lanes whose sums they scale: block b of token h sits in lane 4 (4 h + b) + b
+__device__ __forceinline__ void spread_factors(Columns &x, const float (&back)[2], int lane) {
+  const int t = lane & 3;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x.factor[c][i] = __shfl_sync(0xFFFFFFFFu, back[c], 16 * (t >> 1) + 5 * (2 * (t & 1) + i));
+  }
+}
+
+// One step: y[group][row half] += the products of this lane's token (2 * group + t / 2) over blocks 2 (t % 2) and
+// 2 (t % 2) + 1 of both chunks: the lanes t and t ^ 1 hold the two halves of a sum.
+template <int TG>
+__device__ __forceinline__ void multiply_step(uint32_t slot, const Columns (&x)[TG], int lane, float (&y)[TG][2]) {
+  const int g = lane >> 2, t = lane & 3;
+  uint32_t sc[2][2];  // [row half][chunk]: the scale bytes of the chunk's four blocks
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[h][0]), "=r"(sc[h][1]) : "r"(slot + CODE_BYTES + (g + 8 * h) * 8));
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float acc[TG][4];
+#pragma unroll
+    for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
+    uint32_t lo[4], hi[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3])
+                 : "r"(slot + c * 512 + lane * 16));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3])
+                 : "r"(slot + (2 + c) * 512 + lane * 16));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a[4], b[4];
+      e2m1_to_f16(lo[j], a);
+      e2m1_to_f16(hi[j], b);
+#pragma unroll
+      for (int q = 0; q < TG; ++q) {
+        mma_f16(acc[q], a[0], b[0], a[1], b[1], x[q].v[c][4 * j], x[q].v[c][4 * j + 1]);
+        mma_f16(acc[q], a[2], b[2], a[3], b[3], x[q].v[c][4 * j + 2], x[q].v[c][4 * j + 3]);
+      }
+    }
+    float s[2][2];  // [row half][block of this lane's pair]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) e8m0x2(sc[h][c] >> (16 * (t & 1)), s[h][0], s[h][1]);
+#pragma unroll
+    for (int q = 0; q < TG; ++q) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        y[q][h] = __fmaf_rn(acc[q][2 * h] * x[q].factor[c][0], s[h][0], y[q][h]);
+        y[q][h] = __fmaf_rn(acc[q][2 * h + 1] * x[q].factor[c][1], s[h][1], y[q][h]);
+      }
+    }
+  }
+}
+
+// y of a tile and step into (first) or onto the warp's own sums [2 TG tokens][16 rows]
+template <int TG>
+__device__ __forceinline__ void keep_sums(float *sums, float (&y)[TG][2], bool first, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int q = 0; q < TG; ++q) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
+      if ((t & 1) == 0) {
+        float *o = sums + (2 * q + (t >> 1)) * 16 + g + 8 * h;
+        *o = first ? v : *o + v;
+      }
+    }
+  }
 }
 
 }  // namespace mxmma

@@ -1495,7 +1495,7 @@ static void run_mxf4_product(mxf4_product_t *q) {
     g.c = q->c; g.rsc0 = (int64_t)q->rsc; g.csc0 = 1;
     g.alpha_f = q->alpha; g.beta_f = q->beta;
     run_gemm_body(&g);
-  } else if (!q->along_n && g_ctx.force_path == 0 && skl_b200_mxf4_skinny_supported(q->m, q->n, q->k, q->ta)) {
+  } else if (!q->along_n && g_ctx.force_path == 0 && skl_b200_mxf4_skinny_supported(q->m, q->n, q->k)) {
     g_ctx.last_path = SKL_B200_PATH_GEMV;
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_skinny((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
