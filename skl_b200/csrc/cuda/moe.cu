@@ -231,6 +231,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
 
 constexpr uint32_t UP_DEPTH = 4;   // slots of a ring
 constexpr uint32_t UP_ROUND = 4;   // tiles of a warp between two barriers
+static_assert(8 * UP_ROUND * WARPS <= THREADS, "a thread per feature of a round");
 
 // Shared memory: rings (before them, for a moment, the routing's scratch) | 16-bit weights: x of a pass, bf16 [tokens][pitch]
 // | sums [2][round][warps along d][PASS][16] | lists
@@ -255,18 +256,18 @@ struct UpLayout {
 // its steps, so that the sums do.  The cursor names the warp's next item in that order, for the loads that run ahead.
 template <bool MX>
 struct Cursor {
-  uint32_t r0, r1, step, v;
+  uint32_t r0, r1, step, v, v0;  // the round, the warp's next item, its first tile in the round
   __device__ __forceinline__ void round(const uint32_t start, uint32_t u0, uint32_t u1, uint32_t tiles, uint32_t TW, uint32_t tw, uint32_t kw) {
     r0 = start;
     r1 = min(min(u1, r0 + UP_ROUND * TW), (r0 / tiles + 1u) * tiles);
-    v = r0 + (tw + TW - (r0 - u0) % TW) % TW;
+    v = v0 = r0 + ((tw - (r0 - u0)) & (TW - 1u));  // TW is a power of two
     step = kw;
   }
   __device__ __forceinline__ void next(uint32_t u0, uint32_t u1, uint32_t tiles, uint32_t steps, uint32_t KW, uint32_t TW, uint32_t kw, uint32_t tw) {
     if (MX) {
       v += TW;
       if (v < r1) return;
-      v = r0 + (tw + TW - (r0 - u0) % TW) % TW;
+      v = v0;
       step += KW;
       if (step < steps) return;
     } else {
@@ -311,7 +312,7 @@ __device__ __forceinline__ void up_columns(const MoeParams &p, const int32_t *pa
   }
 }
 
-template <bool MX, bool VEC, bool SVEC>
+template <bool MX, int MODE>
 __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   using F = Format<MX>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   uint32_t fill_at = 0;
   auto fill = [&]() {
     if (ahead.r0 < u1) {
-      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, ahead.step, row_bytes, lane);
+      fill_slot<MX, MODE>(ring + fill_at * F::SLOT, rows, ahead.step, row_bytes, lane);
       const uint32_t v = ahead.v, r0 = ahead.r0;
       ahead.next(u0, u1, tiles, steps, KW, TW, kw, tw);
       if (ahead.v != v) {
@@ -455,9 +456,10 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
     }
     __syncthreads();
     // h = silu(gate) * up; the other half of the sums is written meanwhile
-    const uint32_t outs = (r1 - r0) * 8u * cnt;
-    for (uint32_t i = threadIdx.x; i < outs; i += THREADS) {
-      const uint32_t c = i % (8u * (r1 - r0)), j = i / (8u * (r1 - r0));
+    // (token j, feature c of the round): a round has at most 8 UP_ROUND WARPS = THREADS features
+    for (uint32_t i = threadIdx.x; i < THREADS * cnt; i += THREADS) {
+      const uint32_t c = threadIdx.x, j = i / THREADS;
+      if (c >= 8u * (r1 - r0)) break;
       const uint32_t feature = (r0 - turn * tiles) * 8u + c;
       if (feature < p.f) {
         const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
@@ -485,7 +487,7 @@ struct DownLayout {
   static size_t total(uint32_t m) { return SUMS + (size_t)WARPS * m * 16 * 4; }
 };
 
-template <bool MX, bool VEC, bool SVEC, int DEPTH>
+template <bool MX, int MODE, int DEPTH>
 __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
   using F = Format<MX>;
   using L = DownLayout<MX, DEPTH>;
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
   uint32_t fill_item = warp, fill_a = warp / parts, fill_part = warp % parts, fill_sub = 0, fill_at = 0;
   auto fill = [&]() {
     if (fill_item < items) {
-      fill_slot<MX, VEC, SVEC>(ring + fill_at * F::SLOT, rows, fill_part * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
+      fill_slot<MX, MODE>(ring + fill_at * F::SLOT, rows, fill_part * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
       if (++fill_sub == F::ITEM_SLOTS) {
         fill_sub = 0;
         fill_item += WARPS, fill_a += by_a, fill_part += by_part;
@@ -713,7 +715,7 @@ cudaError_t launch(unsigned grid, size_t smem, cudaStream_t s, const MoeParams &
   return cudaLaunchKernelEx(&cfg, KERNEL, p);
 }
 
-template <bool MX, bool VEC, bool SVEC>
+template <bool MX, int MODE>
 cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
   using F = Format<MX>;
   const uint32_t pairs = p.m * p.topk;
@@ -727,13 +729,13 @@ cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
   if (up.total > MAX_SMEM) return cudaErrorInvalidConfiguration;
   // an SM has room for one CTA; never more CTAs than tiles that can exist
   const uint64_t most = (uint64_t)p.met * ((p.m + p.per_pass - 1) / p.per_pass) * ((p.f + 7) / 8);
-  cudaError_t e = launch<up_kernel<MX, VEC, SVEC>>((unsigned)(most < 148 ? most : 148), up.total, s, p);
+  cudaError_t e = launch<up_kernel<MX, MODE>>((unsigned)(most < 148 ? most : 148), up.total, s, p);
   if (e != cudaSuccess) return e;
   const uint32_t rounds = (p.d + 148u * 16u - 1u) / (148u * 16u), ctas = 148u * rounds;
   p.down_rows = (p.d + ctas - 1u) / ctas;
   const unsigned grid = (p.d + p.down_rows - 1u) / p.down_rows;
-  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch<down_kernel<MX, VEC, SVEC, 4>>(grid, DownLayout<MX, 4>::total(p.m), s, p);
-  return launch<down_kernel<MX, VEC, SVEC, 3>>(grid, DownLayout<MX, 3>::total(p.m), s, p);
+  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch<down_kernel<MX, MODE, 4>>(grid, DownLayout<MX, 4>::total(p.m), s, p);
+  return launch<down_kernel<MX, MODE, 3>>(grid, DownLayout<MX, 3>::total(p.m), s, p);
 }
 
 }  // namespace
@@ -772,13 +774,14 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.list.gate = (float *)(p.list.token + pairs);
   cudaStream_t s = (cudaStream_t)stream;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(p.w1) | reinterpret_cast<uintptr_t>(p.w2);
+  const uint32_t row1 = q->mx ? Format<true>::row_bytes(p.d) : Format<false>::row_bytes(p.d);
+  const uint32_t row2 = q->mx ? Format<true>::row_bytes(p.f) : Format<false>::row_bytes(p.f);
+  const uintptr_t scales = q->mx ? reinterpret_cast<uintptr_t>(p.s1) | reinterpret_cast<uintptr_t>(p.s2) : 0;
+  const int mode = (bases & 15u) || ((row1 | row2) & 15u) ? BYTES : ((row1 | row2) % 128 == 0 && (scales & 7u) == 0 ? WHOLE : ALIGNED);
   if (q->mx) {
-    // packed rows are whole blocks of 16 bytes; the rows of scales start on 8 bytes if their lengths are multiples of 8
-    const bool vec = (bases & 15u) == 0, svec = ((reinterpret_cast<uintptr_t>(p.s1) | reinterpret_cast<uintptr_t>(p.s2)) & 7u) == 0 &&
-                                                (p.d + 31) / 32 % 8 == 0 && (p.f + 31) / 32 % 8 == 0;
-    if (vec && svec) return (int)launch_moe<true, true, true>(p, s);
-    return (int)(vec ? launch_moe<true, true, false>(p, s) : launch_moe<true, false, false>(p, s));
+    if (mode == WHOLE) return (int)launch_moe<true, WHOLE>(p, s);
+    return (int)(mode == ALIGNED ? launch_moe<true, ALIGNED>(p, s) : launch_moe<true, BYTES>(p, s));
   }
-  const bool vec = (bases & 15u) == 0 && p.d % 8 == 0 && p.f % 8 == 0;
-  return (int)(vec ? launch_moe<false, true, false>(p, s) : launch_moe<false, false, false>(p, s));
+  if (mode == WHOLE) return (int)launch_moe<false, WHOLE>(p, s);
+  return (int)(mode == ALIGNED ? launch_moe<false, ALIGNED>(p, s) : launch_moe<false, BYTES>(p, s));
 }

@@ -78,43 +78,42 @@ struct TileRows {
   bool has[2], has_scale;
 };
 
+// How rows can be loaded.  WHOLE: rows start on 16 bytes and are whole steps of 128 bytes, scale rows start on 8 bytes: no
+// bounds within a row, a dozen instructions for a slot (with the checks of ALIGNED the loads took half the kernel's
+// instructions).  ALIGNED: rows start on 16 bytes and are whole units of 16.  BYTES: anything.
+enum RowMode { BYTES = 0, ALIGNED = 1, WHOLE = 2 };
+
 // Bytes [128 step, 128 step + 128) of a tile's 16 rows into a slot, and with SCALES the 8 scale bytes of each row.
 // `row_bytes`: length of a row (MX-FP4: 16 bytes to a block); what lies behind it counts as zeros (blocks that do not exist
-// and rows that do not exist have codes of zero and a scale that is finite).  VEC: rows start on 16 bytes and are whole units
-// of 16; SVEC: scale rows start on 8 bytes.  Without them single bytes are loaded, which are in place when the call returns.
-template <bool SCALES, bool VEC, bool SVEC>
+// and rows that do not exist have codes of zero and a scale that is finite).  Single bytes are in place when the call returns.
+template <bool SCALES, int MODE>
 __device__ __forceinline__ void fill_slot(uint32_t slot, const TileRows &rows, uint32_t step, uint32_t row_bytes, int lane) {
   const uint32_t at = step * 128u, dst = slot + lane * 16;
-  const bool whole = at + 128u <= row_bytes;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint8_t *p = rows.code[h] + at;
-    if (VEC && whole) {  // the usual case first: a dozen instructions for a slot
-      const uint32_t bytes = rows.has[h] ? 16u : 0u;
-      cp_async16(dst + 2 * h * 512, p, bytes);
-      cp_async16(dst + 2 * h * 512 + 512, p + 64, bytes);
-    } else {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t b = at + 64u * c + 16u * (lane & 3), d = dst + (2 * h + c) * 512;
-        if (VEC) {
-          const bool in = rows.has[h] && b < row_bytes;
-          cp_async16(d, p + 64 * c, in ? 16u : 0u);
-        } else {
-          uint32_t q[4] = {0u, 0u, 0u, 0u};
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t b = at + 64u * c + 16u * (lane & 3), d = dst + (2 * h + c) * 512;
+      if (MODE != BYTES) {
+        cp_async16(d, p + 64 * c, rows.has[h] && (MODE == WHOLE || b < row_bytes) ? 16u : 0u);
+      } else {
+        uint32_t q[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (rows.has[h] && b + i < row_bytes) q[i >> 2] |= ld_u8(p + 64 * c + i) << (8 * (i & 3));
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
-        }
+        for (int i = 0; i < 16; ++i)
+          if (rows.has[h] && b + i < row_bytes) q[i >> 2] |= ld_u8(p + 64 * c + i) << (8 * (i & 3));
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
       }
     }
   }
-  if (SCALES && (lane & 1) == 0) {
+  if (SCALES) {
     const uint32_t d = slot + CODE_BYTES + lane * 4, b0 = step * 8u, kblocks = row_bytes / 16u;
-    if (SVEC && whole) {
-      cp_async8(d, rows.scale + b0, rows.has_scale ? 8u : 0u);
-    } else {
+    if (MODE == WHOLE) {
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %3, 0;\n\t"
+          "@p cp.async.ca.shared.global [%0], [%1], 8, %2;\n\t}" ::"r"(d), "l"(rows.scale + b0), "r"(rows.has_scale ? 8u : 0u), "r"(lane & 1)
+          : "memory");
+    } else if ((lane & 1) == 0) {
       uint32_t q[2] = {0u, 0u};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -216,15 +215,19 @@ __device__ __forceinline__ void multiply_step(uint32_t slot, const Columns (&x)[
 template <int TG>
 __device__ __forceinline__ void keep_sums(float *sums, float (&y)[TG][2], bool first, int lane) {
   const int g = lane >> 2, t = lane & 3;
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(sums + (t >> 1) * 16 + g);
 #pragma unroll
   for (int q = 0; q < TG; ++q) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
-      if ((t & 1) == 0) {
-        float *o = sums + (2 * q + (t >> 1)) * 16 + g + 8 * h;
-        *o = first ? v : *o + v;
+      if (!first) {
+        float old;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(old) : "r"(at + (32 * q + 8 * h) * 4));
+        v += old;
       }
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %2, 0;\n\t@p st.shared.f32 [%0], %1;\n\t}" ::"r"(at + (32 * q + 8 * h) * 4), "f"(v), "r"(t & 1)
+                   : "memory");
     }
   }
 }

@@ -1,0 +1,522 @@
+// mxf4_planes.cu -- C = alpha * A W^T + beta * C for a batch of rows of A (bf16 / fp16) and MX-FP4 weights W [n][k], on the
+// block-scaled tensor-core instruction: tcgen05.mma.kind::mxf8f6f4.block_scale takes E2M1 weights with their E8M0 scales as
+// they are, next to an E4M3 operand with scales of its own.
+//
+// A enters as a sum of E4M3 matrices ("planes").  In a block of 32 with largest magnitude in [2^e, 2^(e+1)) the first plane
+// is a / 2^(e - 7) rounded to E4M3 (4 significant bits), the next the remainder / 2^(e - 11) -- at most 16 in the units
+// of the first, 256 in its own -- and so on, each remainder exact in fp32.  bf16 has 8 significant bits, fp16 11: after two
+// and three planes nothing is left of a value of the block's upper 2^14, and what is left of smaller ones is below 2^-20
+// (bf16) or 2^-24 (fp16) of the block's largest, the size of the fp32 sums' own rounding.  Products with E2M1 are exact, sums fp32.
+// A block with an infinity or a NaN gets NaN scales: the row's results are NaN.
+//
+// planes_kernel writes the planes and lays the scales of both operands out the way tcgen05.cp takes them (512 bytes for 128
+// rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows of A by 256 rows of
+// W per CTA, k split over a cluster of CTAs so that the chip is full.  Warp 0 loads, by TMA with the 128-byte swizzle: planes, and
+// packed weights that the copy spreads to 16 elements per 16 bytes; warp 1 copies the scales to TMEM and issues the MMAs
+// (K = 32 each, 4 to a stage and plane); all warps then read the accumulator, the cluster adds its parts through distributed
+// shared memory in a fixed order, and every CTA stores a share of the rows.  The tensor core spends 128 clocks on a 128 x 256 x 32
+// product, 32 weights a clock and SM with two planes: 4.8 TB/s of packed weights.  Every wait is bounded.
+#include <cuda.h>
+
+#include "loads.cuh"
+#include "numerics.cuh"
+
+namespace sklb {
+namespace {
+
+constexpr int BM = 128, BN = 256, BK = 128;  // tile; elements of k of a stage, one byte each in shared memory
+constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+constexpr int SF_BYTES = 512;  // scales of 128 rows and one stage
+constexpr int THREADS = 256;
+constexpr uint32_t ERR_EMPTY = 0x401, ERR_FULL = 0x402, ERR_DONE = 0x403;
+
+template <int PLANES>
+struct Cfg {
+  // bytes that a stage's barrier counts: of the weights the packed ones, half of what they take up in shared memory
+  static constexpr int TX = PLANES * A_BYTES + B_BYTES / 2 + (PLANES + 2) * SF_BYTES;
+  static constexpr int STAGE = (PLANES * A_BYTES + B_BYTES + (PLANES + 2) * SF_BYTES + 1023) / 1024 * 1024;  // tiles start on 1024 bytes
+  static constexpr int STAGES = PLANES == 2 ? 3 : 2;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
+  static_assert(SMEM <= 227 * 1024, "exceeds the shared memory one CTA can have");
+  static_assert(STAGES * STAGE >= BM * BN * 4, "the accumulator is staged where the operands were");
+};
+
+struct PlanesParams {
+  const uint8_t *sfa, *sfb;  // [plane][row tile][stage][512], [128-row tile][stage][512]
+  void *c;
+  int64_t rsc;
+  int m, n, stages, tiles_m;
+  int64_t plane_rows;  // rows of a plane in the tensor map: planes lie below each other
+  int64_t sfa_plane;   // bytes of scales of a plane
+  float alpha, beta;
+  int tc, c_vec;
+  uint64_t wait_ns;
+  uint32_t *status;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait: false when it ran out or another thread of the CTA gave up.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *status, uint32_t code,
+                                         uint64_t limit_ns) {
+  uint64_t t0 = 0;
+  for (uint32_t spins = 0;; ++spins) {
+    if (bar_try(bar, parity)) return true;
+    if ((spins & 63u) == 63u) {
+      if (*abort_flag) return false;
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (t0 == 0) t0 = now;
+      if (now - t0 > limit_ns) {
+        *abort_flag = 1u;
+        atomicCAS(status, 0u, code);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tm),
+               "r"(bar), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// k-major operand, 128-byte rows with the 128-byte swizzle, 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t at) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(16u >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// 32 rows x 16 bytes of scales, no swizzle, 8-row groups 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t at) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)(128u >> 4) << 32 | 1ull << 46;
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------------------------------ planes
+// One thread for 8 elements of k, four lanes to a block.  Planes of rows behind m are not written (whatever lies there only
+// reaches rows of the accumulator that are not stored); their scales are 1.  `stages` * 128 is the k of the planes; the elements behind k are zeros.  The rest of the grid lays out the
+// scales of W: one 4-byte word (4 blocks of a row) per thread, rows behind n get scale 1.
+template <int PLANES>
+__global__ void __launch_bounds__(256)
+    planes_kernel(uint8_t *__restrict__ planes, uint8_t *__restrict__ sfa, const uint16_t *a, int64_t rsa, int m, int k, int stages,
+                  int bf16, int a_vec, int64_t plane_bytes, int64_t sfa_plane, uint32_t *__restrict__ sfb, const uint8_t *sb,
+                  int64_t cssb, int n, int kblocks, int64_t a_blocks, int64_t sfb_words) {
+  dep_wait();
+  const int64_t kp = (int64_t)stages * BK;
+  if ((int64_t)blockIdx.x >= a_blocks) {
+    const int64_t i = ((int64_t)blockIdx.x - a_blocks) * 256 + threadIdx.x;
+    if (i >= sfb_words) return;
+    // i = ((tile * stages + stage) * 128 + slot), slot = (r % 32) * 4 + r / 32
+    const int slot = (int)(i & 127), r = (slot >> 2) + 32 * (slot & 3);
+    const int64_t ts = i >> 7, tile = ts / stages, row = tile * 128 + r;
+    const int b0 = (int)(ts - tile * stages) * 4;
+    uint32_t w = 0x7F7F7F7Fu;
+    if (row < n) {
+      const uint8_t *p = sb + row * cssb + b0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (b0 + e < kblocks) w = (w & ~(0xFFu << (8 * e))) | ld_u8(p + e) << (8 * e);
+    }
+    sfb[i] = w;
+    return;
+  }
+  const int64_t groups = kp / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t rows = (int64_t)((m + BM - 1) / BM) * BM;
+  const int64_t row64 = i / groups;
+  const bool in = row64 < rows;
+  const int row = in ? (int)row64 : 0, g = in ? (int)(i - row64 * groups) : 0, kk = g * 8;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+  if (in && row < m) {
+    const uint16_t *src = a + (int64_t)row * rsa + kk;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (a_vec && kk + 8 <= k) {
+      const uint4 v = ld_v4(src);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (kk + e < k) w[e >> 1] |= ld_u16(src + e) << (16 * (e & 1));
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      x[2 * q] = bf16 ? dec_bf16(w[q] & 0xFFFFu) : dec_f16(w[q] & 0xFFFFu);
+      x[2 * q + 1] = bf16 ? u2f(w[q] & 0xFFFF0000u) : dec_f16(w[q] >> 16);
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, f2u(x[e]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  const int ef = (int)(top >> 23);
+  // scale byte of the first plane: 2^(ef - 127 - 7), then 4 less for each further one, not below 2^-127 (E8M0's smallest; every
+  // bf16 and fp16 value is a multiple of 2^-133, so nothing is lost there)
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
+    int s = ef - 7 - 4 * p;
+    s = s < 0 ? 0 : s;
+    const float up = u2f((uint32_t)(254 - s) << 23), down = s == 0 ? u2f(0x00400000u) : u2f((uint32_t)s << 23);  // 2^(127 - s), 2^(s - 127)
+    uint32_t w[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t lo = hw_e4m3x2(x[4 * q] * up, x[4 * q + 1] * up), hi = hw_e4m3x2(x[4 * q + 2] * up, x[4 * q + 3] * up);
+      w[q] = lo | hi << 16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * q + e] = __fmaf_rn(-dec_e4m3((w[q] >> (8 * e)) & 0xFFu), down, x[4 * q + e]);
+    }
+    if (ef == 255) s = 255, w[0] = w[1] = 0u;
+    if (in) {
+      if (row < m) *reinterpret_cast<uint2 *>(planes + p * plane_bytes + (int64_t)row * kp + kk) = make_uint2(w[0], w[1]);
+      if ((g & 3) == 0) {
+        const int r = row % BM, blk = g >> 2;
+        sfa[p * sfa_plane + (((int64_t)(row / BM) * stages + (blk >> 2)) * SF_BYTES) + (r % 32) * 16 + (r / 32) * 4 + (blk & 3)] =
+            (uint8_t)(row < m ? s : 127);
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- product
+template <int PLANES>
+__global__ void __launch_bounds__(THREADS, 1)
+    product_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb, const PlanesParams p) {
+  using C = Cfg<PLANES>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw), tiles = (raw + 1023u) & ~1023u, bars = tiles + C::STAGES * C::STAGE;
+  const uint32_t full = bars, empty = bars + 8 * C::STAGES, done = bars + 16 * C::STAGES;
+  uint8_t *gen = smem_raw + (bars - raw);
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + 16 * C::STAGES + 8), *abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank, ranks;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const int tile = (int)(blockIdx.x / ranks), mi = tile % p.tiles_m, ni = tile / p.tiles_m;
+  const int k0 = (int)((int64_t)p.stages * rank / ranks), k1 = (int)((int64_t)p.stages * (rank + 1) / ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      bar_init(full + 8 * s, 1);
+      bar_init(empty + 8 * s, 1);
+    }
+    bar_init(done, 1);
+    *abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr((const void *)tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  dep_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int s = k0; s < k1; ++s, ++issued) {
+        const int i = s - k0, st = i % C::STAGES;
+        if (i >= C::STAGES && !bar_wait(empty + 8 * st, (uint32_t)(i / C::STAGES - 1) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns)) break;
+        const uint32_t at = tiles + st * C::STAGE, fb = full + 8 * st, sf = at + PLANES * A_BYTES + B_BYTES;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"((uint32_t)C::TX) : "memory");
+#pragma unroll
+        for (int q = 0; q < PLANES; ++q) {
+          tma_2d(at + q * A_BYTES, &tma, fb, s * BK, (int)(q * p.plane_rows) + mi * BM);
+          bulk(sf + q * SF_BYTES, p.sfa + q * p.sfa_plane + ((int64_t)mi * p.stages + s) * SF_BYTES, SF_BYTES, fb);
+        }
+        tma_2d(at + PLANES * A_BYTES, &tmb, fb, s * BK, ni * BN);
+        bulk(sf + PLANES * SF_BYTES, p.sfb + ((int64_t)(2 * ni) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
+        bulk(sf + (PLANES + 1) * SF_BYTES, p.sfb + ((int64_t)(2 * ni + 1) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
+      }
+      // the copies of the last stages land before the memory is used for anything else, also when a wait has run out
+      for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
+        for (uint32_t spins = 0; spins < (1u << 22) && !bar_try(full + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u); ++spins) {
+        }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int s = k0; s < k1; ++s) {
+        const int i = s - k0, st = i % C::STAGES;
+        if (!bar_wait(full + 8 * st, (uint32_t)(i / C::STAGES) & 1u, abort_flag, p.status, ERR_FULL, p.wait_ns)) {
+          ok = false;
+          break;
+        }
+        // scales of the stage: plane q at columns 256 + 32 (i % 2) + 4 q, W at + 16 (rows 0..127) and + 20 (128..255).  A copy is
+        // ordered before later MMAs of its thread, not behind earlier ones: the MMAs of stage i - 2, which read the region
+        // this stage overwrites, have to be done (those of stage i - 1 keep the tensor core busy meanwhile).
+        if (i >= 2 &&
+            !bar_wait(empty + 8 * ((i - 2) % C::STAGES), (uint32_t)((i - 2) / C::STAGES) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        const uint32_t at = tiles + st * C::STAGE, sf = at + PLANES * A_BYTES + B_BYTES;
+        const uint32_t tsf = tmem + 256u + (uint32_t)(i & 1) * 32u;
+#pragma unroll
+        for (int q = 0; q < PLANES; ++q)
+          asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tsf + 4u * q), "l"(scale_desc(sf + q * SF_BYTES)) : "memory");
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tsf + 16u + 4u * q), "l"(scale_desc(sf + (PLANES + q) * SF_BYTES)) : "memory");
+        const uint64_t db = operand_desc(at + PLANES * A_BYTES);
+#pragma unroll
+        for (int q = 0; q < PLANES; ++q) {
+          const uint64_t da = operand_desc(at + q * A_BYTES);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // E4M3 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; N = 256, M = 128
+            const uint32_t idesc = (uint32_t)j << 4 | 0u << 7 | 5u << 10 | (uint32_t)(BN >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
+                                   (uint32_t)j << 29;
+            const uint32_t accumulate = (i | q | j) != 0;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(tmem),
+                "l"(da + (uint64_t)(2 * j)), "l"(db + (uint64_t)(2 * j)), "r"(idesc), "r"(accumulate), "r"(tsf + 4u * q), "r"(tsf + 16u)
+                : "memory");
+          }
+        }
+        commit(empty + 8 * st);
+      }
+      if (ok) commit(done);
+    }
+  }
+  // every MMA has finished: the accumulator is whole and the stages are free to hold it
+  __syncwarp();
+  const bool whole = k1 > k0 && bar_wait(done, 0u, abort_flag, p.status, ERR_DONE, p.wait_ns);
+  __syncthreads();
+  fence_after();
+  const int rows = min(BM, p.m - mi * BM), cols = min(BN, p.n - ni * BN);
+  float *acc = reinterpret_cast<float *>(smem_raw + (tiles - raw));  // [row][256], 16-byte groups rotated by the row
+  {
+    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+    float4 *out = reinterpret_cast<float4 *>(acc + row * BN);
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch) {
+      uint32_t r[32];
+      const uint32_t at = tmem + (uint32_t)(half * 128 + ch * 32) + ((uint32_t)(quad * 32) << 16);
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+          "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+          "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+            "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+            "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+            "=r"(r[31])
+          : "r"(at));
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int gq = half * 32 + ch * 8 + q;
+        float4 v = make_float4(u2f(r[4 * q]), u2f(r[4 * q + 1]), u2f(r[4 * q + 2]), u2f(r[4 * q + 3]));
+        if (!whole) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a share of k without a stage, or a wait that ran out
+        if (row < rows) out[(gq & ~7) | ((gq + row) & 7)] = v;
+      }
+    }
+  }
+  fence_before();
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+  // rows rank, rank + ranks, ...: a warp takes a row, a lane 4 columns at a time
+  for (int row = (int)rank + (int)ranks * warp; row < rows; row += (int)ranks * (THREADS / 32)) {
+    const int64_t c0 = (int64_t)(mi * BM + row) * p.rsc + (int64_t)ni * BN;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int gq = h * 32 + lane, col = gq * 4;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint32_t at = smem_addr(acc + row * BN + (((gq & ~7) | ((gq + row) & 7)) * 4));
+      for (uint32_t r = 0; r < ranks; ++r) {
+        uint32_t remote;
+        float4 w;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(remote) : "memory");
+        v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = __fmul_rn(p.alpha, v[e]);
+        if (p.beta != 0.0f && col + e < cols) v[e] = __fadd_rn(__fmul_rn(p.beta, load_c_f32(p.tc, p.c, c0 + col + e)), v[e]);
+      }
+      if (p.c_vec && col + 4 <= cols) {
+        if (p.tc == SKL_DT_F32) {
+          *reinterpret_cast<float4 *>((float *)p.c + c0 + col) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+          const bool bf = p.tc == SKL_DT_BF16;
+          const uint32_t lo = bf ? pack_bf16x2_no_nan(v[0], v[1]) : pack_f16x2_no_nan(v[0], v[1]);
+          const uint32_t hi = bf ? pack_bf16x2_no_nan(v[2], v[3]) : pack_f16x2_no_nan(v[2], v[3]);
+          *reinterpret_cast<uint2 *>((uint16_t *)p.c + c0 + col) = make_uint2(lo, hi);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < cols) store_c_f32(p.tc, p.c, c0 + col + e, v[e]);
+      }
+    }
+  }
+  // no CTA leaves while its shared memory may still be read
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = [] {
+    void *sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      return (EncodeFn) nullptr;
+    }
+    return (EncodeFn)sym;
+  }();
+  return fn;
+}
+
+int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+struct Layout {
+  int planes;
+  int64_t stages, rows, kp, plane_bytes, sfa_plane, sfb_bytes, sfa_at, sfb_at, total;
+};
+Layout layout(uint64_t m, uint64_t n, uint64_t k, int ta) {
+  Layout l;
+  l.planes = ta == SKL_DT_BF16 ? 2 : 3;
+  l.stages = up((int64_t)k, BK) / BK;
+  l.kp = l.stages * BK;
+  l.rows = up((int64_t)m, BM);
+  l.plane_bytes = l.rows * l.kp;
+  l.sfa_plane = l.rows / 128 * l.stages * SF_BYTES;
+  l.sfb_bytes = up((int64_t)n, BN) / 128 * l.stages * SF_BYTES;
+  l.sfa_at = l.planes * l.plane_bytes;
+  l.sfb_at = l.sfa_at + l.planes * l.sfa_plane;
+  l.total = l.sfb_at + l.sfb_bytes;
+  return l;
+}
+
+template <int PLANES>
+cudaError_t launch_product(const CUtensorMap &tma, const CUtensorMap &tmb, const PlanesParams &p, unsigned grid, unsigned ranks, cudaStream_t s) {
+  static bool ready[64];  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!ready[dev & 63]) {
+    e = cudaFuncSetAttribute(product_kernel<PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PLANES>::SMEM);
+    if (e != cudaSuccess) return e;
+    ready[dev & 63] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Cfg<PLANES>::SMEM;
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ranks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SKLB_COUNT_LAUNCH();
+  return cudaLaunchKernelEx(&cfg, product_kernel<PLANES>, tma, tmb, p);
+}
+
+}  // namespace
+}  // namespace sklb
+
+using namespace sklb;
+
+// the copy that spreads 4-bit elements wants rows of whole 128 elements on 32 bytes
+extern "C" int skl_b200_mxf4_planes_supported(uint64_t m, uint64_t n, uint64_t k, const void *b, int64_t csb) {
+  return m >= 1 && n >= 1 && k >= 128 && k % 128 == 0 && m < (1ull << 22) && n < (1ull << 30) && k < (1ull << 30) &&
+         (reinterpret_cast<uintptr_t>(b) & 31u) == 0 && (n == 1 || csb % 32 == 0) && encoder() != nullptr;
+}
+
+extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t n, uint64_t k, int ta) { return (size_t)layout(m, n, k, ta).total; }
+
+extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
+                                           const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
+                                           int64_t rsc, void *scratch, uint32_t wait_limit_ms, uint32_t *dev_status, void *stream) {
+  EncodeFn enc = encoder();
+  if (!enc) return (int)cudaErrorNotSupported;
+  const Layout l = layout(m, n, k, ta);
+  cudaStream_t s = (cudaStream_t)stream;
+  uint8_t *base = (uint8_t *)scratch;
+  CUtensorMap tma, tmb;
+  {
+    cuuint64_t dims[2] = {(cuuint64_t)l.kp, (cuuint64_t)(l.planes * l.rows)}, strides[1] = {(cuuint64_t)l.kp};
+    cuuint32_t box[2] = {BK, BM}, step[2] = {1, 1};
+    if (enc(&tma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return (int)cudaErrorInvalidValue;
+  }
+  {
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)n}, strides[1] = {(cuuint64_t)(n == 1 ? up(k / 2, 32) : csb)};
+    cuuint32_t box[2] = {BK, BN}, step[2] = {1, 1};
+    if (enc(&tmb, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void *>(b), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return (int)cudaErrorInvalidValue;
+  }
+  const int es = tc == SKL_DT_F32 ? 4 : 2;
+  {
+    const int64_t a_blocks = (l.rows * (l.kp / 8) + 255) / 256, sfb_words = l.sfb_bytes / 4, blocks = a_blocks + (sfb_words + 255) / 256;
+    if (blocks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
+    const int a_vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && (m == 1 || rsa % 8 == 0);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SKLB_COUNT_LAUNCH();
+    const int bf = ta == SKL_DT_BF16;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, bf ? planes_kernel<2> : planes_kernel<3>, base, base + l.sfa_at, (const uint16_t *)a, rsa, (int)m,
+                                       (int)k, (int)l.stages, bf, a_vec, l.plane_bytes, l.sfa_plane, (uint32_t *)(base + l.sfb_at),
+                                       (const uint8_t *)sb, cssb, (int)n, (int)(k / 32), a_blocks, sfb_words);
+    if (e != cudaSuccess) return (int)e;
+  }
+  PlanesParams p;
+  p.sfa = base + l.sfa_at, p.sfb = base + l.sfb_at, p.c = c, p.rsc = rsc;
+  p.m = (int)m, p.n = (int)n, p.stages = (int)l.stages, p.tiles_m = (int)(l.rows / BM);
+  p.plane_rows = l.rows, p.sfa_plane = l.sfa_plane;
+  p.alpha = alpha, p.beta = beta, p.tc = tc;
+  p.c_vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0 && (m == 1 || rsc * es % 16 == 0);
+  p.wait_ns = (uint64_t)(wait_limit_ms ? wait_limit_ms : 2000u) * 1000000ull;
+  p.status = dev_status;
+  const int64_t tiles = (int64_t)p.tiles_m * (up(n, BN) / BN);
+  // CTAs of a cluster: as many as keep all tiles on the chip at once, one stage each at least
+  unsigned ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= 148 && (int64_t)ranks * 2 <= l.stages) ranks *= 2;
+  if (tiles * ranks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
+  return (int)(l.planes == 2 ? launch_product<2>(tma, tmb, p, (unsigned)(tiles * ranks), ranks, s)
+                             : launch_product<3>(tma, tmb, p, (unsigned)(tiles * ranks), ranks, s));
+}

@@ -56,7 +56,7 @@ __device__ __forceinline__ void load_block(const SkinnyParams &p, uint32_t tok, 
 }
 
 // Shared memory: rings [16][DEPTH] | sums [tile][warps along k][2 TG][16]
-template <int TG, bool BF16, bool VEC, bool SVEC>
+template <int TG, bool BF16, int MODE>
 __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParam
   };
   auto fill = [&]() {
     if (fill_step < p.steps) {
-      fill_slot<true, VEC, SVEC>(ring + fill_at * SLOT_BYTES, at, fill_step, p.kblocks * 16u, lane);
+      fill_slot<true, MODE>(ring + fill_at * SLOT_BYTES, at, fill_step, p.kblocks * 16u, lane);
       fill_tile += TW;
       if (fill_tile >= tiles) {
         fill_tile = tw;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParam
 
 constexpr uint32_t MAX_ROWS = 128;  // of a CTA: bounds its sums; longer matrices take several rounds of CTAs
 
-template <int TG, bool BF16, bool VEC, bool SVEC>
+template <int TG, bool BF16, int MODE>
 cudaError_t launch_skinny(SkinnyParams &p, cudaStream_t s) {
   p.steps = (p.k + STEP - 1) / STEP;
   const uint32_t ctas = 148u * ((p.n + 148u * MAX_ROWS - 1u) / (148u * MAX_ROWS));
@@ -157,7 +157,7 @@ cudaError_t launch_skinny(SkinnyParams &p, cudaStream_t s) {
   p.k_warps = 1;
   while (p.k_warps < (uint32_t)WARPS && p.k_warps * 2u <= p.steps) p.k_warps *= 2u;
   const size_t smem = WARPS * DEPTH * SLOT_BYTES + (size_t)((p.cta_rows + 15u) / 16u) * p.k_warps * (2 * TG * 16) * 4;
-  auto kernel = skinny_kernel<TG, BF16, VEC, SVEC>;
+  auto kernel = skinny_kernel<TG, BF16, MODE>;
   static bool ready[64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -182,9 +182,9 @@ cudaError_t launch_skinny(SkinnyParams &p, cudaStream_t s) {
 }
 
 template <int TG, bool BF16>
-cudaError_t dispatch(SkinnyParams &p, bool vec, bool svec, cudaStream_t s) {
-  if (vec && svec) return launch_skinny<TG, BF16, true, true>(p, s);
-  return vec ? launch_skinny<TG, BF16, true, false>(p, s) : launch_skinny<TG, BF16, false, false>(p, s);
+cudaError_t dispatch(SkinnyParams &p, int mode, cudaStream_t s) {
+  if (mode == WHOLE) return launch_skinny<TG, BF16, WHOLE>(p, s);
+  return mode == ALIGNED ? launch_skinny<TG, BF16, ALIGNED>(p, s) : launch_skinny<TG, BF16, BYTES>(p, s);
 }
 
 }  // namespace
@@ -207,8 +207,9 @@ extern "C" int skl_b200_launch_mxf4_skinny(uint32_t m, uint32_t n, uint32_t k, f
   p.a_vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && (m == 1 || rsa % 8 == 0);
   const bool vec = (reinterpret_cast<uintptr_t>(b) & 15u) == 0 && (n == 1 || csb % 16 == 0);
   const bool svec = (reinterpret_cast<uintptr_t>(sb) & 7u) == 0 && (n == 1 || cssb % 8 == 0);
+  const int mode = !vec ? BYTES : (svec && p.kblocks % 8 == 0 ? WHOLE : ALIGNED);
   cudaStream_t s = (cudaStream_t)stream;
   const bool bf = ta == SKL_DT_BF16;
-  if (m <= 2) return (int)(bf ? dispatch<1, true>(p, vec, svec, s) : dispatch<1, false>(p, vec, svec, s));
-  return (int)(bf ? dispatch<2, true>(p, vec, svec, s) : dispatch<2, false>(p, vec, svec, s));
+  if (m <= 2) return (int)(bf ? dispatch<1, true>(p, mode, s) : dispatch<1, false>(p, mode, s));
+  return (int)(bf ? dispatch<2, true>(p, mode, s) : dispatch<2, false>(p, mode, s));
 }

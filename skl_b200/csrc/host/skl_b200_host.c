@@ -1398,6 +1398,11 @@ static void scratch_trim(void) {
   pthread_mutex_unlock(&g_pool_lock);
 }
 
+/* rows up to which 16-bit x MX-FP4 products run on the block-scaled tensor-core kernel; above it widening W pays */
+#ifndef MXF4_PLANES_MAX
+#define MXF4_PLANES_MAX 512
+#endif
+
 typedef struct {
   size_t m, n, k, rsa, rsb, rss, rsc;
   int ta, tc, along_n; /* along_n: W is packed along n (k packed rows), else along k (n packed rows) */
@@ -1500,6 +1505,17 @@ static void run_mxf4_product(mxf4_product_t *q) {
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_skinny((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
                                                            q->beta, q->c, q->tc, (int64_t)q->rsc, static_b, g_ctx.stream));
+  } else if (!q->along_n && q->m <= MXF4_PLANES_MAX && g_ctx.force_path != SKL_B200_PATH_GENERIC &&
+             skl_b200_mxf4_planes_supported(q->m, q->n, q->k, q->b, (int64_t)q->rsb)) {
+    uint32_t *st = device_status_words();
+    void *scratch = st ? scratch_get(skl_b200_mxf4_planes_scratch(q->m, q->n, q->k, q->ta)) : 0;
+    if (!scratch) return;
+    g_ctx.last_path = SKL_B200_PATH_TCGEN05;
+    (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_planes((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
+                                                           (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
+                                                           q->beta, q->c, q->tc, (int64_t)q->rsc, scratch,
+                                                           g_ctx.wait_limit_ms, st, g_ctx.stream));
+    scratch_put(scratch);
   } else {
     g_ctx.static_weights = 0; /* the widened copy is written by this call */
     mxf4_product_widened(q);
