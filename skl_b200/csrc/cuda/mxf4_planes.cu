@@ -1,21 +1,23 @@
 // mxf4_planes.cu -- C = alpha * A W^T + beta * C for a batch of rows of A (bf16 / fp16) and MX-FP4 weights W [n][k], on the
 // block-scaled tensor-core instruction: tcgen05.mma.kind::mxf8f6f4.block_scale takes E2M1 weights with their E8M0 scales as
-// they are, next to an E4M3 operand with scales of its own.
+// they are, next to an E5M2 operand with scales of its own.
 //
-// A enters as a sum of E4M3 matrices ("planes").  In a block of 32 with largest magnitude in [2^e, 2^(e+1)) the first plane
-// is a / 2^(e - 7) rounded to E4M3 (4 significant bits), the next the remainder / 2^(e - 11) -- at most 16 in the units
-// of the first, 256 in its own -- and so on, each remainder exact in fp32.  bf16 has 8 significant bits, fp16 11: after two
-// and three planes nothing is left of a value of the block's upper 2^14, and what is left of smaller ones is below 2^-20
-// (bf16) or 2^-24 (fp16) of the block's largest, the size of the fp32 sums' own rounding.  Products with E2M1 are exact, sums fp32.
+// A enters as a sum of E5M2 matrices ("planes").  In a block of 32 with largest magnitude in [2^e, 2^(e+1)) the first plane
+// is a / 2^(e - 14) rounded to E5M2 (3 significant bits), the next the remainder / 2^(e - 17), and so on, each remainder exact
+// in fp32.  bf16 has 8 significant bits, fp16 11: after three and four planes nothing is left of a value down to 2^-29 of its
+// block's largest, and less than 2^-36 of the largest is left of smaller ones.  (E4M3 planes, 4 bits each, would be two and
+// three, but their range of exponents rounds what is 2^-20 of a block's largest.)  Products with E2M1 are exact, sums fp32.
 // A block with an infinity or a NaN gets NaN scales: the row's results are NaN.
 //
-// planes_kernel writes the planes and lays the scales of both operands out the way tcgen05.cp takes them (512 bytes for 128
-// rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows of A by 256 rows of
-// W per CTA, k split over a cluster of CTAs so that the chip is full.  Warp 0 loads, by TMA with the 128-byte swizzle: planes, and
-// packed weights that the copy spreads to 16 elements per 16 bytes; warp 1 copies the scales to TMEM and issues the MMAs
-// (K = 32 each, 4 to a stage and plane); all warps then read the accumulator, the cluster adds its parts through distributed
-// shared memory in a fixed order, and every CTA stores a share of the rows.  The tensor core spends 128 clocks on a 128 x 256 x 32
-// product, 32 weights a clock and SM with two planes: 4.8 TB/s of packed weights.  Every wait is bounded.
+// planes_kernel writes the planes, below each other, and lays the scales of both operands out the way tcgen05.cp takes them
+// (512 bytes for 128 rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows by
+// 256 rows of W per CTA, k split over a cluster of CTAs so that the chip is full.  A stage holds as
+// few tiles of A as the planes of its rows need: all planes below each other in one (42 bf16, 32 fp16 rows), pairs of planes
+// (64 rows), or each plane its own; the MMAs add over the tiles, the epilogue over the planes of a tile.  Warp 0 loads planes and scales by TMA, eight warps copy
+// the packed weights with 8-byte cp.async to where the instruction wants them, 16 elements to 16 bytes (the TMA's own spreading
+// copy of 4-bit elements took 1.1 us for a stage's 256 x 128, several times what HBM needs for them); warp 1 copies the scales
+// to TMEM and issues the MMAs (K = 32 each, 4 to a stage and tile).  At the end all warps read the accumulator, the cluster adds
+// its parts through distributed shared memory in a fixed order, and every CTA stores a share of the rows.  Every wait is bounded.
 #include <cuda.h>
 
 #include "loads.cuh"
@@ -27,27 +29,29 @@ namespace {
 constexpr int BM = 128, BN = 256, BK = 128;  // tile; elements of k of a stage, one byte each in shared memory
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
 constexpr int SF_BYTES = 512;  // scales of 128 rows and one stage
-constexpr int THREADS = 256;
+constexpr int LOADERS = 8, THREADS = 64 + 32 * LOADERS;  // warp 0: TMA, warp 1: MMA, then the loaders
 constexpr uint32_t ERR_EMPTY = 0x401, ERR_FULL = 0x402, ERR_DONE = 0x403;
 
+// PLANES: tiles of A to a stage
 template <int PLANES>
 struct Cfg {
-  // bytes that a stage's barrier counts: of the weights the packed ones, half of what they take up in shared memory
-  static constexpr int TX = PLANES * A_BYTES + B_BYTES / 2 + (PLANES + 2) * SF_BYTES;
-  static constexpr int STAGE = (PLANES * A_BYTES + B_BYTES + (PLANES + 2) * SF_BYTES + 1023) / 1024 * 1024;  // tiles start on 1024 bytes
-  static constexpr int STAGES = PLANES == 2 ? 3 : 2;
+  static constexpr int TX = PLANES * A_BYTES + (PLANES + 2) * SF_BYTES;                  // bytes that the TMA brings
+  static constexpr int STAGE = (TX + B_BYTES + 1023) / 1024 * 1024;                      // tiles start on 1024 bytes
+  static constexpr int STAGES = PLANES == 1 ? 4 : (PLANES == 2 ? 3 : 2);
   static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
   static_assert(SMEM <= 227 * 1024, "exceeds the shared memory one CTA can have");
   static_assert(STAGES * STAGE >= BM * BN * 4, "the accumulator is staged where the operands were");
 };
 
 struct PlanesParams {
-  const uint8_t *sfa, *sfb;  // [plane][row tile][stage][512], [128-row tile][stage][512]
+  const uint8_t *sfa, *sfb;  // [row tile of all planes][stage][512], [128-row tile][stage][512]
+  const uint8_t *b;
+  int64_t csb;
   void *c;
   int64_t rsc;
-  int m, n, stages, tiles_m;
-  int64_t plane_rows;  // rows of a plane in the tensor map: planes lie below each other
-  int64_t sfa_plane;   // bytes of scales of a plane
+  int m, n, stages, tiles_m, row_bytes;  // row_bytes: of a packed row
+  int plane_tiles;                       // row tiles from a stage's tile of A to its next
+  int fold;                              // planes of m rows in a tile
   float alpha, beta;
   int tc, c_vec;
   uint64_t wait_ns;
@@ -110,14 +114,15 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------------------ planes
-// One thread for 8 elements of k, four lanes to a block.  Planes of rows behind m are not written (whatever lies there only
-// reaches rows of the accumulator that are not stored); their scales are 1.  `stages` * 128 is the k of the planes; the elements behind k are zeros.  The rest of the grid lays out the
+// One thread for 8 elements of k, four lanes to a block; plane p of row r is row (p / fold) * tile_span + (p % fold) * m + r.
+// PLANES fills whole tiles: planes that are not needed (their elements come out as zeros) are written like the others.  Rows
+// that no plane has are not written, nor are their scales: whatever lies there only reaches accumulator rows that are not used.  `stages` * 128 is the k of the planes; the elements behind k are zeros.  The rest of the grid lays out the
 // scales of W: one 4-byte word (4 blocks of a row) per thread, rows behind n get scale 1.
 template <int PLANES>
 __global__ void __launch_bounds__(256)
     planes_kernel(uint8_t *__restrict__ planes, uint8_t *__restrict__ sfa, const uint16_t *a, int64_t rsa, int m, int k, int stages,
-                  int bf16, int a_vec, int64_t plane_bytes, int64_t sfa_plane, uint32_t *__restrict__ sfb, const uint8_t *sb,
-                  int64_t cssb, int n, int kblocks, int64_t a_blocks, int64_t sfb_words) {
+                  int bf16, int a_vec, int fold, int tile_span, uint32_t *__restrict__ sfb, const uint8_t *sb, int64_t cssb, int n, int kblocks,
+                  int64_t a_blocks, int64_t sfb_words) {
   dep_wait();
   const int64_t kp = (int64_t)stages * BK;
   if ((int64_t)blockIdx.x >= a_blocks) {
@@ -138,14 +143,13 @@ __global__ void __launch_bounds__(256)
     return;
   }
   const int64_t groups = kp / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t rows = (int64_t)((m + BM - 1) / BM) * BM;
   const int64_t row64 = i / groups;
-  const bool in = row64 < rows;
+  const bool in = row64 < m;
   const int row = in ? (int)row64 : 0, g = in ? (int)(i - row64 * groups) : 0, kk = g * 8;
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  if (in && row < m) {
+  if (in) {
     const uint16_t *src = a + (int64_t)row * rsa + kk;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
     if (a_vec && kk + 8 <= k) {
@@ -168,28 +172,28 @@ __global__ void __launch_bounds__(256)
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
   const int ef = (int)(top >> 23);
-  // scale byte of the first plane: 2^(ef - 127 - 7), then 4 less for each further one, not below 2^-127 (E8M0's smallest; every
+  // scale byte of the first plane: 2^(ef - 127 - 14), then 3 less for each further one, not below 2^-127 (E8M0's smallest; every
   // bf16 and fp16 value is a multiple of 2^-133, so nothing is lost there)
 #pragma unroll
   for (int p = 0; p < PLANES; ++p) {
-    int s = ef - 7 - 4 * p;
+    int s = ef - 14 - 3 * p;
     s = s < 0 ? 0 : s;
     const float up = u2f((uint32_t)(254 - s) << 23), down = s == 0 ? u2f(0x00400000u) : u2f((uint32_t)s << 23);  // 2^(127 - s), 2^(s - 127)
     uint32_t w[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const uint32_t lo = hw_e4m3x2(x[4 * q] * up, x[4 * q + 1] * up), hi = hw_e4m3x2(x[4 * q + 2] * up, x[4 * q + 3] * up);
+      const uint32_t lo = hw_e5m2x2(x[4 * q] * up, x[4 * q + 1] * up), hi = hw_e5m2x2(x[4 * q + 2] * up, x[4 * q + 3] * up);
       w[q] = lo | hi << 16;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * q + e] = __fmaf_rn(-dec_e4m3((w[q] >> (8 * e)) & 0xFFu), down, x[4 * q + e]);
+      for (int e = 0; e < 4; ++e) x[4 * q + e] = __fmaf_rn(-dec_e5m2((w[q] >> (8 * e)) & 0xFFu), down, x[4 * q + e]);
     }
     if (ef == 255) s = 255, w[0] = w[1] = 0u;
     if (in) {
-      if (row < m) *reinterpret_cast<uint2 *>(planes + p * plane_bytes + (int64_t)row * kp + kk) = make_uint2(w[0], w[1]);
+      const int64_t at = (int64_t)(p / fold) * tile_span + (int64_t)(p % fold) * m + row;
+      *reinterpret_cast<uint2 *>(planes + at * kp + kk) = make_uint2(w[0], w[1]);
       if ((g & 3) == 0) {
-        const int r = row % BM, blk = g >> 2;
-        sfa[p * sfa_plane + (((int64_t)(row / BM) * stages + (blk >> 2)) * SF_BYTES) + (r % 32) * 16 + (r / 32) * 4 + (blk & 3)] =
-            (uint8_t)(row < m ? s : 127);
+        const int r = (int)(at % BM), blk = g >> 2;
+        sfa[(at / BM * stages + (blk >> 2)) * SF_BYTES + (r % 32) * 16 + (r / 32) * 4 + (blk & 3)] = (uint8_t)s;
       }
     }
   }
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(256)
 // ----------------------------------------------------------------------------------------------------------- product
 template <int PLANES>
 __global__ void __launch_bounds__(THREADS, 1)
-    product_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb, const PlanesParams p) {
+    product_kernel(const __grid_constant__ CUtensorMap tma, const PlanesParams p) {
   using C = Cfg<PLANES>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw), tiles = (raw + 1023u) & ~1023u, bars = tiles + C::STAGES * C::STAGE;
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      bar_init(full + 8 * s, 1);
+      bar_init(full + 8 * s, 1 + LOADERS);
       bar_init(empty + 8 * s, 1);
     }
     bar_init(done, 1);
@@ -242,16 +246,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"((uint32_t)C::TX) : "memory");
 #pragma unroll
         for (int q = 0; q < PLANES; ++q) {
-          tma_2d(at + q * A_BYTES, &tma, fb, s * BK, (int)(q * p.plane_rows) + mi * BM);
-          bulk(sf + q * SF_BYTES, p.sfa + q * p.sfa_plane + ((int64_t)mi * p.stages + s) * SF_BYTES, SF_BYTES, fb);
+          const int row_tile = q * p.plane_tiles + mi;
+          tma_2d(at + q * A_BYTES, &tma, fb, s * BK, row_tile * BM);
+          bulk(sf + q * SF_BYTES, p.sfa + ((int64_t)row_tile * p.stages + s) * SF_BYTES, SF_BYTES, fb);
         }
-        tma_2d(at + PLANES * A_BYTES, &tmb, fb, s * BK, ni * BN);
         bulk(sf + PLANES * SF_BYTES, p.sfb + ((int64_t)(2 * ni) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
         bulk(sf + (PLANES + 1) * SF_BYTES, p.sfb + ((int64_t)(2 * ni + 1) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
       }
       // the copies of the last stages land before the memory is used for anything else, also when a wait has run out
       for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
-        for (uint32_t spins = 0; spins < (1u << 22) && !bar_try(full + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u); ++spins) {
+        for (uint32_t spins = 0; spins < (1u << 20) && !bar_try(full + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u); ++spins) {
         }
     }
   } else if (warp == 1) {
@@ -286,8 +290,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t da = operand_desc(at + q * A_BYTES);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            // E4M3 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; N = 256, M = 128
-            const uint32_t idesc = (uint32_t)j << 4 | 0u << 7 | 5u << 10 | (uint32_t)(BN >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
+            // E5M2 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; N = 256, M = 128
+            const uint32_t idesc = (uint32_t)j << 4 | 1u << 7 | 5u << 10 | (uint32_t)(BN >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
                                    (uint32_t)j << 29;
             const uint32_t accumulate = (i | q | j) != 0;
             asm volatile(
@@ -301,16 +305,53 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (ok) commit(done);
     }
+  } else {
+    // packed weights: 8 lanes to a row, 8 bytes (16 elements) each, a warp takes 4 rows at a time; piece c of row r goes to the
+    // 16-byte chunk c ^ (r % 8) of the row's 128 bytes, the 128-byte swizzle
+    const int lw = warp - 2, sub = lane >> 3, c = lane & 7;
+    int i = 0;
+    bool ok = true;
+    auto arrive = [&](int st) {  // the copies of all lanes are in place: visible to the tensor core, then counted
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + 8 * st) : "memory");
+    };
+    for (int s = k0; s < k1; ++s, ++i) {
+      const int st = i % C::STAGES;
+      if (i >= C::STAGES) ok = bar_wait(empty + 8 * st, (uint32_t)(i / C::STAGES - 1) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
+      const uint32_t at = tiles + st * C::STAGE + PLANES * A_BYTES;
+      const int byte = s * (BK / 2) + 8 * c;
+#pragma unroll
+      for (int r0 = 0; r0 < BN; r0 += 4 * LOADERS) {
+        const int r = r0 + 4 * lw + sub, row = ni * BN + r;
+        const bool in = row < p.n && byte < p.row_bytes;
+        const uint8_t *src = p.b + (in ? (int64_t)row * p.csb + byte : 0);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at + (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4))), "l"(src), "r"(in ? 8u : 0u)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i >= C::STAGES - 2) {  // up to STAGES - 1 stages of copies in flight
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+        arrive((i - (C::STAGES - 2)) % C::STAGES);
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (ok)
+      for (int j = i > C::STAGES - 2 ? i - (C::STAGES - 2) : 0; j < i; ++j) arrive(j % C::STAGES);
   }
   // every MMA has finished: the accumulator is whole and the stages are free to hold it
   __syncwarp();
   const bool whole = k1 > k0 && bar_wait(done, 0u, abort_flag, p.status, ERR_DONE, p.wait_ns);
   __syncthreads();
   fence_after();
-  const int rows = min(BM, p.m - mi * BM), cols = min(BN, p.n - ni * BN);
+  const int rows = min(BM, p.m - mi * BM), cols = min(BN, p.n - ni * BN), used = p.fold > 1 ? p.fold * p.m : rows;  // folded: m <= 64, one row tile
   float *acc = reinterpret_cast<float *>(smem_raw + (tiles - raw));  // [row][256], 16-byte groups rotated by the row
-  {
-    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+  if (warp >= 2) {
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
     float4 *out = reinterpret_cast<float4 *>(acc + row * BN);
 #pragma unroll
     for (int ch = 0; ch < 4; ++ch) {
@@ -331,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int gq = half * 32 + ch * 8 + q;
         float4 v = make_float4(u2f(r[4 * q]), u2f(r[4 * q + 1]), u2f(r[4 * q + 2]), u2f(r[4 * q + 3]));
         if (!whole) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a share of k without a stage, or a wait that ran out
-        if (row < rows) out[(gq & ~7) | ((gq + row) & 7)] = v;
+        if (row < used) out[(gq & ~7) | ((gq + row) & 7)] = v;
       }
     }
   }
@@ -349,13 +390,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int h = 0; h < 2; ++h) {
       const int gq = h * 32 + lane, col = gq * 4;
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const uint32_t at = smem_addr(acc + row * BN + (((gq & ~7) | ((gq + row) & 7)) * 4));
-      for (uint32_t r = 0; r < ranks; ++r) {
-        uint32_t remote;
-        float4 w;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(remote) : "memory");
-        v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+      for (int q = 0; q < p.fold; ++q) {
+        const int from = row + q * p.m;  // the row's planes
+        const uint32_t at = smem_addr(acc + from * BN + (((gq & ~7) | ((gq + from) & 7)) * 4));
+        for (uint32_t r = 0; r < ranks; ++r) {
+          uint32_t remote;
+          float4 w;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(remote) : "memory");
+          v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -401,26 +445,27 @@ EncodeFn encoder() {
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 struct Layout {
-  int planes;
-  int64_t stages, rows, kp, plane_bytes, sfa_plane, sfb_bytes, sfa_at, sfb_at, total;
+  int planes, fold, tiles;  // planes; planes to a tile; tiles of A to a stage
+  int64_t stages, tile_span, tile_rows, kp, sfb_bytes, sfa_at, sfb_at, total;
 };
 Layout layout(uint64_t m, uint64_t n, uint64_t k, int ta) {
   Layout l;
-  l.planes = ta == SKL_DT_BF16 ? 2 : 3;
+  l.planes = ta == SKL_DT_BF16 ? 3 : 4;
+  l.fold = l.planes * m <= BM ? l.planes : (2 * m <= BM ? 2 : 1);
+  l.tiles = (l.planes + l.fold - 1) / l.fold;
   l.stages = up((int64_t)k, BK) / BK;
   l.kp = l.stages * BK;
-  l.rows = up((int64_t)m, BM);
-  l.plane_bytes = l.rows * l.kp;
-  l.sfa_plane = l.rows / 128 * l.stages * SF_BYTES;
+  l.tile_span = up((int64_t)m, BM);
+  l.tile_rows = l.tiles * l.tile_span;
   l.sfb_bytes = up((int64_t)n, BN) / 128 * l.stages * SF_BYTES;
-  l.sfa_at = l.planes * l.plane_bytes;
-  l.sfb_at = l.sfa_at + l.planes * l.sfa_plane;
+  l.sfa_at = l.tile_rows * l.kp;
+  l.sfb_at = l.sfa_at + l.tile_rows / 128 * l.stages * SF_BYTES;
   l.total = l.sfb_at + l.sfb_bytes;
   return l;
 }
 
 template <int PLANES>
-cudaError_t launch_product(const CUtensorMap &tma, const CUtensorMap &tmb, const PlanesParams &p, unsigned grid, unsigned ranks, cudaStream_t s) {
+cudaError_t launch_product(const CUtensorMap &tma, const PlanesParams &p, unsigned grid, unsigned ranks, cudaStream_t s) {
   static bool ready[64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -444,7 +489,7 @@ cudaError_t launch_product(const CUtensorMap &tma, const CUtensorMap &tmb, const
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   SKLB_COUNT_LAUNCH();
-  return cudaLaunchKernelEx(&cfg, product_kernel<PLANES>, tma, tmb, p);
+  return cudaLaunchKernelEx(&cfg, product_kernel<PLANES>, tma, p);
 }
 
 }  // namespace
@@ -452,10 +497,10 @@ cudaError_t launch_product(const CUtensorMap &tma, const CUtensorMap &tmb, const
 
 using namespace sklb;
 
-// the copy that spreads 4-bit elements wants rows of whole 128 elements on 32 bytes
+// packed rows on 8 bytes
 extern "C" int skl_b200_mxf4_planes_supported(uint64_t m, uint64_t n, uint64_t k, const void *b, int64_t csb) {
-  return m >= 1 && n >= 1 && k >= 128 && k % 128 == 0 && m < (1ull << 22) && n < (1ull << 30) && k < (1ull << 30) &&
-         (reinterpret_cast<uintptr_t>(b) & 31u) == 0 && (n == 1 || csb % 32 == 0) && encoder() != nullptr;
+  return m >= 1 && n >= 1 && k >= 1 && m < (1ull << 22) && n < (1ull << 30) && k < (1ull << 30) &&
+         (reinterpret_cast<uintptr_t>(b) & 7u) == 0 && (n == 1 || csb % 8 == 0) && encoder() != nullptr;
 }
 
 extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t n, uint64_t k, int ta) { return (size_t)layout(m, n, k, ta).total; }
@@ -468,24 +513,17 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
   const Layout l = layout(m, n, k, ta);
   cudaStream_t s = (cudaStream_t)stream;
   uint8_t *base = (uint8_t *)scratch;
-  CUtensorMap tma, tmb;
+  CUtensorMap tma;
   {
-    cuuint64_t dims[2] = {(cuuint64_t)l.kp, (cuuint64_t)(l.planes * l.rows)}, strides[1] = {(cuuint64_t)l.kp};
+    cuuint64_t dims[2] = {(cuuint64_t)l.kp, (cuuint64_t)l.tile_rows}, strides[1] = {(cuuint64_t)l.kp};
     cuuint32_t box[2] = {BK, BM}, step[2] = {1, 1};
     if (enc(&tma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return (int)cudaErrorInvalidValue;
   }
-  {
-    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)n}, strides[1] = {(cuuint64_t)(n == 1 ? up(k / 2, 32) : csb)};
-    cuuint32_t box[2] = {BK, BN}, step[2] = {1, 1};
-    if (enc(&tmb, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void *>(b), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return (int)cudaErrorInvalidValue;
-  }
   const int es = tc == SKL_DT_F32 ? 4 : 2;
   {
-    const int64_t a_blocks = (l.rows * (l.kp / 8) + 255) / 256, sfb_words = l.sfb_bytes / 4, blocks = a_blocks + (sfb_words + 255) / 256;
+    const int64_t a_blocks = ((int64_t)m * (l.kp / 8) + 255) / 256, sfb_words = l.sfb_bytes / 4, blocks = a_blocks + (sfb_words + 255) / 256;
     if (blocks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
     const int a_vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && (m == 1 || rsa % 8 == 0);
     cudaLaunchConfig_t cfg = {};
@@ -499,15 +537,18 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
     cfg.numAttrs = 1;
     SKLB_COUNT_LAUNCH();
     const int bf = ta == SKL_DT_BF16;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, bf ? planes_kernel<2> : planes_kernel<3>, base, base + l.sfa_at, (const uint16_t *)a, rsa, (int)m,
-                                       (int)k, (int)l.stages, bf, a_vec, l.plane_bytes, l.sfa_plane, (uint32_t *)(base + l.sfb_at),
-                                       (const uint8_t *)sb, cssb, (int)n, (int)(k / 32), a_blocks, sfb_words);
+    // planes written: whole tiles
+    const auto kernel = l.fold * l.tiles == 3 ? planes_kernel<3> : planes_kernel<4>;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, base, base + l.sfa_at, (const uint16_t *)a, rsa, (int)m,
+                                       (int)k, (int)l.stages, bf, a_vec, l.fold, (int)l.tile_span, (uint32_t *)(base + l.sfb_at),
+                                       (const uint8_t *)sb, cssb, (int)n, (int)((k + 31) / 32), a_blocks, sfb_words);
     if (e != cudaSuccess) return (int)e;
   }
   PlanesParams p;
   p.sfa = base + l.sfa_at, p.sfb = base + l.sfb_at, p.c = c, p.rsc = rsc;
-  p.m = (int)m, p.n = (int)n, p.stages = (int)l.stages, p.tiles_m = (int)(l.rows / BM);
-  p.plane_rows = l.rows, p.sfa_plane = l.sfa_plane;
+  p.b = (const uint8_t *)b, p.csb = csb;
+  p.m = (int)m, p.n = (int)n, p.stages = (int)l.stages, p.tiles_m = (int)((m + BM - 1) / BM);
+  p.row_bytes = (int)((k + 31) / 32 * 16), p.plane_tiles = (int)(l.tile_span / BM), p.fold = l.fold;
   p.alpha = alpha, p.beta = beta, p.tc = tc;
   p.c_vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0 && (m == 1 || rsc * es % 16 == 0);
   p.wait_ns = (uint64_t)(wait_limit_ms ? wait_limit_ms : 2000u) * 1000000ull;
@@ -517,6 +558,11 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
   unsigned ranks = 1;
   while (ranks < 8 && tiles * ranks * 2 <= 148 && (int64_t)ranks * 2 <= l.stages) ranks *= 2;
   if (tiles * ranks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
-  return (int)(l.planes == 2 ? launch_product<2>(tma, tmb, p, (unsigned)(tiles * ranks), ranks, s)
-                             : launch_product<3>(tma, tmb, p, (unsigned)(tiles * ranks), ranks, s));
+  const unsigned grid = (unsigned)(tiles * ranks);
+  switch (l.tiles) {
+    case 1: return (int)launch_product<1>(tma, p, grid, ranks, s);
+    case 2: return (int)launch_product<2>(tma, p, grid, ranks, s);
+    case 3: return (int)launch_product<3>(tma, p, grid, ranks, s);
+    default: return (int)launch_product<4>(tma, p, grid, ranks, s);
+  }
 }
