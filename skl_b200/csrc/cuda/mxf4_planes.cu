@@ -9,13 +9,13 @@
 // three, but their range of exponents rounds what is 2^-20 of a block's largest.)  Products with E2M1 are exact, sums fp32.
 // A block with an infinity or a NaN gets NaN scales: the row's results are NaN.
 //
-// planes_kernel writes the planes, below each other, and lays the scales of both operands out the way tcgen05.cp takes them
-// (512 bytes for 128 rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows by
-// 256 rows of W per CTA, k split over a cluster of CTAs so that the chip is full.  A stage holds as
+// planes_kernel writes the planes, below each other, and lays their scales out the way tcgen05.cp takes them (512 bytes for 128
+// rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows by
+// up to 256 rows of W per CTA, k split over a cluster of CTAs so that the chip is full.  A stage holds as
 // few tiles of A as the planes of its rows need: all planes below each other in one (42 bf16, 32 fp16 rows), pairs of planes
-// (64 rows), or each plane its own; the MMAs add over the tiles, the epilogue over the planes of a tile.  Warp 0 loads planes and scales by TMA, eight warps copy
-// the packed weights with 8-byte cp.async to where the instruction wants them, 16 elements to 16 bytes (the TMA's own spreading
-// copy of 4-bit elements took 1.1 us for a stage's 256 x 128, several times what HBM needs for them); warp 1 copies the scales
+// (64 rows), or each plane its own; the MMAs add over the tiles, the epilogue over the planes of a tile.  Warp 0 loads planes and scales by TMA, eight warps bring
+// the packed weights through registers to where the instruction wants them, 16 elements to 16 bytes, and their scales (the TMA's
+// own spreading copy of 4-bit elements took 1.1 us for a stage's 256 x 128, several times what HBM needs for them); warp 1 copies the scales
 // to TMEM and issues the MMAs (K = 32 each, 4 to a stage and tile).  At the end all warps read the accumulator, the cluster adds
 // its parts through distributed shared memory in a fixed order, and every CTA stores a share of the rows.  Every wait is bounded.
 #include <cuda.h>
@@ -26,7 +26,8 @@
 namespace sklb {
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 128;  // tile; elements of k of a stage, one byte each in shared memory
+constexpr int BM = 128, BN = 256, BK = 128;  // largest tile; elements of k of a stage, one byte each in shared memory
+constexpr int AHEAD = 3;                      // stages of packed weights that a loader holds in registers
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
 constexpr int SF_BYTES = 512;  // scales of 128 rows and one stage
 constexpr int LOADERS = 8, THREADS = 64 + 32 * LOADERS;  // warp 0: TMA, warp 1: MMA, then the loaders
@@ -35,8 +36,8 @@ constexpr uint32_t ERR_EMPTY = 0x401, ERR_FULL = 0x402, ERR_DONE = 0x403;
 // PLANES: tiles of A to a stage
 template <int PLANES>
 struct Cfg {
-  static constexpr int TX = PLANES * A_BYTES + (PLANES + 2) * SF_BYTES;                  // bytes that the TMA brings
-  static constexpr int STAGE = (TX + B_BYTES + 1023) / 1024 * 1024;                      // tiles start on 1024 bytes
+  static constexpr int TX = PLANES * (A_BYTES + SF_BYTES);                                          // bytes that the TMA brings
+  static constexpr int STAGE = (PLANES * A_BYTES + B_BYTES + (PLANES + 2) * SF_BYTES + 1023) / 1024 * 1024;  // tiles start on 1024 bytes
   static constexpr int STAGES = PLANES == 1 ? 4 : (PLANES == 2 ? 3 : 2);
   static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
   static_assert(SMEM <= 227 * 1024, "exceeds the shared memory one CTA can have");
@@ -44,16 +45,16 @@ struct Cfg {
 };
 
 struct PlanesParams {
-  const uint8_t *sfa, *sfb;  // [row tile of all planes][stage][512], [128-row tile][stage][512]
-  const uint8_t *b;
-  int64_t csb;
+  const uint8_t *sfa;  // [row tile of all planes][stage][512]
+  const uint8_t *b, *sb;
+  int64_t csb, cssb;
   void *c;
   int64_t rsc;
-  int m, n, stages, tiles_m, row_bytes;  // row_bytes: of a packed row
+  int m, n, stages, tiles_m, row_bytes, bn;  // row_bytes: of a packed row; bn: rows of W of a tile, a multiple of 16
   int plane_tiles;                       // row tiles from a stage's tile of A to its next
   int fold;                              // planes of m rows in a tile
   float alpha, beta;
-  int tc, c_vec;
+  int tc, c_vec, b_vec, s_vec;
   uint64_t wait_ns;
   uint32_t *status;
 };
@@ -116,32 +117,13 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 // ------------------------------------------------------------------------------------------------------------ planes
 // One thread for 8 elements of k, four lanes to a block; plane p of row r is row (p / fold) * tile_span + (p % fold) * m + r.
 // PLANES fills whole tiles: planes that are not needed (their elements come out as zeros) are written like the others.  Rows
-// that no plane has are not written, nor are their scales: whatever lies there only reaches accumulator rows that are not used.  `stages` * 128 is the k of the planes; the elements behind k are zeros.  The rest of the grid lays out the
-// scales of W: one 4-byte word (4 blocks of a row) per thread, rows behind n get scale 1.
+// that no plane has are not written, nor are their scales: whatever lies there only reaches accumulator rows that are not used.  `stages` * 128 is the k of the planes; the elements behind k are zeros.
 template <int PLANES>
 __global__ void __launch_bounds__(256)
     planes_kernel(uint8_t *__restrict__ planes, uint8_t *__restrict__ sfa, const uint16_t *a, int64_t rsa, int m, int k, int stages,
-                  int bf16, int a_vec, int fold, int tile_span, uint32_t *__restrict__ sfb, const uint8_t *sb, int64_t cssb, int n, int kblocks,
-                  int64_t a_blocks, int64_t sfb_words) {
+                  int bf16, int a_vec, int fold, int tile_span) {
   dep_wait();
   const int64_t kp = (int64_t)stages * BK;
-  if ((int64_t)blockIdx.x >= a_blocks) {
-    const int64_t i = ((int64_t)blockIdx.x - a_blocks) * 256 + threadIdx.x;
-    if (i >= sfb_words) return;
-    // i = ((tile * stages + stage) * 128 + slot), slot = (r % 32) * 4 + r / 32
-    const int slot = (int)(i & 127), r = (slot >> 2) + 32 * (slot & 3);
-    const int64_t ts = i >> 7, tile = ts / stages, row = tile * 128 + r;
-    const int b0 = (int)(ts - tile * stages) * 4;
-    uint32_t w = 0x7F7F7F7Fu;
-    if (row < n) {
-      const uint8_t *p = sb + row * cssb + b0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (b0 + e < kblocks) w = (w & ~(0xFFu << (8 * e))) | ld_u8(p + e) << (8 * e);
-    }
-    sfb[i] = w;
-    return;
-  }
   const int64_t groups = kp / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row64 = i / groups;
   const bool in = row64 < m;
@@ -250,8 +232,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_2d(at + q * A_BYTES, &tma, fb, s * BK, row_tile * BM);
           bulk(sf + q * SF_BYTES, p.sfa + ((int64_t)row_tile * p.stages + s) * SF_BYTES, SF_BYTES, fb);
         }
-        bulk(sf + PLANES * SF_BYTES, p.sfb + ((int64_t)(2 * ni) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
-        bulk(sf + (PLANES + 1) * SF_BYTES, p.sfb + ((int64_t)(2 * ni + 1) * p.stages + s) * SF_BYTES, SF_BYTES, fb);
       }
       // the copies of the last stages land before the memory is used for anything else, also when a wait has run out
       for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
@@ -291,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             // E5M2 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; N = 256, M = 128
-            const uint32_t idesc = (uint32_t)j << 4 | 1u << 7 | 5u << 10 | (uint32_t)(BN >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
+            const uint32_t idesc = (uint32_t)j << 4 | 1u << 7 | 5u << 10 | (uint32_t)(p.bn >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
                                    (uint32_t)j << 29;
             const uint32_t accumulate = (i | q | j) != 0;
             asm volatile(
@@ -306,49 +286,94 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (ok) commit(done);
     }
   } else {
-    // packed weights: 8 lanes to a row, 8 bytes (16 elements) each, a warp takes 4 rows at a time; piece c of row r goes to the
-    // 16-byte chunk c ^ (r % 8) of the row's 128 bytes, the 128-byte swizzle
-    const int lw = warp - 2, sub = lane >> 3, c = lane & 7;
-    int i = 0;
-    bool ok = true;
-    auto arrive = [&](int st) {  // the copies of all lanes are in place: visible to the tensor core, then counted
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + 8 * st) : "memory");
-    };
-    for (int s = k0; s < k1; ++s, ++i) {
-      const int st = i % C::STAGES;
-      if (i >= C::STAGES) ok = bar_wait(empty + 8 * st, (uint32_t)(i / C::STAGES - 1) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns);
-      if (!__all_sync(0xFFFFFFFFu, ok)) {
-        ok = false;
-        break;
-      }
-      const uint32_t at = tiles + st * C::STAGE + PLANES * A_BYTES;
-      const int byte = s * (BK / 2) + 8 * c;
+    // packed weights: 4 lanes to a row, 16 bytes (32 elements) each, a warp takes 8 rows at a time, AHEAD stages of loads in flight;
+    // the halves of lane c's piece go to the 16-byte chunks 2 c and 2 c + 1 of row r, chunk i at i ^ (r % 8): the 128-byte swizzle.
+    // Scales: one row to a thread, 16 blocks (four stages) to a load where they are aligned.
+    constexpr int PIECES = BN / (8 * LOADERS);
+    const int lw = warp - 2, sub = lane >> 2, c = lane & 3;
+    uint4 w[AHEAD][PIECES];
+    auto load = [&](uint4 (&v)[PIECES], int s) {
+      const int byte = s * (BK / 2) + 16 * c;
 #pragma unroll
-      for (int r0 = 0; r0 < BN; r0 += 4 * LOADERS) {
-        const int r = r0 + 4 * lw + sub, row = ni * BN + r;
-        const bool in = row < p.n && byte < p.row_bytes;
-        const uint8_t *src = p.b + (in ? (int64_t)row * p.csb + byte : 0);
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at + (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4))), "l"(src), "r"(in ? 8u : 0u)
-                     : "memory");
+      for (int q = 0; q < PIECES; ++q) {
+        const int r = q * 8 * LOADERS + 8 * lw + sub, row = ni * p.bn + r;
+        v[q] = make_uint4(0u, 0u, 0u, 0u);
+        if (s < k1 && r < p.bn && row < p.n && byte < p.row_bytes) {
+          const uint8_t *src = p.b + (int64_t)row * p.csb + byte;
+          if (p.b_vec) {
+            v[q] = ld_stream_v4(src);
+          } else {
+            const uint2 lo = ld_v2(src), hi = ld_v2(src + 8);
+            v[q] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (i >= C::STAGES - 2) {  // up to STAGES - 1 stages of copies in flight
-        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
-        arrive((i - (C::STAGES - 2)) % C::STAGES);
+    };
+    const int srow = 32 * lw + lane, wrow = ni * p.bn + srow;
+    const bool has_scale = srow < p.bn && wrow < p.n;
+    const uint8_t *ssrc = p.sb + (has_scale ? (int64_t)wrow * p.cssb : 0);
+    const uint32_t sdst = (uint32_t)((srow / 128) * SF_BYTES + (srow % 32) * 16 + (srow % 128 / 32) * 4);
+    const int kblocks = p.row_bytes / 16;
+    uint4 sc = make_uint4(0u, 0u, 0u, 0u), sc_next = sc;
+    // the scales of stages s & ~3 .. s | 3; blocks and rows that do not exist get 0, a scale that is finite
+    auto load_scales = [&](uint4 &v, int s) {
+      const int b0 = (s & ~3) * 4;
+      v = make_uint4(0u, 0u, 0u, 0u);
+      if (!has_scale || s >= k1) return;
+      if (p.s_vec && b0 + 16 <= kblocks) {
+        v = ld_v4(ssrc + b0);
+      } else {
+        uint32_t q[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (b0 + e < kblocks) q[e >> 2] |= ld_u8(ssrc + b0 + e) << (8 * (e & 3));
+        v = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+    };
+    load_scales(sc, k0);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) load(w[j], k0 + j);
+    load_scales(sc_next, (k0 | 3) + 1);
+    bool ok = true;
+    for (int i0 = 0; ok && k0 + i0 < k1; i0 += AHEAD) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = i0 + j, s = k0 + i, st = i % C::STAGES;
+        if (s >= k1) break;
+        if (i >= C::STAGES) ok = bar_wait(empty + 8 * st, (uint32_t)(i / C::STAGES - 1) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = tiles + st * C::STAGE + PLANES * A_BYTES;
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+          const int r = q * 8 * LOADERS + 8 * lw + sub;
+          if (r < p.bn) {
+            const uint32_t row = at + (uint32_t)r * 128u;
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(row + (uint32_t)(((2 * c) ^ (r & 7)) << 4)), "r"(w[j][q].x), "r"(w[j][q].y) : "memory");
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(row + (uint32_t)(((2 * c + 1) ^ (r & 7)) << 4)), "r"(w[j][q].z), "r"(w[j][q].w) : "memory");
+          }
+        }
+        const uint32_t word = (s & 3) == 0 ? sc.x : ((s & 3) == 1 ? sc.y : ((s & 3) == 2 ? sc.z : sc.w));
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + B_BYTES + PLANES * SF_BYTES + sdst), "r"(word) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor core, then counted
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + 8 * st) : "memory");
+        load(w[j], s + AHEAD);
+        if ((s & 3) == 3) {
+          sc = sc_next;
+          load_scales(sc_next, s + 5);
+        }
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (ok)
-      for (int j = i > C::STAGES - 2 ? i - (C::STAGES - 2) : 0; j < i; ++j) arrive(j % C::STAGES);
   }
   // every MMA has finished: the accumulator is whole and the stages are free to hold it
   __syncwarp();
   const bool whole = k1 > k0 && bar_wait(done, 0u, abort_flag, p.status, ERR_DONE, p.wait_ns);
   __syncthreads();
   fence_after();
-  const int rows = min(BM, p.m - mi * BM), cols = min(BN, p.n - ni * BN), used = p.fold > 1 ? p.fold * p.m : rows;  // folded: m <= 64, one row tile
+  const int rows = min(BM, p.m - mi * BM), cols = min(p.bn, p.n - ni * p.bn), used = p.fold > 1 ? p.fold * p.m : rows;  // folded: m <= 64, one row tile
   float *acc = reinterpret_cast<float *>(smem_raw + (tiles - raw));  // [row][256], 16-byte groups rotated by the row
   if (warp >= 2) {
     const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
@@ -385,10 +410,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   // rows rank, rank + ranks, ...: a warp takes a row, a lane 4 columns at a time
   for (int row = (int)rank + (int)ranks * warp; row < rows; row += (int)ranks * (THREADS / 32)) {
-    const int64_t c0 = (int64_t)(mi * BM + row) * p.rsc + (int64_t)ni * BN;
+    const int64_t c0 = (int64_t)(mi * BM + row) * p.rsc + (int64_t)ni * p.bn;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int gq = h * 32 + lane, col = gq * 4;
+      if (col >= cols) continue;
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int q = 0; q < p.fold; ++q) {
         const int from = row + q * p.m;  // the row's planes
@@ -446,9 +472,9 @@ int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 struct Layout {
   int planes, fold, tiles;  // planes; planes to a tile; tiles of A to a stage
-  int64_t stages, tile_span, tile_rows, kp, sfb_bytes, sfa_at, sfb_at, total;
+  int64_t stages, tile_span, tile_rows, kp, sfa_at, total;
 };
-Layout layout(uint64_t m, uint64_t n, uint64_t k, int ta) {
+Layout layout(uint64_t m, uint64_t k, int ta) {
   Layout l;
   l.planes = ta == SKL_DT_BF16 ? 3 : 4;
   l.fold = l.planes * m <= BM ? l.planes : (2 * m <= BM ? 2 : 1);
@@ -457,39 +483,74 @@ Layout layout(uint64_t m, uint64_t n, uint64_t k, int ta) {
   l.kp = l.stages * BK;
   l.tile_span = up((int64_t)m, BM);
   l.tile_rows = l.tiles * l.tile_span;
-  l.sfb_bytes = up((int64_t)n, BN) / 128 * l.stages * SF_BYTES;
   l.sfa_at = l.tile_rows * l.kp;
-  l.sfb_at = l.sfa_at + l.tile_rows / 128 * l.stages * SF_BYTES;
-  l.total = l.sfb_at + l.sfb_bytes;
+  l.total = l.sfa_at + l.tile_rows / 128 * l.stages * SF_BYTES;
   return l;
 }
 
+cudaLaunchConfig_t product_config(unsigned grid, unsigned ranks, size_t smem, cudaStream_t s, cudaLaunchAttribute *attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+// Rows of W to a tile and CTAs to a cluster: the pair whose longest CTA has the fewest stages x rows, with all tiles on the chip
+// at once if they fit.  How many clusters of a size fit is asked of the driver: with one CTA to an SM some SMs have no
+// partners left for clusters of 4 and 8, and a second round costs as much as the first.
 template <int PLANES>
-cudaError_t launch_product(const CUtensorMap &tma, const PlanesParams &p, unsigned grid, unsigned ranks, cudaStream_t s) {
-  static bool ready[64];  // per device
+cudaError_t launch_product(const CUtensorMap &tma, PlanesParams &p, cudaStream_t s) {
+  struct Device {
+    bool ready;
+    int fit[4];  // clusters of 1, 2, 4, 8
+  };
+  static Device devices[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (!ready[dev & 63]) {
+  Device &d = devices[dev & 63];
+  cudaLaunchAttribute attr[2];
+  if (!d.ready) {
     e = cudaFuncSetAttribute(product_kernel<PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PLANES>::SMEM);
     if (e != cudaSuccess) return e;
-    ready[dev & 63] = true;
+    for (int i = 0; i < 4; ++i) {
+      cudaLaunchConfig_t q = product_config(1u << i, 1u << i, Cfg<PLANES>::SMEM, s, attr);
+      q.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, product_kernel<PLANES>, &q) != cudaSuccess) {
+        (void)cudaGetLastError();
+        n = 0;
+      }
+      d.fit[i] = n;
+    }
+    if (d.fit[0] < 1) d.fit[0] = 1;
+    d.ready = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Cfg<PLANES>::SMEM;
-  cfg.stream = s;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ranks;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  unsigned ranks = 1;
+  int64_t best = INT64_MAX, tiles = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = 1ll << i, fit = d.fit[i];
+    if (fit < 1 || r > p.stages) break;
+    const int64_t room = fit / p.tiles_m;  // tiles along n that fit
+    int64_t bn = room > 0 ? up((p.n + room - 1) / room, 16) : BN;
+    bn = bn > BN ? BN : (bn < 64 ? 64 : bn);
+    const int64_t all = p.tiles_m * ((p.n + bn - 1) / bn), rounds = (all + fit - 1) / fit;
+    const int64_t cost = rounds * ((p.stages + r - 1) / r) * (bn + 64);  // 64: a stage's part that does not shrink with bn
+    if (cost < best) best = cost, ranks = (unsigned)r, p.bn = (int)bn, tiles = all;
+  }
+  if (tiles * ranks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  const cudaLaunchConfig_t cfg = product_config((unsigned)(tiles * ranks), ranks, Cfg<PLANES>::SMEM, s, attr);
   SKLB_COUNT_LAUNCH();
-  return cudaLaunchKernelEx(&cfg, product_kernel<PLANES>, tma, p);
+  return cudaLaunchKernelEx(&cfg, product_kernel<PLANES>, tma, (const PlanesParams)p);
 }
 
 }  // namespace
@@ -503,14 +564,14 @@ extern "C" int skl_b200_mxf4_planes_supported(uint64_t m, uint64_t n, uint64_t k
          (reinterpret_cast<uintptr_t>(b) & 7u) == 0 && (n == 1 || csb % 8 == 0) && encoder() != nullptr;
 }
 
-extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t n, uint64_t k, int ta) { return (size_t)layout(m, n, k, ta).total; }
+extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t k, int ta) { return (size_t)layout(m, k, ta).total; }
 
 extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                            const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
                                            int64_t rsc, void *scratch, uint32_t wait_limit_ms, uint32_t *dev_status, void *stream) {
   EncodeFn enc = encoder();
   if (!enc) return (int)cudaErrorNotSupported;
-  const Layout l = layout(m, n, k, ta);
+  const Layout l = layout(m, k, ta);
   cudaStream_t s = (cudaStream_t)stream;
   uint8_t *base = (uint8_t *)scratch;
   CUtensorMap tma;
@@ -523,7 +584,7 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
   }
   const int es = tc == SKL_DT_F32 ? 4 : 2;
   {
-    const int64_t a_blocks = ((int64_t)m * (l.kp / 8) + 255) / 256, sfb_words = l.sfb_bytes / 4, blocks = a_blocks + (sfb_words + 255) / 256;
+    const int64_t blocks = ((int64_t)m * (l.kp / 8) + 255) / 256;
     if (blocks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
     const int a_vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && (m == 1 || rsa % 8 == 0);
     cudaLaunchConfig_t cfg = {};
@@ -540,29 +601,24 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
     // planes written: whole tiles
     const auto kernel = l.fold * l.tiles == 3 ? planes_kernel<3> : planes_kernel<4>;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, base, base + l.sfa_at, (const uint16_t *)a, rsa, (int)m,
-                                       (int)k, (int)l.stages, bf, a_vec, l.fold, (int)l.tile_span, (uint32_t *)(base + l.sfb_at),
-                                       (const uint8_t *)sb, cssb, (int)n, (int)((k + 31) / 32), a_blocks, sfb_words);
+                                       (int)k, (int)l.stages, bf, a_vec, l.fold, (int)l.tile_span);
     if (e != cudaSuccess) return (int)e;
   }
   PlanesParams p;
-  p.sfa = base + l.sfa_at, p.sfb = base + l.sfb_at, p.c = c, p.rsc = rsc;
-  p.b = (const uint8_t *)b, p.csb = csb;
+  p.sfa = base + l.sfa_at, p.c = c, p.rsc = rsc;
+  p.b = (const uint8_t *)b, p.csb = csb, p.sb = (const uint8_t *)sb, p.cssb = cssb;
+  p.b_vec = (reinterpret_cast<uintptr_t>(b) & 15u) == 0 && (n == 1 || csb % 16 == 0);
+  p.s_vec = (reinterpret_cast<uintptr_t>(sb) & 15u) == 0 && (n == 1 || cssb % 16 == 0);
   p.m = (int)m, p.n = (int)n, p.stages = (int)l.stages, p.tiles_m = (int)((m + BM - 1) / BM);
   p.row_bytes = (int)((k + 31) / 32 * 16), p.plane_tiles = (int)(l.tile_span / BM), p.fold = l.fold;
   p.alpha = alpha, p.beta = beta, p.tc = tc;
   p.c_vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0 && (m == 1 || rsc * es % 16 == 0);
   p.wait_ns = (uint64_t)(wait_limit_ms ? wait_limit_ms : 2000u) * 1000000ull;
   p.status = dev_status;
-  const int64_t tiles = (int64_t)p.tiles_m * (up(n, BN) / BN);
-  // CTAs of a cluster: as many as keep all tiles on the chip at once, one stage each at least
-  unsigned ranks = 1;
-  while (ranks < 8 && tiles * ranks * 2 <= 148 && (int64_t)ranks * 2 <= l.stages) ranks *= 2;
-  if (tiles * ranks > 0x7FFFFFFFll) return (int)cudaErrorInvalidValue;
-  const unsigned grid = (unsigned)(tiles * ranks);
   switch (l.tiles) {
-    case 1: return (int)launch_product<1>(tma, p, grid, ranks, s);
-    case 2: return (int)launch_product<2>(tma, p, grid, ranks, s);
-    case 3: return (int)launch_product<3>(tma, p, grid, ranks, s);
-    default: return (int)launch_product<4>(tma, p, grid, ranks, s);
+    case 1: return (int)launch_product<1>(tma, p, s);
+    case 2: return (int)launch_product<2>(tma, p, s);
+    case 3: return (int)launch_product<3>(tma, p, s);
+    default: return (int)launch_product<4>(tma, p, s);
   }
 }

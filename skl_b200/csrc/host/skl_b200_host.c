@@ -1398,10 +1398,11 @@ static void scratch_trim(void) {
   pthread_mutex_unlock(&g_pool_lock);
 }
 
-/* rows up to which 16-bit x MX-FP4 products run on the block-scaled tensor-core kernel; above it widening W pays */
-#ifndef MXF4_PLANES_MAX
-#define MXF4_PLANES_MAX 512
-#endif
+/* Rows up to which 16-bit x MX-FP4 products run on the block-scaled tensor-core kernel, whose work grows with the planes that
+ * A is cut into; above it widening W once pays.  Measured on 14336 x 4096: bf16 256 rows 51 us against 91, 512 rows 140
+ * against 93; fp16 (four planes, and two products of the widened kind) 512 rows 167 us against 180, 1024 about even. */
+#define MXF4_PLANES_MAX_BF16 256
+#define MXF4_PLANES_MAX_F16 512
 
 typedef struct {
   size_t m, n, k, rsa, rsb, rss, rsc;
@@ -1505,10 +1506,10 @@ static void run_mxf4_product(mxf4_product_t *q) {
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_skinny((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
                                                            q->beta, q->c, q->tc, (int64_t)q->rsc, static_b, g_ctx.stream));
-  } else if (!q->along_n && q->m <= MXF4_PLANES_MAX && g_ctx.force_path != SKL_B200_PATH_GENERIC &&
+  } else if (!q->along_n && q->m <= (q->ta == SKL_DT_BF16 ? MXF4_PLANES_MAX_BF16 : MXF4_PLANES_MAX_F16) && g_ctx.force_path != SKL_B200_PATH_GENERIC &&
              skl_b200_mxf4_planes_supported(q->m, q->n, q->k, q->b, (int64_t)q->rsb)) {
     uint32_t *st = device_status_words();
-    void *scratch = st ? scratch_get(skl_b200_mxf4_planes_scratch(q->m, q->n, q->k, q->ta)) : 0;
+    void *scratch = st ? scratch_get(skl_b200_mxf4_planes_scratch(q->m, q->k, q->ta)) : 0;
     if (!scratch) return;
     g_ctx.last_path = SKL_B200_PATH_TCGEN05;
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_planes((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
