@@ -213,25 +213,13 @@ __device__ __forceinline__ void multiply_wide(uint32_t slot, uint32_t x, uint32_
 }
 
 // --------------------------------------------------------------------------------------------------------------- up
-// 8 elements of a bf16 row (zeros behind `cols`) as packed words
-__device__ __forceinline__ void load_x8(uint32_t (&w)[4], const uint16_t *row, uint32_t at, uint32_t cols, bool vec) {
-  w[0] = w[1] = w[2] = w[3] = 0u;
-  if (vec && at + 8u <= cols) {
-    const uint4 v = ld_v4(row + at);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (at + e < cols) w[e >> 1] |= ld_u16(row + at + e) << (16 * (e & 1));
-  }
-}
 __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 constexpr uint32_t UP_DEPTH = 4;   // slots of a ring
-constexpr uint32_t UP_ROUND = 4;   // tiles of a warp between two barriers
-static_assert(8 * UP_ROUND * WARPS <= THREADS, "a thread per feature of a round");
+template <bool MX>
+constexpr uint32_t UP_ROUND = MX ? 8 : 4;  // tiles of a warp between two barriers (16-bit weights: x takes the room)
 
 // Shared memory: rings (before them, for a moment, the routing's scratch) | 16-bit weights: x of a pass, bf16 [tokens][pitch]
 // | sums [2][round][warps along d][PASS][16] | lists
@@ -244,7 +232,7 @@ struct UpLayout {
     const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (WARPS * p.experts + pairs + p.experts) * 4u;
     x = ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
     sums = x + (MX ? 0u : p.per_pass * F::x_pitch(steps));
-    sums_half = UP_ROUND * WARPS * PASS * 16u;
+    sums_half = UP_ROUND<MX> * WARPS * PASS * 16u;
     lists = sums + 2u * sums_half * 4u;
     total = lists + (1u + p.met + 2u * (p.met + 1u) + pairs) * 4u;
   }
@@ -259,7 +247,7 @@ struct Cursor {
   uint32_t r0, r1, step, v, v0;  // the round, the warp's next item, its first tile in the round
   __device__ __forceinline__ void round(const uint32_t start, uint32_t u0, uint32_t u1, uint32_t tiles, uint32_t TW, uint32_t tw, uint32_t kw) {
     r0 = start;
-    r1 = min(min(u1, r0 + UP_ROUND * TW), (r0 / tiles + 1u) * tiles);
+    r1 = min(min(u1, r0 + UP_ROUND<MX> * TW), (r0 / tiles + 1u) * tiles);
     v = v0 = r0 + ((tw - (r0 - u0)) & (TW - 1u));  // TW is a power of two
     step = kw;
   }
@@ -282,33 +270,23 @@ struct Cursor {
   }
 };
 
+// The activations of a step as the columns of TG groups
 template <int TG>
 __device__ __forceinline__ void up_columns(const MoeParams &p, const int32_t *pairs, uint32_t cnt, uint32_t step, int lane, Columns (&x)[TG]) {
-  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int q = 0; q < TG; ++q) {
-    const uint32_t j = 2u * q + (uint32_t)(g >> 2);
-    float back[2];
+    const uint32_t j = 2u * q + (uint32_t)(lane >> 4);
+    const uint16_t *row = p.x + (int64_t)((uint32_t)pairs[min(j, cnt - 1u)] / p.topk) * p.rsx;
+    uint32_t w[2][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) load_row8(w[c], row, step * STEP + 128u * c + 8u * (lane & 15), j < cnt ? p.d : 0u, p.x_vec);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const uint32_t k0 = step * STEP + 128u * c + 32u * t;
-      if ((g & 3) == t && j < cnt && k0 < p.d) {
-        const uint16_t *row = p.x + (int64_t)((uint32_t)pairs[j] / p.topk) * p.rsx;
-        float e[32];
+      float e[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
-          load_x8(w, row, k0 + 8u * i, p.d, p.x_vec);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) e[8 * i + 2 * h] = dec_bf16(w[h] & 0xFFFFu), e[8 * i + 2 * h + 1] = u2f(w[h] & 0xFFFF0000u);
-        }
-        pack_block(x[q], c, e, back[c]);
-      } else {
-        no_block(x[q], c, back[c]);
-      }
+      for (int i = 0; i < 4; ++i) e[2 * i] = dec_bf16(w[c][i] & 0xFFFFu), e[2 * i + 1] = u2f(w[c][i] & 0xFFFF0000u);
+      gather_chunk(x[q], c, e, lane);
     }
-    __syncwarp();
-    spread_factors(x[q], back, lane);
   }
 }
 
@@ -432,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
         for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
           const uint32_t j = i / groups, gr = i - j * groups;
           uint32_t v[4];
-          load_x8(v, p.x + (int64_t)((uint32_t)list.pairs[pair0 + j] / p.topk) * p.rsx, gr * 8u, p.d, p.x_vec);
+          load_row8(v, p.x + (int64_t)((uint32_t)list.pairs[pair0 + j] / p.topk) * p.rsx, gr * 8u, p.d, p.x_vec);
           st_shared_v4(x + j * x_pitch + gr * 16u, v[0], v[1], v[2], v[3]);
         }
         held = turn;
@@ -456,10 +434,9 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
     }
     __syncthreads();
     // h = silu(gate) * up; the other half of the sums is written meanwhile
-    // (token j, feature c of the round): a round has at most 8 UP_ROUND WARPS = THREADS features
-    for (uint32_t i = threadIdx.x; i < THREADS * cnt; i += THREADS) {
-      const uint32_t c = threadIdx.x, j = i / THREADS;
-      if (c >= 8u * (r1 - r0)) break;
+    const uint32_t feats = 8u * (r1 - r0);
+    for (uint32_t i = threadIdx.x; i < feats * cnt; i += THREADS) {
+      const uint32_t j = i / feats, c = i - j * feats;
       const uint32_t feature = (r0 - turn * tiles) * 8u + c;
       if (feature < p.f) {
         const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
@@ -625,6 +602,11 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
     for (int32_t at = first; at < last; at += PASS) {
       const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)PASS);
       if (at != first) load_h(v, at, last, part * F::ITEM);
+      // where this lane's sums go: tokens 2 q + t / 2 of the pass (4-bit weights), 2 t and 2 t + 1 (16-bit)
+      const uint32_t j0 = MX ? (uint32_t)(t >> 1) : 2u * (t & 1), j1 = MX ? j0 + 2u : j0 + 1u;
+      const int32_t at0 = at + (int32_t)min(j0, cnt - 1u), at1 = at + (int32_t)min(j1, cnt - 1u);
+      float *own0 = own + p.list.token[at0] * 16 + g, *own1 = own + p.list.token[at1] * 16 + g;
+      const float gate0 = p.list.gate[at0], gate1 = p.list.gate[at1];
       __syncwarp();  // the h before has been read
       store_h(v, cnt);
       if (at + PASS >= last && more) load_h(v, next_first, next_last, next_part * F::ITEM);
@@ -650,8 +632,8 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
             const float s = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
             const uint32_t j = 2u * q + (uint32_t)(t >> 1);
             if ((t & 1) == 0 && j < cnt) {
-              float *o = own + p.list.token[at + j] * 16 + g + 8 * h;
-              *o = __fmaf_rn(p.list.gate[at + j], s, *o);
+              float *o = (q ? own1 : own0) + 8 * h;
+              *o = __fmaf_rn(q ? gate1 : gate0, s, *o);
             }
           }
         }
@@ -667,8 +649,8 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
           const float s = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
           const uint32_t j = 2u * t + (q & 1);
           if (t < 2 && j < cnt) {
-            float *o = own + p.list.token[at + j] * 16 + g + 8 * (q >> 1);
-            *o = __fmaf_rn(p.list.gate[at + j], s, *o);
+            float *o = (q & 1 ? own1 : own0) + 8 * (q >> 1);
+            *o = __fmaf_rn(q & 1 ? gate1 : gate0, s, *o);
           }
         }
       }

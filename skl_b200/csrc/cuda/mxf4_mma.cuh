@@ -140,28 +140,44 @@ struct Columns {
   uint32_t v[2][16];
   float factor[2][2];
 };
-// a lane that holds no block, or a block that does not exist
-__device__ __forceinline__ void no_block(Columns &x, int c, float &back) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x.v[c][i] = 0u;
-  back = 1.0f;
-}
-// 32 fp32 values into the block of chunk c
-__device__ __forceinline__ void pack_block(Columns &x, int c, const float (&e)[32], float &back) {
+// Chunk c of a group from 8 fp32 elements of every lane: lane L brings elements 8 (L % 4) .. + 7 of block L / 4 % 4 of token
+// L / 16 (zeros where there is none).  The four lanes of a quad are the four parts of one block, and the lane that has to hold
+// the block is one of them: the block's maximum takes two shuffles, the parts sixteen.
+__device__ __forceinline__ void gather_chunk(Columns &x, int c, const float (&e)[8], int lane) {
+  const int g = lane >> 2, t = lane & 3;
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, f2u(e[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 8; ++i) top = max(top, f2u(e[i]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  float back;
   const float factor = block_factor(top, back);
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x.v[c][i] = pack_f16x2_no_nan(e[2 * i] * factor, e[2 * i + 1] * factor);
+  for (int i = 0; i < 4; ++i) w[i] = pack_f16x2_no_nan(e[2 * i] * factor, e[2 * i + 1] * factor);
+  const bool mine = (g & 3) == t;
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = __shfl_sync(0xFFFFFFFFu, w[i], part, 4);
+      x.v[c][4 * part + i] = mine ? v : 0u;
+    }
+  }
+  // the factors travel to the lanes whose sums they scale: block b of token h is quad 4 h + b's
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x.factor[c][i] = __shfl_sync(0xFFFFFFFFu, back, 16 * (t >> 1) + 4 * (2 * (t & 1) + i));
 }
-// the factors travel to the lanes whose sums they scale: block b of token h sits in lane 4 (4 h + b) + b
-__device__ __forceinline__ void spread_factors(Columns &x, const float (&back)[2], int lane) {
-  const int t = lane & 3;
+// 8 consecutive 16-bit elements of a row (zeros from `len` on) as packed words
+__device__ __forceinline__ void load_row8(uint32_t (&w)[4], const uint16_t *row, uint32_t at, uint32_t len, bool vec) {
+  w[0] = w[1] = w[2] = w[3] = 0u;
+  if (vec && at + 8u <= len) {
+    const uint4 v = ld_v4(row + at);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) x.factor[c][i] = __shfl_sync(0xFFFFFFFFu, back[c], 16 * (t >> 1) + 5 * (2 * (t & 1) + i));
+    for (int e = 0; e < 8; ++e)
+      if (at + e < len) w[e >> 1] |= ld_u16(row + at + e) << (16 * (e & 1));
   }
 }
 

@@ -28,33 +28,6 @@ struct SkinnyParams {
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// 32 elements of a row of A as fp32 (zeros behind k)
-template <bool BF16>
-__device__ __forceinline__ void load_block(const SkinnyParams &p, uint32_t tok, uint32_t k0, float (&e)[32]) {
-  const uint16_t *src = (const uint16_t *)p.a + (int64_t)tok * p.rsa + k0;
-  uint32_t w[16];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (p.a_vec && k0 + 8u * i + 8u <= p.k) {
-      const uint4 v = ld_v4(src + 8 * i);
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[4 * i + j] = 0u;
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          if (k0 + 8u * i + 2u * j + q < p.k) w[4 * i + j] |= ld_u16(src + 8 * i + 2 * j + q) << (16 * q);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    e[2 * i] = BF16 ? dec_bf16(w[i] & 0xFFFFu) : dec_f16(w[i] & 0xFFFFu);
-    e[2 * i + 1] = BF16 ? u2f(w[i] & 0xFFFF0000u) : dec_f16(w[i] >> 16);
-  }
-}
-
 // Shared memory: rings [16][DEPTH] | sums [tile][warps along k][2 TG][16]
 template <int TG, bool BF16, int MODE>
 __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParams p) {
@@ -104,23 +77,27 @@ __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParam
   uint32_t slot = 0;
   for (uint32_t step = kw; step < p.steps && tw < tiles; step += KW) {
     Columns x[TG];
+    uint32_t w[TG][2][4];
 #pragma unroll
     for (int q = 0; q < TG; ++q) {
-      const uint32_t tok = 2u * q + (uint32_t)(g >> 2);
-      float back[2];
+      const uint32_t tok = 2u * q + (uint32_t)(lane >> 4);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        load_row8(w[q][c], (const uint16_t *)p.a + (int64_t)min(tok, p.m - 1u) * p.rsa, step * STEP + 128u * c + 8u * (lane & 15),
+                  tok < p.m ? p.k : 0u, p.a_vec);
+    }
+#pragma unroll
+    for (int q = 0; q < TG; ++q) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint32_t k0 = step * STEP + 128u * c + 32u * t;
-        if ((g & 3) == t && tok < p.m && k0 < p.k) {
-          float e[32];
-          load_block<BF16>(p, tok, k0, e);
-          pack_block(x[q], c, e, back[c]);
-        } else {
-          no_block(x[q], c, back[c]);
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[2 * i] = BF16 ? dec_bf16(w[q][c][i] & 0xFFFFu) : dec_f16(w[q][c][i] & 0xFFFFu);
+          e[2 * i + 1] = BF16 ? u2f(w[q][c][i] & 0xFFFF0000u) : dec_f16(w[q][c][i] >> 16);
         }
+        gather_chunk(x[q], c, e, lane);
       }
-      __syncwarp();
-      spread_factors(x[q], back, lane);
     }
     for (uint32_t tile = tw; tile < tiles; tile += TW) {
       float y[TG][2];
