@@ -74,52 +74,132 @@ __device__ __forceinline__ void load_eight_tail(Eight<DT> &v, const void *base, 
   }
 }
 
+// Which rows and groups of 8 elements a thread takes: a warp takes 32 * UNROLL consecutive groups of the matrix (rows one
+// after the other, 4 groups to a block), its lanes 32 consecutive ones at a time.  Where they lie in one row (`whole`, the same
+// for the warp) everything follows from the first with constants; the general case divides for every group, which is half
+// of the instructions of these kernels.
+template <int UNROLL>
+struct Groups {
+  uint64_t row0;   // row and group of the warp's first group
+  uint32_t rem0;
+  bool whole;
+  __device__ __forceinline__ Groups(uint32_t m, uint32_t per_row) {
+    const uint64_t first = (uint64_t)blockIdx.x * (THREADS * UNROLL) + (threadIdx.x >> 5) * (32u * UNROLL);
+    if (first >> 32) {
+      row0 = first / per_row;
+      rem0 = (uint32_t)(first - row0 * per_row);
+    } else {
+      row0 = (uint32_t)first / per_row;
+      rem0 = (uint32_t)first - (uint32_t)row0 * per_row;
+    }
+    whole = row0 < m && rem0 + 32u * UNROLL <= per_row;
+  }
+  // row (m: behind the end) and group of this lane's u-th group
+  __device__ __forceinline__ void at(int u, uint32_t m, uint32_t per_row, uint32_t &row, uint32_t &g) const {
+    const uint32_t r = rem0 + u * 32 + (threadIdx.x & 31);
+    if (whole) {
+      row = (uint32_t)row0;
+      g = r;
+    } else {
+      const uint64_t wide = row0 + r / per_row;
+      row = wide < m ? (uint32_t)wide : m;
+      g = r % per_row;
+    }
+  }
+  // the block whose scale this lane loads or stores, one byte for all groups of the warp: block lane % UNROLL * 8 + lane / 4 of the
+  // warp's 8 * UNROLL (UNROLL = 4) or block lane / 4 (UNROLL = 1, the first lane of each quad)
+  __device__ __forceinline__ bool own_block(uint32_t m, uint32_t per_row, uint32_t &r, uint32_t &blk) const {
+    const uint32_t lane = threadIdx.x & 31, i = rem0 + (UNROLL == 1 ? lane & ~3u : (lane % UNROLL) * 32u + (lane & ~3u));
+    if (whole) {
+      r = (uint32_t)row0;
+      blk = i >> 2;
+      return UNROLL > 1 || (lane & 3u) == 0u;
+    }
+    const uint64_t wide = row0 + i / per_row;
+    r = wide < m ? (uint32_t)wide : m;
+    blk = i % per_row >> 2;
+    return wide < m && (UNROLL > 1 || (lane & 3u) == 0u);
+  }
+};
+
+// 8 elements of a block (four lanes together hold it): the block's scale byte and the lane's codes
+template <int DT>
+__device__ __forceinline__ uint32_t encode_eight(const Eight<DT> &v, uint32_t &s) {
+  uint32_t top = 0;
+  if (DT == SKL_DT_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v.get(e)));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  } else {
+    // magnitudes of 16-bit floats order like their bits, two at a time
+    uint32_t pair = 0;
+#pragma unroll
+    for (int i = 0; i < Eight<DT>::W; ++i) pair = __vmaxu2(pair, v.w[i] & 0x7FFF7FFFu);
+    pair = __vmaxu2(pair, __shfl_xor_sync(0xFFFFFFFFu, pair, 1));
+    pair = __vmaxu2(pair, __shfl_xor_sync(0xFFFFFFFFu, pair, 2));
+    top = f2u(widen<DT>(max(pair & 0xFFFFu, pair >> 16)));
+  }
+  float factor;
+  s = scale_byte(top, factor);
+  uint32_t w;
+  if (DT == SKL_DT_BF16) {  // the exact product by a power of two, two elements at a time (what underflows becomes a zero code)
+    const uint32_t f = (f2u(factor) >> 16) * 0x00010001u;
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v.w[i % Eight<DT>::W]), "r"(f));
+    w = codes2(u2f(p[0] << 16), u2f(p[0] & 0xFFFF0000u), 1.0f) | codes2(u2f(p[1] << 16), u2f(p[1] & 0xFFFF0000u), 1.0f) << 8 |
+        codes2(u2f(p[2] << 16), u2f(p[2] & 0xFFFF0000u), 1.0f) << 16 | codes2(u2f(p[3] << 16), u2f(p[3] & 0xFFFF0000u), 1.0f) << 24;
+  } else {
+    w = codes2(v.get(0), v.get(1), factor) | codes2(v.get(2), v.get(3), factor) << 8 | codes2(v.get(4), v.get(5), factor) << 16 |
+        codes2(v.get(6), v.get(7), factor) << 24;
+  }
+  return s == 255u ? 0u : w;
+}
+
 // Rows with unit stride, 16-byte aligned.  Four lanes share a block: a lane takes 8 elements (one or two 16-byte loads), the
 // block's largest magnitude is two shuffles, the lane's 8 codes are one 4-byte store; loads and stores of a warp are
-// contiguous.  UNROLL groups per thread keep that many loads in flight.
+// contiguous.  UNROLL groups per thread keep that many loads in flight, and the warp's 32 scale bytes leave in one store.
 template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     quant_rows_kernel(uint8_t *__restrict__ dst, int64_t rsd, uint8_t *__restrict__ scales, int64_t rss,
                       const void *__restrict__ src, int64_t rs, uint32_t m, uint32_t k, uint32_t kblocks) {
+  static_assert(UNROLL == 1 || UNROLL == 4, "a lane stores one scale byte");
   dep_wait();
-  const uint32_t per_row = kblocks * 4u;  // groups of 8 elements
-  const uint64_t first = (uint64_t)blockIdx.x * (THREADS * UNROLL);
-  const uint64_t row0 = first / per_row;
-  const uint32_t rem0 = (uint32_t)(first - row0 * per_row);
+  const uint32_t per_row = kblocks * 4u;
+  const Groups<UNROLL> at(m, per_row);
   Eight<DT> v[UNROLL];
-  uint32_t row[UNROLL], g[UNROLL];
+  uint32_t byte = 0, s;
+  if (at.whole && (at.rem0 + 32u * UNROLL) * 8u <= k) {
+    const uint32_t g = at.rem0 + (threadIdx.x & 31);
+    const int64_t from = (int64_t)at.row0 * rs + (int64_t)g * 8;
+    uint8_t *to = dst + (int64_t)at.row0 * rsd + (int64_t)g * 4;
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const uint32_t r = rem0 + u * THREADS + threadIdx.x;
-    const uint64_t wide_row = row0 + r / per_row;
-    row[u] = wide_row < m ? (uint32_t)wide_row : m;
-    g[u] = r % per_row;
-    const int64_t at = (int64_t)row[u] * rs + (int64_t)g[u] * 8;
-    const int left = row[u] < m ? (int)k - (int)(g[u] * 8) : 0;
-    if (left >= 8) load_eight<DT>(v[u], src, at);
-    else load_eight_tail<DT>(v[u], src, at, left);
-  }
+    for (int u = 0; u < UNROLL; ++u) load_eight<DT>(v[u], src, from + 256 * u);
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    float x[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = v[u].get(e);
-      top = max(top, mag_bits(x[e]));
+    for (int u = 0; u < UNROLL; ++u) {
+      *reinterpret_cast<uint32_t *>(to + 128 * u) = encode_eight<DT>(v[u], s);
+      if (UNROLL == 1 || (int)(threadIdx.x & 3) == u) byte = s;
     }
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    float factor;
-    const uint32_t s = scale_byte(top, factor);
-    uint32_t w = codes2(x[0], x[1], factor) | codes2(x[2], x[3], factor) << 8 | codes2(x[4], x[5], factor) << 16 |
-                 codes2(x[6], x[7], factor) << 24;
-    if (s == 255u) w = 0u;
-    if (row[u] < m) {
-      *reinterpret_cast<uint32_t *>(dst + (int64_t)row[u] * rsd + (int64_t)g[u] * 4) = w;
-      if ((g[u] & 3u) == 0u) scales[(int64_t)row[u] * rss + (g[u] >> 2)] = (uint8_t)s;
+  } else {
+    uint32_t row[UNROLL], g[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      at.at(u, m, per_row, row[u], g[u]);
+      const int64_t from = (int64_t)row[u] * rs + (int64_t)g[u] * 8;
+      const int left = row[u] < m ? (int)k - (int)(g[u] * 8) : 0;
+      if (left >= 8) load_eight<DT>(v[u], src, from);
+      else load_eight_tail<DT>(v[u], src, from, left);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const uint32_t w = encode_eight<DT>(v[u], s);
+      if (row[u] < m) *reinterpret_cast<uint32_t *>(dst + (int64_t)row[u] * rsd + (int64_t)g[u] * 4) = w;
+      if (UNROLL == 1 || (int)(threadIdx.x & 3) == u) byte = s;
     }
   }
+  uint32_t r, blk;
+  if (at.own_block(m, per_row, r, blk)) scales[(int64_t)r * rss + blk] = (uint8_t)byte;
 }
 
 // Any two strides, any alignment: one warp per block of 32, one element per lane (consecutive lanes read consecutive
@@ -233,12 +313,6 @@ __global__ void __launch_bounds__(THREADS)
 __device__ __forceinline__ float scale_value(uint32_t s) {
   return u2f(s == 255u ? 0x7FC00000u : (s == 0u ? 0x00400000u : s << 23));  // 2^(s - 127); 2^-127 is subnormal
 }
-// the two E2M1 codes of byte `i` of w as floats
-__device__ __forceinline__ float2 values2(uint32_t byte) {
-  uint32_t h;
-  asm("{.reg .b8 t; cvt.u8.u32 t, %1; cvt.rn.f16x2.e2m1x2 %0, t;}" : "=r"(h) : "r"(byte));
-  return make_float2(dec_f16(h & 0xFFFFu), dec_f16(h >> 16));
-}
 template <int DT>
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
   return DT == SKL_DT_BF16 ? pack_bf16x2_no_nan(lo, hi) : pack_f16x2_no_nan(lo, hi);
@@ -249,59 +323,85 @@ __device__ __forceinline__ void store_one(void *dst, int64_t at, float v) {
   else ((uint16_t *)dst)[at] = (uint16_t)(narrow2<DT>(v, 0.0f) & 0xFFFFu);
 }
 
+// 8 elements from their codes
+template <int DT>
+__device__ __forceinline__ void decode_eight(uint32_t w, uint32_t s, float (&x)[8]) {
+  const float f = scale_value(s);
+  uint32_t h[4];
+  asm("{.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    x[2 * q] = __fmul_rn(dec_f16(h[q] & 0xFFFFu), f);
+    x[2 * q + 1] = __fmul_rn(dec_f16(h[q] >> 16), f);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_eight(void *dst, int64_t at, const float (&x)[8]) {
+  if (DT == SKL_DT_F32) {
+    float4 *o = reinterpret_cast<float4 *>((float *)dst + at);
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4 *>((uint16_t *)dst + at) =
+        make_uint4(narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3]), narrow2<DT>(x[4], x[5]), narrow2<DT>(x[6], x[7]));
+  }
+}
+
 // A thread widens 8 elements: one 4-byte load, one (16-bit types) or two 16-byte stores; the loads and stores of a warp are
-// contiguous.  vec: 4-byte aligned packed rows and 16-byte aligned output rows; without it, and in the ragged end of a row,
-// single bytes and elements.
+// contiguous, its 32 scale bytes come in one load.  vec: 4-byte aligned packed rows and 16-byte aligned output rows; without
+// it, and in the ragged end of a row, single bytes and elements.
 template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     widen_rows_kernel(void *__restrict__ dst, int64_t rsd, const uint8_t *__restrict__ src, int64_t rsa,
                       const uint8_t *__restrict__ scales, int64_t rss, uint32_t m, uint32_t k, int vec) {
+  static_assert(UNROLL == 1 || UNROLL == 4, "a lane loads one scale byte");
   dep_wait();
-  const uint32_t per_row = (k + 7u) / 8u;
-  const uint64_t first = (uint64_t)blockIdx.x * (THREADS * UNROLL);
-  const uint64_t row0 = first / per_row;
-  const uint32_t rem0 = (uint32_t)(first - row0 * per_row);
-  uint32_t row[UNROLL], g[UNROLL], w[UNROLL], s[UNROLL];
+  const uint32_t per_row = (k + 31u) / 32u * 4u;
+  const Groups<UNROLL> at(m, per_row);
+  uint32_t w[UNROLL], r, blk;
+  const uint32_t byte = at.own_block(m, per_row, r, blk) ? ld_u8(scales + (int64_t)r * rss + blk) : 0u;
+  float x[8];
+  if (vec && at.whole && (at.rem0 + 32u * UNROLL) * 8u <= k) {
+    const uint32_t g = at.rem0 + (threadIdx.x & 31);
+    const uint8_t *from = src + (int64_t)at.row0 * rsa + (int64_t)g * 4;
+    const int64_t to = (int64_t)at.row0 * rsd + (int64_t)g * 8;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) w[u] = ld_u32(from + 128 * u);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      decode_eight<DT>(w[u], __shfl_sync(0xFFFFFFFFu, byte, (threadIdx.x & 28) + (UNROLL == 1 ? 0 : u)), x);
+      store_eight<DT>(dst, to + 256 * u, x);
+    }
+    return;
+  }
+  uint32_t row[UNROLL], g[UNROLL], s[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    const uint32_t r = rem0 + u * THREADS + threadIdx.x;
-    const uint64_t wide_row = row0 + r / per_row;
-    row[u] = wide_row < m ? (uint32_t)wide_row : m;
-    g[u] = r % per_row;
-    w[u] = s[u] = 0u;
+    at.at(u, m, per_row, row[u], g[u]);
+    w[u] = 0u;
     if (row[u] < m) {
       const uint8_t *p = src + (int64_t)row[u] * rsa + (int64_t)g[u] * 4;
       if (vec) w[u] = ld_u32(p);
       else w[u] = ld_u8(p) | ld_u8(p + 1) << 8 | ld_u8(p + 2) << 16 | ld_u8(p + 3) << 24;
-      s[u] = ld_u8(scales + (int64_t)row[u] * rss + (g[u] >> 2));
     }
   }
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    if (row[u] >= m) continue;
-    const float f = scale_value(s[u]);
-    float x[8];
+  for (int u = 0; u < UNROLL; ++u) s[u] = __shfl_sync(0xFFFFFFFFu, byte, (threadIdx.x & 28) + (UNROLL == 1 ? 0 : u));
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 t = values2(w[u] >> (8 * q) & 0xFFu);
-      x[2 * q] = __fmul_rn(t.x, f);
-      x[2 * q + 1] = __fmul_rn(t.y, f);
-    }
-    const int64_t at = (int64_t)row[u] * rsd + (int64_t)g[u] * 8;
+  for (int u = 0; u < UNROLL; ++u) {
+    if (row[u] >= m || g[u] * 8u >= k) continue;
+    decode_eight<DT>(w[u], s[u], x);
+    const int64_t to = (int64_t)row[u] * rsd + (int64_t)g[u] * 8;
     const uint32_t left = k - g[u] * 8u;
     if (vec && left >= 8u) {
-      if (DT == SKL_DT_F32) {
-        float4 *o = reinterpret_cast<float4 *>((float *)dst + at);
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
-      } else {
-        *reinterpret_cast<uint4 *>((uint16_t *)dst + at) =
-            make_uint4(narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3]), narrow2<DT>(x[4], x[5]), narrow2<DT>(x[6], x[7]));
-      }
+      store_eight<DT>(dst, to, x);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if ((uint32_t)e < left) store_one<DT>(dst, at + e, x[e]);
+        if ((uint32_t)e < left) store_one<DT>(dst, to + e, x[e]);
     }
   }
 }
@@ -378,7 +478,7 @@ cudaError_t launch_widen(void *dst, int64_t rsd, const uint8_t *src, int64_t rsa
                          uint32_t m, uint32_t k, cudaStream_t s) {
   const int es = DT == SKL_DT_F32 ? 4 : 2;
   const int vec = aligned(src, 4) && aligned(dst, 16) && (m == 1 || (rsa % 4 == 0 && rsd * es % 16 == 0));
-  const uint64_t groups = (uint64_t)m * ((k + 7) / 8);
+  const uint64_t groups = (uint64_t)m * ((k + 31) / 32) * 4;
   if (groups < (1u << 18)) return launch(widen_rows_kernel<DT, 1>, ceil_div(groups, THREADS), s, dst, rsd, src, rsa, scales, rss, m, k, vec);
   return launch(widen_rows_kernel<DT, UNROLL>, ceil_div(groups, THREADS * UNROLL), s, dst, rsd, src, rsa, scales, rss, m, k, vec);
 }
