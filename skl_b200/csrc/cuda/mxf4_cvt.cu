@@ -267,18 +267,49 @@ __global__ void __launch_bounds__(THREADS)
         }
       }
     }
+    // 16-bit types, RPL = 4: a word holds two rows' elements, whose maxima and products (bf16) are taken two at a time
+    constexpr bool PAIRED = DT != SKL_DT_F32 && RPL > 1;
+    uint32_t pair_top[WORDS];
+    if (PAIRED) {
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) {
+        pair_top[j] = 0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) pair_top[j] = __vmaxu2(pair_top[j], raw[e][j] & 0x7FFF7FFFu);
+      }
+    }
+    uint32_t s_of[RPL];
+    float factor_of[RPL];
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) {
+      uint32_t top = 0;
+      if (PAIRED) {
+        const uint32_t bits = pair_top[(i / 2) % WORDS];
+        top = f2u(widen<DT>((i & 1) ? bits >> 16 : bits & 0xFFFFu));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = max(top, mag_bits(DT == SKL_DT_F32 ? u2f(raw[e][i % WORDS]) : widen<DT>(raw[e][0] & 0xFFFFu)));
+      }
+      s_of[i] = scale_byte(top, factor_of[i]);
+    }
+    if (PAIRED && DT == SKL_DT_BF16) {  // exact products by powers of two (what underflows becomes a zero code)
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) {
+        const uint32_t f = f2u(factor_of[(2 * j) % RPL]) >> 16 | (f2u(factor_of[(2 * j + 1) % RPL]) & 0xFFFF0000u);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(raw[e][j]) : "r"(raw[e][j]), "r"(f));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RPL; ++i) {
       auto val = [&](int e) {
         if (DT == SKL_DT_F32) return u2f(raw[e][i % WORDS]);
         const uint32_t w = raw[e][(i / 2) % WORDS];
+        if (DT == SKL_DT_BF16) return u2f((i & 1) ? w & 0xFFFF0000u : w << 16);
         return widen<DT>((i & 1) ? w >> 16 : w & 0xFFFFu);
       };
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < 32; ++e) top = max(top, mag_bits(val(e)));
-      float factor;
-      const uint32_t s = scale_byte(top, factor);
+      const uint32_t s = s_of[i];
+      const float factor = PAIRED && DT == SKL_DT_BF16 ? 1.0f : factor_of[i];
       uint32_t w[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
