@@ -29,7 +29,7 @@ constexpr size_t MAX_SMEM = 226 * 1024;
 
 // The routed pairs (token * topk + j) sorted by expert: n experts met, in ascending order, expert[a] with the pairs
 // pairs[first[a]] .. pairs[first[a + 1] - 1], in token order; they are taken `per_pass` at a time, passes before expert a: turn[a].
-// token[], gate[]: of the pairs, in the same order (only in the workspace, for the second kernel).
+// turn[] only in the first kernel; token[], gate[]: of the pairs, in the same order, only in the workspace for the second.
 struct Lists {
   int32_t *n, *expert, *first, *turn, *pairs, *token;
   float *gate;
@@ -76,15 +76,29 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 __device__ __forceinline__ float key_logit(uint32_t key) { return u2f((key >> 31) ? key & 0x7FFFFFFFu : ~key); }
 
 // One warp, one token: the routed slots (-1: a logit of minus infinity, which routes nowhere) and, with `write`, ids and
-// gates to global memory.  keys: `experts` words of this warp's shared memory.
+// gates to global memory.  The keys stay in registers up to 128 experts, above that in `keys`, `experts` words of this warp's
+// shared memory.
 __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, uint32_t *keys, int32_t *slots, int lane, bool write) {
   const float *row = p.logits + (int64_t)tok * p.rsl;
+  const bool small = p.experts <= 128u;
+  uint32_t reg[4];  // experts lane, lane + 32, ...
+#pragma unroll
+  for (int i = 0; i < 4; ++i) reg[i] = lane + 32u * i < p.experts && small ? logit_key(u2f(ld_u32(row + lane + 32 * i))) : 0u;
   uint32_t best = 0u, at = 0xFFFFFFFFu;  // this lane's largest key and its lowest index
-  for (uint32_t e = lane; e < p.experts; e += 32u) {
-    const uint32_t key = logit_key(u2f(ld_u32(row + e)));
-    keys[e] = key;
-    if (key > best) best = key, at = e;
+  if (!small) {
+    for (uint32_t e = lane; e < p.experts; e += 32u) {
+      const uint32_t key = logit_key(u2f(ld_u32(row + e)));
+      keys[e] = key;
+      if (key > best) best = key, at = e;
+    }
   }
+  auto scan = [&]() {
+    best = 0u, at = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (reg[i] > best) best = reg[i], at = lane + 32u * i;
+  };
+  if (small) scan();
   float top = 0.0f, mine = 0.0f, all = 0.0f;  // the largest logit; lane j keeps exp(logit_j - top)
   bool routed = false;
   int32_t my_id = -1;
@@ -96,7 +110,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
       top = v;
       if (write && !p.renormalise) {
         for (uint32_t i = lane; i < p.experts; i += 32u) {
-          const float w = key_logit(keys[i]);
+          const float w = u2f(ld_u32(row + i));
           all += w == -INFINITY ? 0.0f : expf(__fsub_rn(w, top));
         }
       }
@@ -106,7 +120,13 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
       routed = v != -INFINITY;
       mine = routed ? expf(__fsub_rn(v, top)) : 0.0f;
     }
-    if (at == e) {  // the owner of the winner looks for its next one
+    // the owner of the winner looks for its next one
+    if (small) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32u * i == e) reg[i] = 0u;
+      scan();
+    } else if (at == e) {
       keys[e] = 0u;
       best = 0u, at = 0xFFFFFFFFu;
       for (uint32_t i = lane; i < p.experts; i += 32u) {
@@ -126,60 +146,78 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
   }
 }
 
-// The whole CTA: every token's choice, then the lists.  scratch: keys [warps][experts] | slots [m * topk] | counts [experts].
+// The whole CTA: every token's choice, then the lists.  scratch: slots [m * topk, filled up to a multiple of 4 with -1] |
+// one bit for each expert that is met [32 words] | with more than 128 experts keys [warps][experts].  A thread per pair counts
+// the pairs that belong before it.
 __device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, bool write) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t pairs = p.m * p.topk;
-  int32_t *slots = reinterpret_cast<int32_t *>(scratch + WARPS * p.experts), *counts = slots + pairs;
-  for (uint32_t tok = warp; tok < p.m; tok += WARPS) route_token(p, tok, scratch + warp * p.experts, slots, lane, write);
+  const int32_t pairs = (int32_t)(p.m * p.topk), filled = (pairs + 3) & ~3;
+  int32_t *slots = reinterpret_cast<int32_t *>(scratch);
+  uint32_t *met = scratch + filled, *keys = met + 32;
+  if (threadIdx.x < 32) met[threadIdx.x] = 0u;
+  if ((int32_t)threadIdx.x < filled - pairs) slots[pairs + threadIdx.x] = -1;
+  for (uint32_t tok = warp; tok < p.m; tok += WARPS) route_token(p, tok, keys + warp * p.experts, slots, lane, write);
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < p.experts; e += THREADS) {
-    int32_t c = 0;
-    for (uint32_t i = 0; i < pairs; ++i) c += slots[i] == (int32_t)e;
-    counts[e] = c;
+  const int32_t per = (pairs + THREADS - 1) / THREADS;  // at most 2048 pairs: 4 to a thread
+  int32_t before[4], same[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int32_t i = (int32_t)threadIdx.x + q * THREADS, e = q < per && i < pairs ? slots[i] : -1;
+    before[q] = same[q] = 0;
+    if (e >= 0) {
+      int32_t less = 0, earlier = 0;
+      for (int32_t j = 0; j < filled; j += 4) {
+        const int4 s = *reinterpret_cast<const int4 *>(slots + j);
+        less += ((uint32_t)s.x < (uint32_t)e) + ((uint32_t)s.y < (uint32_t)e) + ((uint32_t)s.z < (uint32_t)e) + ((uint32_t)s.w < (uint32_t)e);
+        earlier += (s.x == e && j < i) + (s.y == e && j + 1 < i) + (s.z == e && j + 2 < i) + (s.w == e && j + 3 < i);
+        same[q] += (s.x == e) + (s.y == e) + (s.z == e) + (s.w == e);
+      }
+      out.pairs[less + earlier] = i;
+      before[q] = earlier == 0 ? less : -1;  // the first pair of its expert
+      if (earlier == 0) atomicOr(met + (e >> 5), 1u << (e & 31));
+    } else {
+      before[q] = -1;
+    }
   }
   __syncthreads();
-  if (warp == 0) {  // experts in ascending order: position in the list, first pair, first turn
-    int32_t n = 0, first = 0, turn = 0;
-    for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
-      const uint32_t e = e0 + lane;
-      const int32_t c = e < p.experts ? counts[e] : 0, q = (c + (int32_t)p.per_pass - 1) / (int32_t)p.per_pass;
-      const uint32_t met = __ballot_sync(0xFFFFFFFFu, c > 0);
-      int32_t ci = c, qi = q;
+  int32_t n = 0, total = 0;
+  for (int w = 0; w < 32; ++w) n += __popc(met[w]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (before[q] >= 0) {
+      const int32_t e = slots[threadIdx.x + q * THREADS];
+      int32_t a = __popc(met[e >> 5] & ((1u << (e & 31)) - 1u));
+      for (int w = 0; w < e >> 5; ++w) a += __popc(met[w]);
+      out.expert[a] = e;
+      out.first[a] = before[q];
+      if (a == n - 1) out.first[n] = before[q] + same[q];
+    }
+  }
+  if (n == 0 && threadIdx.x == 0) out.first[0] = 0;
+  __syncthreads();
+  if (warp == 0) {  // turns: passes over the experts before
+    for (int32_t a0 = 0; a0 < n; a0 += 32) {
+      const int32_t a = a0 + lane;
+      const int32_t c = a < n ? (out.first[a + 1] - out.first[a] + (int32_t)p.per_pass - 1) / (int32_t)p.per_pass : 0;
+      int32_t incl = c;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int32_t a = __shfl_up_sync(0xFFFFFFFFu, ci, off), b = __shfl_up_sync(0xFFFFFFFFu, qi, off);
-        if (lane >= off) ci += a, qi += b;
+        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, incl, off);
+        if (lane >= off) incl += o;
       }
-      if (c > 0) {
-        const int32_t a = n + __popc(met & ((1u << lane) - 1u));
-        out.expert[a] = (int32_t)e;
-        out.first[a] = first + ci - c;
-        out.turn[a] = turn + qi - q;
-      }
-      if (e < p.experts) counts[e] = first + ci - c;
-      n += __popc(met);
-      first += __shfl_sync(0xFFFFFFFFu, ci, 31);
-      turn += __shfl_sync(0xFFFFFFFFu, qi, 31);
+      if (a < n) out.turn[a] = total + incl - c;
+      total += __shfl_sync(0xFFFFFFFFu, incl, 31);
     }
     if (lane == 0) {
+      out.turn[n] = total;
       *out.n = n;
-      out.first[n] = first;
-      out.turn[n] = turn;
     }
-  }
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e < p.experts; e += THREADS) {
-    int32_t at = counts[e];
-    for (uint32_t i = 0; i < pairs; ++i)
-      if (slots[i] == (int32_t)e) out.pairs[at++] = (int32_t)i;
   }
   __syncthreads();
   if (write) {
-    const int32_t n = *out.n;
     if (threadIdx.x == 0) *p.list.n = n;
     for (int32_t i = threadIdx.x; i < n; i += THREADS) p.list.expert[i] = out.expert[i];
-    for (int32_t i = threadIdx.x; i <= n; i += THREADS) p.list.first[i] = out.first[i], p.list.turn[i] = out.turn[i];
+    for (int32_t i = threadIdx.x; i <= n; i += THREADS) p.list.first[i] = out.first[i];
     for (int32_t i = threadIdx.x; i < out.first[n]; i += THREADS) {
       const int32_t pair = out.pairs[i];
       p.list.pairs[i] = pair;
@@ -229,7 +267,7 @@ struct UpLayout {
   __host__ __device__ UpLayout(const MoeParams &p) {
     using F = Format<MX>;
     const uint32_t steps = F::steps(p.d), pairs = p.m * p.topk;
-    const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (WARPS * p.experts + pairs + p.experts) * 4u;
+    const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (pairs + 3u + 32u + (p.experts > 128u ? WARPS * p.experts : 0u)) * 4u;
     x = ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
     sums = x + (MX ? 0u : p.per_pass * F::x_pitch(steps));
     sums_half = UP_ROUND<MX> * WARPS * PASS * 16u;
@@ -729,10 +767,10 @@ extern "C" int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64
   return m <= MAX_TOKENS && d <= 32768 && f <= 32768 && experts <= MAX_EXPERTS && topk <= MAX_TOPK;
 }
 
-// h [m * topk][f] fp32, then n, expert[], first[], turn[], pairs[], token[], gate[]
+// h [m * topk][f] fp32, then n, expert[], first[], pairs[], token[], gate[]
 extern "C" size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk) {
   const size_t pairs = (size_t)(m * topk), met = pairs < experts ? pairs : (size_t)experts;
-  return (pairs * (size_t)f + 1 + met + 2 * (met + 1) + 3 * pairs) * 4;
+  return (pairs * (size_t)f + 1 + met + met + 1 + 3 * pairs) * 4;
 }
 
 extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
@@ -750,8 +788,8 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.list.n = (int32_t *)(p.h + pairs * p.f);
   p.list.expert = p.list.n + 1;
   p.list.first = p.list.expert + met;
-  p.list.turn = p.list.first + met + 1;
-  p.list.pairs = p.list.turn + met + 1;
+  p.list.turn = nullptr;
+  p.list.pairs = p.list.first + met + 1;
   p.list.token = p.list.pairs + pairs;
   p.list.gate = (float *)(p.list.token + pairs);
   cudaStream_t s = (cudaStream_t)stream;
