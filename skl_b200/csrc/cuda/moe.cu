@@ -9,12 +9,13 @@
 // ring in shared memory (mxf4_mma.cuh), so that about 100 KB are in flight on an SM and no weight is read twice:
 //   up     every CTA finds the routing itself (a warp per token; cheaper than a kernel before it) and takes an equal run of the
 //          tiles of all met experts, 8 gate rows with their 8 up rows to a tile, so that both sums of a feature end in the
-//          same CTA.  Warps split d, their sums meet in shared memory, where h is formed; h stays fp32.
+//          same CTA.  Warps split d, their sums meet in shared memory, where h is formed.
 //   down   a CTA owns up to 16 rows of W2 of every expert, so nothing has to be added across CTAs; its warps take (expert,
 //          piece of f) items in turn, each adding gate * product to sums of its own, which are added in order at the end.
 // Columns of the mma hold the tokens of an expert, at most 4 at a time.  16-bit weights: mma.sync bf16; x enters as it is, h as
 // the sum of two bf16 values in two columns (16 significant bits, so that h is not rounded to 8).  4-bit weights:
-// mxf4_mma.cuh; h enters as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result).
+// mxf4_mma.cuh; h is kept as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result), which
+// every CTA of `down` can copy as it is: converting fp32 there took as many instructions as the products.
 #include "mxf4_mma.cuh"
 
 namespace sklb {
@@ -43,21 +44,21 @@ struct MoeParams {
   uint16_t *y;
   int64_t rsy;
   int32_t *ids;
-  float *gates, *h;
+  float *gates;
+  float *h;        // 16-bit weights: [pairs][f]
+  uint16_t *h16;   // 4-bit weights: [pairs][f up to a multiple of 32] and a factor per block [pairs][blocks]
+  float *hf;
   Lists list;  // in the workspace, for the second kernel
   uint32_t m, d, f, experts, topk, met;  // met: the most experts that can be met
   uint32_t per_pass, k_warps, down_rows;
   int renormalise, x_vec, h_vec;
 };
 
-// What differs between the two weight formats: elements of a 128-byte step, bytes of a slot, elements of an item of `down`
-// and its slots.
+// What differs between the two weight formats: elements of a 128-byte step and bytes of a slot.
 template <bool MX>
 struct Format {
   static constexpr uint32_t K = MX ? 256 : 64;
   static constexpr uint32_t SLOT = MX ? SLOT_BYTES : CODE_BYTES;
-  static constexpr uint32_t ITEM = MX ? 256 : 128;
-  static constexpr uint32_t ITEM_SLOTS = ITEM / K;
   static __host__ __device__ uint32_t row_bytes(uint32_t cols) { return MX ? (cols + 31u) / 32u * 16u : cols * 2u; }
   static __host__ __device__ uint32_t steps(uint32_t cols) { return (cols + K - 1u) / K; }
   // a token's bf16 activations in shared memory: a pitch 64 bytes more than a multiple of 128, so that the rows of an mma
@@ -66,6 +67,7 @@ struct Format {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__host__ __device__ __forceinline__ uint32_t h_pitch(uint32_t f) { return (f + 31u) / 32u * 32u; }
 
 // ------------------------------------------------------------------------------------------------------------ route
 // order-preserving key of a logit: larger value, larger key; NaN above everything, -0 equal to +0; 0 is never a value's key
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const UpLayout<MX> at(p);
-  const uint32_t steps = F::steps(p.d), row_bytes = F::row_bytes(p.d), kblocks = (p.d + 31u) / 32u, tiles = (p.f + 7u) / 8u;
+  const uint32_t steps = F::steps(p.d), row_bytes = F::row_bytes(p.d), kblocks = (p.d + 31u) / 32u;
+  const uint32_t tiles = MX ? (p.f + 31u) / 32u * 4u : (p.f + 7u) / 8u;  // 4-bit weights: whole blocks of 32 features
   const uint32_t x = smem_addr(smem) + at.x, x_pitch = F::x_pitch(steps), ring = smem_addr(smem) + warp * (UP_DEPTH * F::SLOT);
   float *sums = reinterpret_cast<float *>(smem + at.sums);
   Lists list;
@@ -347,8 +350,9 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   dep_wait();
   route(p, reinterpret_cast<uint32_t *>(smem), list, blockIdx.x == 0);
   const int32_t n = *list.n;
-  const uint64_t total = (uint64_t)list.turn[n] * tiles;  // every pass over an expert counts
-  const uint32_t u0 = (uint32_t)(total * blockIdx.x / gridDim.x), u1 = (uint32_t)(total * (blockIdx.x + 1) / gridDim.x);
+  constexpr uint32_t UNIT = MX ? 4 : 1;  // tiles that stay together
+  const uint64_t total = (uint64_t)list.turn[n] * (tiles / UNIT);  // every pass over an expert counts
+  const uint32_t u0 = (uint32_t)(total * blockIdx.x / gridDim.x) * UNIT, u1 = (uint32_t)(total * (blockIdx.x + 1) / gridDim.x) * UNIT;
   __syncthreads();  // the routing's scratch becomes the rings
 
   const uint32_t KW = p.k_warps, TW = WARPS / KW, kw = warp % KW, tw = warp / KW;
@@ -475,15 +479,23 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
     const uint32_t feats = 8u * (r1 - r0);
     for (uint32_t i = threadIdx.x; i < feats * cnt; i += THREADS) {
       const uint32_t j = i / feats, c = i - j * feats;
-      const uint32_t feature = (r0 - turn * tiles) * 8u + c;
-      if (feature < p.f) {
-        const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
-        float gate = 0.0f, up = 0.0f;
-        for (uint32_t q = 0; q < KW; ++q) {
-          gate += s[q * (PASS * 16)];
-          up += s[q * (PASS * 16) + 8];
-        }
-        p.h[(uint64_t)list.pairs[pair0 + j] * p.f + feature] = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
+      const uint32_t feature = (r0 - turn * tiles) * 8u + c, pair = (uint32_t)list.pairs[pair0 + j];
+      const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
+      float gate = 0.0f, up = 0.0f;
+      for (uint32_t q = 0; q < KW; ++q) {
+        gate += s[q * (PASS * 16)];
+        up += s[q * (PASS * 16) + 8];
+      }
+      float h = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
+      if (MX) {  // a warp has a block of 32 features (feats is a multiple of 32)
+        if (feature >= p.f) h = 0.0f;
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, f2u(h) & 0x7FFFFFFFu);
+        float back;
+        const float factor = block_factor(top, back);
+        p.h16[(uint64_t)pair * h_pitch(p.f) + feature] = (uint16_t)(pack_f16x2_no_nan(h * factor, 0.0f) & 0xFFFFu);
+        if (lane == 0) p.hf[(uint64_t)pair * (h_pitch(p.f) / 32u) + feature / 32u] = back;
+      } else if (feature < p.f) {
+        p.h[(uint64_t)pair * p.f + feature] = h;
       }
     }
     half ^= 1u;
@@ -492,49 +504,181 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- down
-// Shared memory: rings | per warp: h of an item (4-bit: fp16 [4][256] and factors [4][8]; 16-bit: bf16, the
-// first parts of four tokens, then the second parts, [8][128] with a pitch of 320 bytes) | per warp: sums [m][16]
-template <bool MX, int DEPTH>
-struct DownLayout {
-  static constexpr uint32_t PITCH = MX ? 512 : 320;
-  static constexpr uint32_t STAGE = MX ? PASS * PITCH + PASS * 32 : 2 * PASS * PITCH;
-  static constexpr uint32_t STAGES = WARPS * DEPTH * Format<MX>::SLOT, SUMS = STAGES + WARPS * STAGE;
-  static size_t total(uint32_t m) { return SUMS + (size_t)WARPS * m * 16 * 4; }
-};
+// The warps' sums [warp][m][16], in order, into y
+__device__ __forceinline__ void add_up(const MoeParams &p, const float *sums, uint32_t row0, uint32_t nrows) {
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < p.m * 16u; i += THREADS) {
+    const uint32_t tok = i >> 4, r = i & 15u;
+    float s = sums[i];
+#pragma unroll
+    for (int q = 1; q < WARPS; ++q) s += sums[(size_t)q * p.m * 16 + i];
+    if (r < nrows) p.y[(int64_t)tok * p.rsy + row0 + r] = (uint16_t)enc_bf16(s);
+  }
+}
 
-template <bool MX, int MODE, int DEPTH>
-__global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
-  using F = Format<MX>;
-  using L = DownLayout<MX, DEPTH>;
-  constexpr int PER = F::ITEM / 32;  // elements of an item that a lane converts
+// 4-bit weights.  A slot of a ring holds an item: 16 rows x 256 elements of W2 and the h of up to PASS of the expert's pairs, fp16
+// [4][256] and factors [4][8], all by cp.async, so that a warp does little more than multiply.  Shared memory: rings | per warp:
+// sums [m][16]
+constexpr uint32_t H_BYTES = PASS * 512 + PASS * 32, DOWN_SLOT = SLOT_BYTES + H_BYTES;
+
+template <int MODE, int DEPTH>
+__global__ void __launch_bounds__(THREADS, 1) down_mx_kernel(const MoeParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t row0 = blockIdx.x * p.down_rows, nrows = min(p.down_rows, p.d - row0);
-  const uint32_t row_bytes = F::row_bytes(p.f), kblocks = (p.f + 31u) / 32u;
-  const uint32_t ring = smem_addr(smem) + warp * (DEPTH * F::SLOT);
-  const uint32_t stage = smem_addr(smem) + L::STAGES + warp * L::STAGE, factors = stage + PASS * L::PITCH;
-  float *sums = reinterpret_cast<float *>(smem + L::SUMS), *own = sums + (size_t)warp * p.m * 16;
+  const uint32_t kblocks = (p.f + 31u) / 32u, row_bytes = kblocks * 16u, pitch = kblocks * 32u;
+  const uint32_t ring = smem_addr(smem) + warp * (DEPTH * DOWN_SLOT);
+  float *sums = reinterpret_cast<float *>(smem + WARPS * DEPTH * DOWN_SLOT), *own = sums + (size_t)warp * p.m * 16;
   for (uint32_t i = lane; i < p.m * 16u; i += 32u) own[i] = 0.0f;
   __syncwarp();
   dep_wait();
 
-  const uint32_t parts = (p.f + F::ITEM - 1u) / F::ITEM, items = (uint32_t)*p.list.n * parts;
+  const uint32_t parts = (p.f + STEP - 1u) / STEP, items = (uint32_t)*p.list.n * parts;
   // a row that does not exist may lie outside the matrix, its pointer is never followed
   TileRows rows;
   rows.has[0] = g < nrows, rows.has[1] = g + 8u < nrows, rows.has_scale = (uint32_t)(lane >> 1) < nrows;
   const uint64_t expert_by = (uint64_t)p.d * row_bytes, first_row = (uint64_t)(row0 + g) * row_bytes + 16 * t;
+  const uint32_t by_a = WARPS / parts, by_part = WARPS % parts;  // an item ahead: WARPS parts further
+  // h of the pairs `at` .. `last` - 1, at most PASS, elements 256 part ..
+  auto load_h = [&](uint32_t slot, int32_t at, int32_t last, uint32_t part) {
+    const uint32_t h = slot + SLOT_BYTES, col = part * STEP + lane * 8u;
+#pragma unroll
+    for (int j = 0; j < PASS; ++j)
+      if (at + j < last) cp_async16(h + j * 512 + lane * 16, p.h16 + (uint64_t)p.list.pairs[at + j] * pitch + min(col, pitch - 8u), col < pitch ? 16u : 0u);
+    const int32_t j = lane >> 3;  // the factors: 8 lanes to a pair
+    const uint32_t blk = part * 8u + (lane & 7);
+    if (at + j < last)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(h + PASS * 512 + lane * 4),
+                   "l"(p.hf + (uint64_t)p.list.pairs[at + j] * kblocks + min(blk, kblocks - 1u)), "r"(blk < kblocks ? 4u : 0u)
+                   : "memory");
+  };
+  uint32_t fill_item = warp, fill_a = warp / parts, fill_part = warp % parts, fill_at = 0;
+  auto fill = [&]() {
+    if (fill_item < items) {
+      const uint32_t slot = ring + fill_at * DOWN_SLOT;
+      const uint64_t e = (uint64_t)p.list.expert[fill_a];
+      rows.code[0] = p.w2 + e * expert_by + first_row;
+      rows.code[1] = rows.code[0] + 8u * row_bytes;
+      rows.scale = p.s2 + (e * p.d + row0 + (lane >> 1)) * kblocks;
+      fill_slot<true, MODE>(slot, rows, fill_part, row_bytes, lane);
+      load_h(slot, p.list.first[fill_a], p.list.first[fill_a + 1], fill_part);
+      fill_item += WARPS, fill_a += by_a, fill_part += by_part;
+      if (fill_part >= parts) fill_part -= parts, ++fill_a;
+    }
+    cp_commit();
+    fill_at = fill_at + 1 == DEPTH ? 0 : fill_at + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; ++i) fill();
+
+  uint32_t a = warp / parts, part = warp % parts, at_slot = 0;
+  for (uint32_t item = warp; item < items; item += WARPS) {
+    const uint32_t slot = ring + at_slot * DOWN_SLOT, h = slot + SLOT_BYTES;
+    const int32_t first = p.list.first[a], last = p.list.first[a + 1];
+    cp_wait<DEPTH - 2>();
+    __syncwarp();
+    fill();
+    for (int32_t at = first; at < last; at += PASS) {
+      const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)PASS);
+      if (at != first) {  // more pairs than a slot holds: fetched when they are needed
+        __syncwarp();
+        load_h(slot, at, last, part);
+        cp_commit();
+        cp_wait<0>();
+        __syncwarp();
+      }
+      // where this lane's sums go: tokens t / 2 and 2 + t / 2 of the pass
+      const int32_t at0 = at + (int32_t)min((uint32_t)(t >> 1), cnt - 1u), at1 = at + (int32_t)min(2u + (uint32_t)(t >> 1), cnt - 1u);
+      float *own0 = own + p.list.token[at0] * 16 + g, *own1 = own + p.list.token[at1] * 16 + g;
+      const float gate0 = p.list.gate[at0], gate1 = p.list.gate[at1];
+      // tokens 2 q and 2 q + 1 of the pass as the columns of a group
+      auto columns = [&](Columns &c, int q) {
+        const uint32_t j = 2u * q + (uint32_t)(g >> 2);
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t *w = c.v[ch] + 4 * i;
+            w[0] = w[1] = w[2] = w[3] = 0u;
+            if ((g & 3) == t && j < cnt)
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                           : "r"(h + j * 512 + ch * 256u + t * 64u + 16u * i));
+          }
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                       : "=f"(c.factor[ch][0]), "=f"(c.factor[ch][1])
+                       : "r"(h + PASS * 512 + min(2u * q + (uint32_t)(t >> 1), cnt - 1u) * 32u + ch * 16u + (uint32_t)(t & 1) * 8u));
+        }
+      };
+      float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+      if (cnt <= 2) {
+        Columns x[1];
+        float y1[1][2] = {{0.0f, 0.0f}};
+        columns(x[0], 0);
+        multiply_step<1>(slot, x, lane, y1);
+        y[0][0] = y1[0][0], y[0][1] = y1[0][1];
+      } else {
+        Columns x[2];
+        columns(x[0], 0);
+        columns(x[1], 1);
+        multiply_step<2>(slot, x, lane, y);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q == 1 && cnt <= 2) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float s = y[q][i] + __shfl_xor_sync(0xFFFFFFFFu, y[q][i], 1);
+          if ((t & 1) == 0 && 2u * q + (uint32_t)(t >> 1) < cnt) {
+            float *o = (q ? own1 : own0) + 8 * i;
+            *o = __fmaf_rn(q ? gate1 : gate0, s, *o);
+          }
+        }
+      }
+    }
+    at_slot = at_slot + 1 == DEPTH ? 0 : at_slot + 1;
+    a += by_a, part += by_part;
+    if (part >= parts) part -= parts, ++a;
+  }
+  add_up(p, sums, row0, nrows);
+}
+
+// 16-bit weights.  An item is 16 rows x 128 elements of W2, two slots of a ring; h is fetched an item ahead into registers and
+// split into two bf16 parts.  Shared memory: rings | per warp: h of an item, bf16, the first parts of four tokens, then the
+// second parts, [8][128] with a pitch of 320 bytes | per warp: sums [m][16]
+constexpr uint32_t WIDE_PITCH = 320, WIDE_STAGE = 2 * PASS * WIDE_PITCH;
+
+template <int MODE, int DEPTH>
+__global__ void __launch_bounds__(THREADS, 1) down_wide_kernel(const MoeParams p) {
+  using F = Format<false>;
+  constexpr uint32_t ITEM = 128, SLOTS = ITEM / F::K;
+  constexpr int PER = ITEM / 32;  // elements of an item that a lane converts
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t row0 = blockIdx.x * p.down_rows, nrows = min(p.down_rows, p.d - row0), row_bytes = F::row_bytes(p.f);
+  const uint32_t ring = smem_addr(smem) + warp * (DEPTH * F::SLOT);
+  const uint32_t stage = smem_addr(smem) + WARPS * DEPTH * F::SLOT + warp * WIDE_STAGE;
+  float *sums = reinterpret_cast<float *>(smem + WARPS * (DEPTH * F::SLOT + WIDE_STAGE)), *own = sums + (size_t)warp * p.m * 16;
+  for (uint32_t i = lane; i < p.m * 16u; i += 32u) own[i] = 0.0f;
+  __syncwarp();
+  dep_wait();
+
+  const uint32_t parts = (p.f + ITEM - 1u) / ITEM, items = (uint32_t)*p.list.n * parts;
+  // a row that does not exist may lie outside the matrix, its pointer is never followed
+  TileRows rows;
+  rows.has[0] = g < nrows, rows.has[1] = g + 8u < nrows, rows.has_scale = false;
+  rows.scale = nullptr;
+  const uint64_t expert_by = (uint64_t)p.d * row_bytes, first_row = (uint64_t)(row0 + g) * row_bytes + 16 * t;
   auto aim = [&](uint32_t a) {
-    const uint64_t e = (uint64_t)p.list.expert[a];
-    rows.code[0] = p.w2 + e * expert_by + first_row;
+    rows.code[0] = p.w2 + (uint64_t)p.list.expert[a] * expert_by + first_row;
     rows.code[1] = rows.code[0] + 8u * row_bytes;
-    if (MX) rows.scale = p.s2 + (e * p.d + row0 + (lane >> 1)) * kblocks;
   };
   const uint32_t by_a = WARPS / parts, by_part = WARPS % parts;  // an item ahead: WARPS parts further
   uint32_t fill_item = warp, fill_a = warp / parts, fill_part = warp % parts, fill_sub = 0, fill_at = 0;
   auto fill = [&]() {
     if (fill_item < items) {
-      fill_slot<MX, MODE>(ring + fill_at * F::SLOT, rows, fill_part * F::ITEM_SLOTS + fill_sub, row_bytes, lane);
-      if (++fill_sub == F::ITEM_SLOTS) {
+      fill_slot<false, MODE>(ring + fill_at * F::SLOT, rows, fill_part * SLOTS + fill_sub, row_bytes, lane);
+      if (++fill_sub == SLOTS) {
         fill_sub = 0;
         fill_item += WARPS, fill_a += by_a, fill_part += by_part;
         if (fill_part >= parts) fill_part -= parts, ++fill_a;
@@ -554,11 +698,8 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
       if (at + j < last) {
         const float *src = p.h + (uint64_t)p.list.pairs[at + j] * p.f + col;
         if (p.h_vec && col + PER <= p.f) {
-#pragma unroll
-          for (int q = 0; q < PER; q += 4) {
-            const float4 w = __ldcg(reinterpret_cast<const float4 *>(src + q));
-            v[j][q] = w.x, v[j][q + 1] = w.y, v[j][q + 2] = w.z, v[j][q + 3] = w.w;
-          }
+          const float4 w = __ldcg(reinterpret_cast<const float4 *>(src));
+          v[j][0] = w.x, v[j][1] = w.y, v[j][2] = w.z, v[j][3] = w.w;
         } else {
 #pragma unroll
           for (int q = 0; q < PER; ++q)
@@ -571,49 +712,17 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
 #pragma unroll
     for (int j = 0; j < PASS; ++j) {
       if ((uint32_t)j >= cnt) break;
-      if (MX) {
-        uint32_t top = 0;
+      uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int q = 0; q < PER; ++q) top = max(top, f2u(v[j][q]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        float back;
-        const float c = block_factor(top, back);
-        st_shared_v4(stage + j * L::PITCH + lane * 16u, pack_f16x2_no_nan(v[j][0] * c, v[j][1] * c), pack_f16x2_no_nan(v[j][2] * c, v[j][3] * c),
-                     pack_f16x2_no_nan(v[j][4 % PER] * c, v[j][5 % PER] * c), pack_f16x2_no_nan(v[j][6 % PER] * c, v[j][7 % PER] * c));
-        if (t == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(factors + j * 32u + g * 4u), "f"(back) : "memory");
-      } else {
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const float a = v[j][2 * q], b = v[j][2 * q + 1];
-          hi[q] = pack_bf16x2_no_nan(a, b);
-          const float a0 = u2f(hi[q] << 16), b0 = u2f(hi[q] & 0xFFFF0000u);
-          // an infinity or NaN stays in the first part
-          lo[q] = pack_bf16x2_no_nan(fabsf(a0) < INFINITY ? a - a0 : 0.0f, fabsf(b0) < INFINITY ? b - b0 : 0.0f);
-        }
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + j * L::PITCH + lane * 8u), "r"(hi[0]), "r"(hi[1]) : "memory");
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + (j + PASS) * L::PITCH + lane * 8u), "r"(lo[0]), "r"(lo[1]) : "memory");
+      for (int q = 0; q < 2; ++q) {
+        const float a = v[j][2 * q], b = v[j][2 * q + 1];
+        hi[q] = pack_bf16x2_no_nan(a, b);
+        const float a0 = u2f(hi[q] << 16), b0 = u2f(hi[q] & 0xFFFF0000u);
+        // an infinity or NaN stays in the first part
+        lo[q] = pack_bf16x2_no_nan(fabsf(a0) < INFINITY ? a - a0 : 0.0f, fabsf(b0) < INFINITY ? b - b0 : 0.0f);
       }
-    }
-  };
-  // tokens 2 q and 2 q + 1 of the staged h as the columns of a group (4-bit weights)
-  auto columns = [&](Columns &c, int q, uint32_t cnt) {
-    const uint32_t j = 2u * q + (uint32_t)(g >> 2);
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t *w = c.v[ch] + 4 * i;
-        w[0] = w[1] = w[2] = w[3] = 0u;
-        if ((g & 3) == t && j < cnt)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(stage + j * L::PITCH + ch * 256u + t * 64u + 16u * i));
-      }
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                   : "=f"(c.factor[ch][0]), "=f"(c.factor[ch][1])
-                   : "r"(factors + min(2u * q + (uint32_t)(t >> 1), cnt - 1u) * 32u + ch * 16u + (uint32_t)(t & 1) * 8u));
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + j * WIDE_PITCH + lane * 8u), "r"(hi[0]), "r"(hi[1]) : "memory");
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + (j + PASS) * WIDE_PITCH + lane * 8u), "r"(lo[0]), "r"(lo[1]) : "memory");
     }
   };
   if (fill_item < items) aim(fill_a);
@@ -625,89 +734,49 @@ __global__ void __launch_bounds__(THREADS, 1) down_kernel(const MoeParams p) {
   int32_t first = 0, last = 0;
   if ((uint32_t)warp < items) {
     first = p.list.first[a], last = p.list.first[a + 1];
-    load_h(v, first, last, part * F::ITEM);
+    load_h(v, first, last, part * ITEM);
   }
   for (uint32_t item = warp; item < items; item += WARPS) {
     uint32_t next_a = a + by_a, next_part = part + by_part;
     if (next_part >= parts) next_part -= parts, ++next_a;
     const bool more = item + WARPS < items;
     const int32_t next_first = more ? p.list.first[next_a] : 0, next_last = more ? p.list.first[next_a + 1] : 0;
-#pragma unroll
-    for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) {
-      cp_wait<DEPTH - 1 - (int)F::ITEM_SLOTS>();  // all slots of the item
-      if (s == 0) __syncwarp();
-    }
+    cp_wait<DEPTH - 1 - (int)SLOTS>();  // all slots of the item
     for (int32_t at = first; at < last; at += PASS) {
       const uint32_t cnt = min((uint32_t)(last - at), (uint32_t)PASS);
-      if (at != first) load_h(v, at, last, part * F::ITEM);
-      // where this lane's sums go: tokens 2 q + t / 2 of the pass (4-bit weights), 2 t and 2 t + 1 (16-bit)
-      const uint32_t j0 = MX ? (uint32_t)(t >> 1) : 2u * (t & 1), j1 = MX ? j0 + 2u : j0 + 1u;
-      const int32_t at0 = at + (int32_t)min(j0, cnt - 1u), at1 = at + (int32_t)min(j1, cnt - 1u);
+      if (at != first) load_h(v, at, last, part * ITEM);
+      // where this lane's sums go: tokens 2 t and 2 t + 1 of the pass
+      const uint32_t j0 = 2u * (t & 1);
+      const int32_t at0 = at + (int32_t)min(j0, cnt - 1u), at1 = at + (int32_t)min(j0 + 1u, cnt - 1u);
       float *own0 = own + p.list.token[at0] * 16 + g, *own1 = own + p.list.token[at1] * 16 + g;
       const float gate0 = p.list.gate[at0], gate1 = p.list.gate[at1];
       __syncwarp();  // the h before has been read
       store_h(v, cnt);
-      if (at + PASS >= last && more) load_h(v, next_first, next_last, next_part * F::ITEM);
+      if (at + PASS >= last && more) load_h(v, next_first, next_last, next_part * ITEM);
       __syncwarp();
-      if (MX) {
-        float y[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-        if (cnt <= 2) {
-          Columns x[1];
-          float y1[1][2] = {{0.0f, 0.0f}};
-          columns(x[0], 0, cnt);
-          multiply_step<1>(ring + slot * F::SLOT, x, lane, y1);
-          y[0][0] = y1[0][0], y[0][1] = y1[0][1];
-        } else {
-          Columns x[2];
-          columns(x[0], 0, cnt);
-          columns(x[1], 1, cnt);
-          multiply_step<2>(ring + slot * F::SLOT, x, lane, y);
-        }
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+      for (uint32_t s = 0; s < SLOTS; ++s) {
+        const uint32_t i = slot + s >= DEPTH ? slot + s - DEPTH : slot + s;
+        multiply_wide(ring + i * F::SLOT, stage + s * (F::K * 2u), WIDE_PITCH, 7u, lane, acc);
+      }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float s = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
-            const uint32_t j = 2u * q + (uint32_t)(t >> 1);
-            if ((t & 1) == 0 && j < cnt) {
-              float *o = (q ? own1 : own0) + 8 * h;
-              *o = __fmaf_rn(q ? gate1 : gate0, s, *o);
-            }
-          }
-        }
-      } else {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) {
-          const uint32_t i = slot + s >= DEPTH ? slot + s - DEPTH : slot + s;
-          multiply_wide(ring + i * F::SLOT, stage + s * (F::K * 2u), L::PITCH, 7u, lane, acc);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // columns 2 t, 2 t + 1: the first parts of the four tokens in lanes t = 0, 1, the second in 2, 3
-          const float s = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
-          const uint32_t j = 2u * t + (q & 1);
-          if (t < 2 && j < cnt) {
-            float *o = (q & 1 ? own1 : own0) + 8 * (q >> 1);
-            *o = __fmaf_rn(q & 1 ? gate1 : gate0, s, *o);
-          }
+      for (int q = 0; q < 4; ++q) {  // columns 2 t, 2 t + 1: the first parts of the four tokens in lanes t = 0, 1, the second in 2, 3
+        const float s = acc[q] + __shfl_xor_sync(0xFFFFFFFFu, acc[q], 2);
+        if (t < 2 && j0 + (q & 1) < cnt) {
+          float *o = (q & 1 ? own1 : own0) + 8 * (q >> 1);
+          *o = __fmaf_rn(q & 1 ? gate1 : gate0, s, *o);
         }
       }
     }
     __syncwarp();  // every lane has read the item's slots
 #pragma unroll
-    for (uint32_t s = 0; s < F::ITEM_SLOTS; ++s) fill();
-    slot += F::ITEM_SLOTS;
+    for (uint32_t s = 0; s < SLOTS; ++s) fill();
+    slot += SLOTS;
     if (slot >= DEPTH) slot -= DEPTH;
     a = next_a, part = next_part, first = next_first, last = next_last;
   }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < p.m * 16u; i += THREADS) {
-    const uint32_t tok = i >> 4, r = i & 15u;
-    float s = sums[i];
-#pragma unroll
-    for (int q = 1; q < WARPS; ++q) s += sums[(size_t)q * p.m * 16 + i];
-    if (r < nrows) p.y[(int64_t)tok * p.rsy + row0 + r] = (uint16_t)enc_bf16(s);
-  }
+  add_up(p, sums, row0, nrows);
 }
 
 template <auto KERNEL>
@@ -748,14 +817,22 @@ cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
   const UpLayout<MX> up(p);
   if (up.total > MAX_SMEM) return cudaErrorInvalidConfiguration;
   // an SM has room for one CTA; never more CTAs than tiles that can exist
-  const uint64_t most = (uint64_t)p.met * ((p.m + p.per_pass - 1) / p.per_pass) * ((p.f + 7) / 8);
+  const uint64_t most = (uint64_t)p.met * ((p.m + p.per_pass - 1) / p.per_pass) * (MX ? (p.f + 31) / 32 : (p.f + 7) / 8);
   cudaError_t e = launch<up_kernel<MX, MODE>>((unsigned)(most < 148 ? most : 148), up.total, s, p);
   if (e != cudaSuccess) return e;
   const uint32_t rounds = (p.d + 148u * 16u - 1u) / (148u * 16u), ctas = 148u * rounds;
   p.down_rows = (p.d + ctas - 1u) / ctas;
   const unsigned grid = (p.d + p.down_rows - 1u) / p.down_rows;
-  if (DownLayout<MX, 4>::total(p.m) <= MAX_SMEM) return launch<down_kernel<MX, MODE, 4>>(grid, DownLayout<MX, 4>::total(p.m), s, p);
-  return launch<down_kernel<MX, MODE, 3>>(grid, DownLayout<MX, 3>::total(p.m), s, p);
+  const size_t sums = (size_t)WARPS * p.m * 16 * 4;
+  if constexpr (MX) {
+    const size_t slot = (size_t)WARPS * DOWN_SLOT;
+    if (3 * slot + sums <= MAX_SMEM) return launch<down_mx_kernel<MODE, 3>>(grid, 3 * slot + sums, s, p);
+    return launch<down_mx_kernel<MODE, 2>>(grid, 2 * slot + sums, s, p);
+  } else {
+    const size_t slot = (size_t)WARPS * F::SLOT, stage = (size_t)WARPS * WIDE_STAGE;
+    if (4 * slot + stage + sums <= MAX_SMEM) return launch<down_wide_kernel<MODE, 4>>(grid, 4 * slot + stage + sums, s, p);
+    return launch<down_wide_kernel<MODE, 3>>(grid, 3 * slot + stage + sums, s, p);
+  }
 }
 
 }  // namespace
@@ -767,10 +844,15 @@ extern "C" int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64
   return m <= MAX_TOKENS && d <= 32768 && f <= 32768 && experts <= MAX_EXPERTS && topk <= MAX_TOPK;
 }
 
-// h [m * topk][f] fp32, then n, expert[], first[], pairs[], token[], gate[]
+// h, either [pairs][f] fp32 or [pairs][f up to a multiple of 32] fp16 with a factor per block, then n, expert[], first[], pairs[],
+// token[], gate[]; a multiple of 16 bytes up to the lists
+static size_t h_bytes(uint64_t pairs, uint64_t f) {
+  const size_t wide = (size_t)(pairs * f) * 4, blocks = (size_t)pairs * ((f + 31) / 32), packed = blocks * (32 * 2 + 4);
+  return ((wide > packed ? wide : packed) + 15) / 16 * 16;
+}
 extern "C" size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk) {
   const size_t pairs = (size_t)(m * topk), met = pairs < experts ? pairs : (size_t)experts;
-  return (pairs * (size_t)f + 1 + met + met + 1 + 3 * pairs) * 4;
+  return h_bytes(pairs, f) + (1 + met + met + 1 + 3 * pairs) * 4;
 }
 
 extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
@@ -784,8 +866,10 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.x_vec = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.m == 1 || p.rsx % 8 == 0);
   const size_t pairs = (size_t)p.m * p.topk, met = pairs < p.experts ? pairs : p.experts;
   p.h = (float *)q->workspace;
+  p.h16 = (uint16_t *)q->workspace;
+  p.hf = (float *)(p.h16 + pairs * h_pitch(p.f));
   p.h_vec = (reinterpret_cast<uintptr_t>(p.h) & 15u) == 0 && p.f % 4 == 0;
-  p.list.n = (int32_t *)(p.h + pairs * p.f);
+  p.list.n = (int32_t *)((uint8_t *)q->workspace + h_bytes(pairs, p.f));
   p.list.expert = p.list.n + 1;
   p.list.first = p.list.expert + met;
   p.list.turn = nullptr;
