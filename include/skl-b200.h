@@ -338,8 +338,8 @@ SKL_FUNC void skl_gemm_f16_mxf4e2m1r_f16_sm100a(size_t m, size_t n, size_t k, fl
  * minus infinity gets zeros.  Sums are fp32, h is kept in fp32 and enters the second product with at least 11 significant
  * bits, y is rounded once.
  * 1 <= topk <= 32, experts <= 1024, m <= 64, d and f from 1 to 32768; larger calls are refused (SKL_B200_ERR_UNSUPPORTED).
- * All pointers are device memory.  `workspace`: skl_b200_moe_workspace_size bytes of the caller's, 4-byte aligned (16 is
- * faster), not initialised, one for each call or captured graph that may run at the same time; ids and gates are dense
+ * All pointers are device memory.  `workspace`: skl_b200_moe_workspace_size bytes of the caller's, 4-byte aligned,
+ * not initialised, one for each call or captured graph that may run at the same time; ids and gates are dense
  * m x topk outputs.  Outputs must not overlap inputs.  Nothing is allocated, so the call can be captured. */
 SKL_FUNC size_t skl_b200_moe_workspace_size(size_t m, size_t f, size_t experts, size_t topk);
 SKL_FUNC void skl_moe_swiglu_bf16_bf16_bf16_sm100a(size_t m, size_t d, size_t f, size_t experts, size_t topk, int renormalise,

@@ -2,7 +2,8 @@
 //
 // Such a kernel may run before its predecessor on the stream has finished and waits for it with griddepcontrol.wait.  A
 // load that the compiler knows to be invariant (__ldg, a const __restrict__ pointer) could be moved above that wait, so
-// these are volatile: they stay where they are written, behind the wait.
+// these are volatile: they stay where they are written, behind the wait.  None of these kernels lets its successor start early
+// (griddepcontrol.launch_dependents): with a grid far larger than the chip in front of a kernel of clusters that hung the chip.
 #pragma once
 
 #include <cstdint>
@@ -10,7 +11,6 @@
 namespace sklb {
 
 __device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t ld_u8(const void *p) {
   uint32_t v;

@@ -262,17 +262,19 @@ template <bool MX>
 constexpr uint32_t UP_ROUND = MX ? 8 : 4;  // tiles of a warp between two barriers (16-bit weights: x takes the room)
 
 // Shared memory: rings (before them, for a moment, the routing's scratch) | 16-bit weights: x of a pass, bf16 [tokens][pitch]
-// | sums [2][round][warps along d][PASS][16] | lists
+// | sums [2][round][warps along d][tokens][16] | lists
 template <bool MX>
 struct UpLayout {
   uint32_t x, sums, sums_half, lists, total;
+  // long rows of 16-bit weights leave room for fewer tokens
+  static __host__ __device__ uint32_t sums_of_tile(uint32_t per_pass) { return (MX ? (uint32_t)PASS : per_pass) * 16u; }
   __host__ __device__ UpLayout(const MoeParams &p) {
     using F = Format<MX>;
     const uint32_t steps = F::steps(p.d), pairs = p.m * p.topk;
     const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (pairs + 3u + 32u + (p.experts > 128u ? WARPS * p.experts : 0u)) * 4u;
     x = ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
     sums = x + (MX ? 0u : p.per_pass * F::x_pitch(steps));
-    sums_half = UP_ROUND<MX> * WARPS * PASS * 16u;
+    sums_half = UP_ROUND<MX> * WARPS * sums_of_tile(p.per_pass);
     lists = sums + 2u * sums_half * 4u;
     total = lists + (1u + p.met + 2u * (p.met + 1u) + pairs) * 4u;
   }
@@ -414,6 +416,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
     const uint32_t pair0 = (uint32_t)list.first[a] + (turn - (uint32_t)list.turn[a]) * p.per_pass;
     const uint32_t cnt = min(p.per_pass, (uint32_t)list.first[a + 1] - pair0);
     float *round = sums + half * at.sums_half;
+    const uint32_t tile_sums = UpLayout<MX>::sums_of_tile(p.per_pass);
     if (MX) {
       if (now.v < r1) {
         for (uint32_t step = kw; step < steps; step += KW) {
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
         __syncthreads();
       }
       for (uint32_t v = now.v; v < r1; v += TW) {
-        float *own = round + ((v - r0) * KW + kw) * (PASS * 16);
+        float *own = round + ((v - r0) * KW + kw) * tile_sums;
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (uint32_t step = kw; step < steps; step += KW) {
           cp_wait<UP_DEPTH - 2>();
@@ -470,7 +473,8 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
         }
         if (t < 2) {  // columns 2 t and 2 t + 1 of the four tokens
 #pragma unroll
-          for (int q = 0; q < 4; ++q) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
+          for (int q = 0; q < 4; ++q)
+            if (2u * t + (q & 1) < cnt) own[(2 * t + (q & 1)) * 16 + g + 8 * (q >> 1)] = acc[q];
         }
       }
     }
@@ -480,11 +484,11 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
     for (uint32_t i = threadIdx.x; i < feats * cnt; i += THREADS) {
       const uint32_t j = i / feats, c = i - j * feats;
       const uint32_t feature = (r0 - turn * tiles) * 8u + c, pair = (uint32_t)list.pairs[pair0 + j];
-      const float *s = round + (c >> 3) * KW * (PASS * 16) + j * 16 + (c & 7u);
+      const float *s = round + (c >> 3) * KW * tile_sums + j * 16 + (c & 7u);
       float gate = 0.0f, up = 0.0f;
       for (uint32_t q = 0; q < KW; ++q) {
-        gate += s[q * (PASS * 16)];
-        up += s[q * (PASS * 16) + 8];
+        gate += s[q * tile_sums];
+        up += s[q * tile_sums + 8];
       }
       float h = __fmul_rn(__fmul_rn(logistic_f32(1.0f, gate), gate), up);
       if (MX) {  // a warp has a block of 32 features (feats is a multiple of 32)
@@ -844,7 +848,7 @@ extern "C" int skl_b200_moe_supported(uint64_t m, uint64_t d, uint64_t f, uint64
   return m <= MAX_TOKENS && d <= 32768 && f <= 32768 && experts <= MAX_EXPERTS && topk <= MAX_TOPK;
 }
 
-// h, either [pairs][f] fp32 or [pairs][f up to a multiple of 32] fp16 with a factor per block, then n, expert[], first[], pairs[],
+// Up to 12 bytes that bring the workspace to a 16-byte boundary, h, either [pairs][f] fp32 or [pairs][f up to a multiple of 32] fp16 with a factor per block, then n, expert[], first[], pairs[],
 // token[], gate[]; a multiple of 16 bytes up to the lists
 static size_t h_bytes(uint64_t pairs, uint64_t f) {
   const size_t wide = (size_t)(pairs * f) * 4, blocks = (size_t)pairs * ((f + 31) / 32), packed = blocks * (32 * 2 + 4);
@@ -852,7 +856,7 @@ static size_t h_bytes(uint64_t pairs, uint64_t f) {
 }
 extern "C" size_t skl_b200_moe_scratch_bytes(uint64_t m, uint64_t f, uint64_t experts, uint64_t topk) {
   const size_t pairs = (size_t)(m * topk), met = pairs < experts ? pairs : (size_t)experts;
-  return h_bytes(pairs, f) + (1 + met + met + 1 + 3 * pairs) * 4;
+  return 12 + h_bytes(pairs, f) + (1 + met + met + 1 + 3 * pairs) * 4;
 }
 
 extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
@@ -865,11 +869,12 @@ extern "C" int skl_b200_launch_moe(const skl_b200_moe_args *q, void *stream) {
   p.m = q->m, p.d = q->d, p.f = q->f, p.experts = q->experts, p.topk = q->topk, p.renormalise = q->renormalise;
   p.x_vec = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && (p.m == 1 || p.rsx % 8 == 0);
   const size_t pairs = (size_t)p.m * p.topk, met = pairs < p.experts ? pairs : p.experts;
-  p.h = (float *)q->workspace;
-  p.h16 = (uint16_t *)q->workspace;
+  uint8_t *work = (uint8_t *)((reinterpret_cast<uintptr_t>(q->workspace) + 15u) / 16u * 16u);
+  p.h = (float *)work;
+  p.h16 = (uint16_t *)work;
   p.hf = (float *)(p.h16 + pairs * h_pitch(p.f));
-  p.h_vec = (reinterpret_cast<uintptr_t>(p.h) & 15u) == 0 && p.f % 4 == 0;
-  p.list.n = (int32_t *)((uint8_t *)q->workspace + h_bytes(pairs, p.f));
+  p.h_vec = p.f % 4 == 0;
+  p.list.n = (int32_t *)(work + h_bytes(pairs, p.f));
   p.list.expert = p.list.n + 1;
   p.list.first = p.list.expert + met;
   p.list.turn = nullptr;

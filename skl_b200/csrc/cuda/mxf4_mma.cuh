@@ -62,12 +62,9 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// `bytes`: how much of the 16 (8) is read, the rest is zeros
+// `bytes`: how much of the 16 is read, the rest is zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // How a lane addresses the 16 rows of a tile: rows g and g + 8 for the codes (from byte 16 t on), row lane / 2 for the scales;

@@ -9,15 +9,16 @@
 // three, but their range of exponents rounds what is 2^-20 of a block's largest.)  Products with E2M1 are exact, sums fp32.
 // A block with an infinity or a NaN gets NaN scales: the row's results are NaN.
 //
-// planes_kernel writes the planes, below each other, and lays their scales out the way tcgen05.cp takes them (512 bytes for 128
-// rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows by
-// up to 256 rows of W per CTA, k split over a cluster of CTAs so that the chip is full.  A stage holds as
-// few tiles of A as the planes of its rows need: all planes below each other in one (42 bf16, 32 fp16 rows), pairs of planes
-// (64 rows), or each plane its own; the MMAs add over the tiles, the epilogue over the planes of a tile.  Warp 0 loads planes and scales by TMA, eight warps bring
-// the packed weights through registers to where the instruction wants them, 16 elements to 16 bytes, and their scales (the TMA's
-// own spreading copy of 4-bit elements took 1.1 us for a stage's 256 x 128, several times what HBM needs for them); warp 1 copies the scales
-// to TMEM and issues the MMAs (K = 32 each, 4 to a stage and tile).  At the end all warps read the accumulator, the cluster adds
-// its parts through distributed shared memory in a fixed order, and every CTA stores a share of the rows.  Every wait is bounded.
+// planes_kernel writes the planes, below each other, and lays their scales out the way tcgen05.cp takes them (512 bytes for
+// 128 rows and 4 blocks of k: row r at (r % 32) * 16 + (r / 32) * 4).  The product kernel: one tile of 128 rows by up to 256
+// rows of W per CTA, k split over a cluster of CTAs so that the chip is full.  A stage holds as few tiles of A as the planes of
+// its rows need: all planes below each other in one (42 bf16, 32 fp16 rows), pairs of planes (64 rows), or each plane its own;
+// the MMAs add over the tiles, the epilogue over the planes of a tile.  Warp 0 loads planes and scales by TMA; eight warps bring
+// the packed weights through registers to where the instruction wants them, 16 elements to 16 bytes, and their scales (the
+// TMA's own spreading copy of 4-bit elements took 1.1 us for a stage's 256 x 128, several times what HBM needs for them);
+// warp 1 copies the scales to TMEM and issues the MMAs (K = 32 each, 4 to a stage and tile).  At the end all warps read the
+// accumulator, the cluster adds its parts through distributed shared memory in a fixed order, and every CTA stores a share of
+// the rows.  Every wait is bounded.
 #include <cuda.h>
 
 #include "loads.cuh"
@@ -117,7 +118,8 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 // ------------------------------------------------------------------------------------------------------------ planes
 // One thread for 8 elements of k, four lanes to a block; plane p of row r is row (p / fold) * tile_span + (p % fold) * m + r.
 // PLANES fills whole tiles: planes that are not needed (their elements come out as zeros) are written like the others.  Rows
-// that no plane has are not written, nor are their scales: whatever lies there only reaches accumulator rows that are not used.  `stages` * 128 is the k of the planes; the elements behind k are zeros.
+// that no plane has are not written, nor are their scales: whatever lies there only reaches accumulator rows that are not
+// used.  `stages` * 128 is the k of the planes; the elements behind k are zeros.
 template <int PLANES>
 __global__ void __launch_bounds__(256)
     planes_kernel(uint8_t *__restrict__ planes, uint8_t *__restrict__ sfa, const uint16_t *a, int64_t rsa, int m, int k, int stages,
@@ -519,7 +521,7 @@ cudaError_t launch_product(const CUtensorMap &tma, PlanesParams &p, cudaStream_t
   if (e != cudaSuccess) return e;
   Device &d = devices[dev & 63];
   cudaLaunchAttribute attr[2];
-  if (!d.ready) {
+  if (!__atomic_load_n(&d.ready, __ATOMIC_ACQUIRE)) {  // threads that meet here find the same values
     e = cudaFuncSetAttribute(product_kernel<PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PLANES>::SMEM);
     if (e != cudaSuccess) return e;
     for (int i = 0; i < 4; ++i) {
@@ -533,7 +535,7 @@ cudaError_t launch_product(const CUtensorMap &tma, PlanesParams &p, cudaStream_t
       d.fit[i] = n;
     }
     if (d.fit[0] < 1) d.fit[0] = 1;
-    d.ready = true;
+    __atomic_store_n(&d.ready, true, __ATOMIC_RELEASE);
   }
   unsigned ranks = 1;
   int64_t best = INT64_MAX, tiles = 0;

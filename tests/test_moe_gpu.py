@@ -175,6 +175,36 @@ def test_strides_and_alignment(skl, mx):
 
 
 @pytest.mark.parametrize("mx", [False, True])
+def test_workspace_at_any_word(skl, mx):
+    """The workspace needs no more than its words' alignment, and no byte outside the asked-for size is touched."""
+    c = Case(5, 96, 80, 6, 3, mx)
+    for off in (4, 8, 12):
+        c.out()
+        whole = c.work
+        c.work = whole[off:]
+        c.call()
+        c.check()
+        import torch
+
+        assert torch.all(whole[:off] == 255)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_largest_routing_and_rows(skl, mx):
+    """64 tokens, 1024 experts, 32 of them to a token, rows of 32768 elements."""
+    c = Case(64, 32768, 1, 1024, 32, mx)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_long_hidden_rows(skl, mx):
+    c = Case(6, 3, 32768, 4, 2, mx)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
 def test_every_token_to_one_expert(skl, mx):
     """More tokens of one expert than a pass takes."""
     logits = np.zeros((37, 5), np.float32)
