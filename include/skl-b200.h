@@ -296,9 +296,16 @@ SKL_FUNC void skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k
  * C is rounded once.  beta == 0 does not read C; k == 0 gives beta * C.
  * A row of A that holds an infinity or a NaN gives results that are not finite where the sum is not; the results of other
  * rows do not depend on it.
- * Few rows run on a kernel that streams the packed weights once; more rows widen W exactly to bf16 in device memory taken
- * from the stream (cudaMallocAsync: captured calls own theirs, so graphs may run side by side) and run on the bf16
- * tensor-core kernel; fp16 activations then enter as the exact sum of two bf16 matrices. */
+ * Scale bytes are 0 to 252 (all that skl_cvt_<t>rc_mxf4e2m1 writes) or 255; with 253 and 254, whose largest elements are
+ * beyond 32-bit floats, results may be infinite or NaN where the sum is not.
+ * How it runs: up to 4 rows on a kernel that streams the packed weights once; up to 256 rows (bf16) or 512 (fp16), with
+ * packed rows on 8-byte boundaries, on the block-scaled tensor-core instruction; everything else, and the gradient, widens
+ * W exactly to bf16 and runs on the 16-bit tensor-core kernel, where fp16 activations enter as the exact sum of two bf16
+ * matrices.  On the first two, elements of A far below the largest of their block of 32 lose bits: bf16 elements under
+ * 2^-31 of it (first kernel), elements under 2^-29 of it (second kernel), which changes a sum by less than 2^-36 of the
+ * block's largest magnitude per element.  In the second kernel a block of A with an infinity or a NaN makes its row NaN.
+ * Scratch memory for the second and third comes from a pool of the library's own, ordered on the call's stream
+ * (cudaMallocFromPoolAsync: captured calls own theirs, so graphs may run side by side). */
 SKL_FUNC void skl_gemm_bf16_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
                                                 const uint8_t *b, size_t csb, const uint8_t *sb, size_t cssb, float beta,
                                                 float *c, size_t rsc);
