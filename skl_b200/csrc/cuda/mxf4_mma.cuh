@@ -9,8 +9,9 @@
 // (row, 4 * token + b) is the unscaled sum of block b, which is multiplied by the weight block's and the activation block's
 // scale and added to the running fp32 sum: 4 multiply-adds for 64 weights per lane.  A group of columns thus serves two
 // tokens; it stays in registers while the warp goes through its tiles (read from shared memory for each, it kept the
-// shared-memory pipe busier than the weights did).  Measured: the conversion with the mma behind it runs at 22 T elements/s on the whole chip, against 12 T that HBM
-// delivers (17/32 byte per element at 6.4 TB/s); placing the bits of bf16 with integer instructions reached 12 T.
+// shared-memory pipe busier than the weights did).  Measured: the conversion with the mma behind it runs at 22 T elements/s
+// on the whole chip, against 12 T that HBM delivers (17/32 byte per element at 6.4 TB/s); placing the bits of bf16 with
+// integer instructions reached 12 T.
 //
 // fp16 activations are used as they are.  bf16 activations are brought into fp16's range with one power of two per block of
 // 32 that puts the block's largest magnitude into [2^14, 2^15): a bf16 value has 8 significant bits, so every value down to
@@ -189,9 +190,7 @@ __device__ __forceinline__ void multiply_step(uint32_t slot, const Columns (&x)[
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[h][0]), "=r"(sc[h][1]) : "r"(slot + CODE_BYTES + (g + 8 * h) * 8));
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    float acc[TG][4];
-#pragma unroll
-    for (int q = 0; q < TG; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
+    float acc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};  // one group: two chains of dependent mmas, too
     uint32_t lo[4], hi[4];
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3])
@@ -207,8 +206,12 @@ __device__ __forceinline__ void multiply_step(uint32_t slot, const Columns (&x)[
 #pragma unroll
       for (int q = 0; q < TG; ++q) {
         mma_f16(acc[q], a[0], b[0], a[1], b[1], x[q].v[c][4 * j], x[q].v[c][4 * j + 1]);
-        mma_f16(acc[q], a[2], b[2], a[3], b[3], x[q].v[c][4 * j + 2], x[q].v[c][4 * j + 3]);
+        mma_f16(acc[TG == 1 ? 1 : q], a[2], b[2], a[3], b[3], x[q].v[c][4 * j + 2], x[q].v[c][4 * j + 3]);
       }
+    }
+    if (TG == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[0][i] += acc[1][i];
     }
     float s[2][2];  // [row half][block of this lane's pair]
 #pragma unroll
