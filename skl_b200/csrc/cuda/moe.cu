@@ -77,10 +77,11 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 }
 __device__ __forceinline__ float key_logit(uint32_t key) { return u2f((key >> 31) ? key & 0x7FFFFFFFu : ~key); }
 
-// One warp, one token: the routed slots (-1: a logit of minus infinity, which routes nowhere) and, with `write`, ids and
-// gates to global memory.  The keys stay in registers up to 128 experts, above that in `keys`, `experts` words of this warp's
+// One warp, one token: the routed slots (-1: a logit of minus infinity, which routes nowhere), the token's bit for each of its
+// experts (tokens[2][experts]) and, with `write`, ids and gates to global memory.  The keys stay in registers up to 128 experts, above that in `keys`, `experts` words of this warp's
 // shared memory.
-__device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, uint32_t *keys, int32_t *slots, int lane, bool write) {
+__device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, uint32_t *keys, int32_t *slots, uint32_t *tokens, int lane,
+                                            bool write) {
   const float *row = p.logits + (int64_t)tok * p.rsl;
   const bool small = p.experts <= 128u;
   uint32_t reg[4];  // experts lane, lane + 32, ...
@@ -138,6 +139,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
     }
   }
   if ((uint32_t)lane < p.topk) slots[tok * p.topk + lane] = routed ? my_id : -1;
+  if (routed) atomicOr(tokens + (tok >> 5) * p.experts + my_id, 1u << (tok & 31u));
   if (!write) return;
   float sum = p.renormalise ? mine : all;
 #pragma unroll
@@ -148,85 +150,83 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
   }
 }
 
-// The whole CTA: every token's choice, then the lists.  scratch: slots [m * topk, filled up to a multiple of 4 with -1] |
-// one bit for each expert that is met [32 words] | with more than 128 experts keys [warps][experts].  A thread per pair counts
-// the pairs that belong before it.
+// The whole CTA: every token's choice, then the lists.  A token has an expert at most once, so 64 bits tell an expert's tokens,
+// how many there are and which comes when; one scan over the experts places them.  (Comparing every pair with every other took
+// several times as long from 16 tokens on.)  scratch, in words: totals of the warps [32] | tokens [2][experts] | first pair of an
+// expert [experts] | slots [pairs] | with more than 128 experts keys [warps][experts].
 __device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, bool write) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int32_t pairs = (int32_t)(p.m * p.topk), filled = (pairs + 3) & ~3;
-  int32_t *slots = reinterpret_cast<int32_t *>(scratch);
-  uint32_t *met = scratch + filled, *keys = met + 32;
-  if (threadIdx.x < 32) met[threadIdx.x] = 0u;
-  if ((int32_t)threadIdx.x < filled - pairs) slots[pairs + threadIdx.x] = -1;
-  for (uint32_t tok = warp; tok < p.m; tok += WARPS) route_token(p, tok, keys + warp * p.experts, slots, lane, write);
+  const uint32_t pairs = p.m * p.topk;
+  unsigned long long *totals = reinterpret_cast<unsigned long long *>(scratch);
+  uint32_t *tokens = scratch + 32, *base = tokens + 2u * p.experts, *keys = base + p.experts + pairs;
+  int32_t *slots = reinterpret_cast<int32_t *>(base + p.experts);
+  for (uint32_t i = threadIdx.x; i < 2u * p.experts; i += THREADS) tokens[i] = 0u;
   __syncthreads();
-  const int32_t per = (pairs + THREADS - 1) / THREADS;  // at most 2048 pairs: 4 to a thread
-  int32_t before[4], same[4];
+  dep_wait();
+  for (uint32_t tok = warp; tok < p.m; tok += WARPS) route_token(p, tok, keys + warp * p.experts, slots, tokens, lane, write);
+  __syncthreads();
+  // experts 2 tid and 2 tid + 1: pairs | met << 16 | passes << 32 (at most 2048, 1024 and 2048), summed up over the experts
+  unsigned long long own[2], sum;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int32_t i = (int32_t)threadIdx.x + q * THREADS, e = q < per && i < pairs ? slots[i] : -1;
-    before[q] = same[q] = 0;
-    if (e >= 0) {
-      int32_t less = 0, earlier = 0;
-      for (int32_t j = 0; j < filled; j += 4) {
-        const int4 s = *reinterpret_cast<const int4 *>(slots + j);
-        less += ((uint32_t)s.x < (uint32_t)e) + ((uint32_t)s.y < (uint32_t)e) + ((uint32_t)s.z < (uint32_t)e) + ((uint32_t)s.w < (uint32_t)e);
-        earlier += (s.x == e && j < i) + (s.y == e && j + 1 < i) + (s.z == e && j + 2 < i) + (s.w == e && j + 3 < i);
-        same[q] += (s.x == e) + (s.y == e) + (s.z == e) + (s.w == e);
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t e = 2u * threadIdx.x + q;
+    const uint32_t c = e < p.experts ? __popc(tokens[e]) + __popc(tokens[p.experts + e]) : 0u;
+    own[q] = (unsigned long long)((c + p.per_pass - 1u) / p.per_pass) << 32 | (c != 0u ? 0x10000u : 0u) | c;
+  }
+  sum = own[0] + own[1];
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const unsigned long long o = __shfl_up_sync(0xFFFFFFFFu, sum, off);
+    if (lane >= off) sum += o;
+  }
+  if (lane == 31) totals[warp] = sum;
+  __syncthreads();
+  unsigned long long before = sum - own[0] - own[1], all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += totals[w];
+    all += totals[w];
+  }
+  const int32_t n = (int32_t)(all >> 16 & 0xFFFFu);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t e = 2u * threadIdx.x + q;
+    if (own[q] != 0) {
+      const uint32_t a = (uint32_t)(before >> 16) & 0xFFFFu, first = (uint32_t)before & 0xFFFFu;
+      base[e] = first;
+      out.expert[a] = (int32_t)e;
+      out.first[a] = (int32_t)first;
+      out.turn[a] = (int32_t)(before >> 32);
+      if (write) {
+        p.list.expert[a] = (int32_t)e;
+        p.list.first[a] = (int32_t)first;
       }
-      out.pairs[less + earlier] = i;
-      before[q] = earlier == 0 ? less : -1;  // the first pair of its expert
-      if (earlier == 0) atomicOr(met + (e >> 5), 1u << (e & 31));
-    } else {
-      before[q] = -1;
+    }
+    before += own[q];
+  }
+  if (threadIdx.x == 0) {
+    *out.n = n;
+    out.first[n] = (int32_t)(all & 0xFFFFu);
+    out.turn[n] = (int32_t)(all >> 32);
+    if (write) {
+      *p.list.n = n;
+      p.list.first[n] = (int32_t)(all & 0xFFFFu);
     }
   }
   __syncthreads();
-  int32_t n = 0, total = 0;
-  for (int w = 0; w < 32; ++w) n += __popc(met[w]);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (before[q] >= 0) {
-      const int32_t e = slots[threadIdx.x + q * THREADS];
-      int32_t a = __popc(met[e >> 5] & ((1u << (e & 31)) - 1u));
-      for (int w = 0; w < e >> 5; ++w) a += __popc(met[w]);
-      out.expert[a] = e;
-      out.first[a] = before[q];
-      if (a == n - 1) out.first[n] = before[q] + same[q];
-    }
-  }
-  if (n == 0 && threadIdx.x == 0) out.first[0] = 0;
-  __syncthreads();
-  if (warp == 0) {  // turns: passes over the experts before
-    for (int32_t a0 = 0; a0 < n; a0 += 32) {
-      const int32_t a = a0 + lane;
-      const int32_t c = a < n ? (out.first[a + 1] - out.first[a] + (int32_t)p.per_pass - 1) / (int32_t)p.per_pass : 0;
-      int32_t incl = c;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, incl, off);
-        if (lane >= off) incl += o;
-      }
-      if (a < n) out.turn[a] = total + incl - c;
-      total += __shfl_sync(0xFFFFFFFFu, incl, 31);
-    }
-    if (lane == 0) {
-      out.turn[n] = total;
-      *out.n = n;
+  for (uint32_t i = threadIdx.x; i < pairs; i += THREADS) {
+    const int32_t e = slots[i];
+    if (e < 0) continue;
+    const uint32_t tok = i / p.topk, low = tokens[e], high = tokens[p.experts + e], bits = (1u << (tok & 31u)) - 1u;
+    const uint32_t at = base[e] + (tok < 32u ? __popc(low & bits) : __popc(low) + __popc(high & bits));
+    out.pairs[at] = (int32_t)i;
+    if (write) {
+      p.list.pairs[at] = (int32_t)i;
+      p.list.token[at] = (int32_t)tok;
+      p.list.gate[at] = p.gates[i];  // written by this CTA, before a barrier
     }
   }
   __syncthreads();
-  if (write) {
-    if (threadIdx.x == 0) *p.list.n = n;
-    for (int32_t i = threadIdx.x; i < n; i += THREADS) p.list.expert[i] = out.expert[i];
-    for (int32_t i = threadIdx.x; i <= n; i += THREADS) p.list.first[i] = out.first[i];
-    for (int32_t i = threadIdx.x; i < out.first[n]; i += THREADS) {
-      const int32_t pair = out.pairs[i];
-      p.list.pairs[i] = pair;
-      p.list.token[i] = pair / (int32_t)p.topk;
-      p.list.gate[i] = p.gates[pair];  // written by this CTA, before a barrier
-    }
-  }
 }
 
 // ------------------------------------------------------------------------------------------------------ 16-bit step
@@ -271,7 +271,7 @@ struct UpLayout {
   __host__ __device__ UpLayout(const MoeParams &p) {
     using F = Format<MX>;
     const uint32_t steps = F::steps(p.d), pairs = p.m * p.topk;
-    const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (pairs + 3u + 32u + (p.experts > 128u ? WARPS * p.experts : 0u)) * 4u;
+    const uint32_t ring = WARPS * UP_DEPTH * F::SLOT, scratch = (32u + 3u * p.experts + pairs + (p.experts > 128u ? WARPS * p.experts : 0u)) * 4u;
     x = ((ring > scratch ? ring : scratch) + 15u) / 16u * 16u;
     sums = x + (MX ? 0u : p.per_pass * F::x_pitch(steps));
     sums_half = UP_ROUND<MX> * WARPS * sums_of_tile(p.per_pass);
@@ -349,7 +349,6 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   list.turn = list.first + p.met + 1;
   list.pairs = list.turn + p.met + 1;
 
-  dep_wait();
   route(p, reinterpret_cast<uint32_t *>(smem), list, blockIdx.x == 0);
   const int32_t n = *list.n;
   constexpr uint32_t UNIT = MX ? 4 : 1;  // tiles that stay together
