@@ -28,7 +28,7 @@ namespace sklb {
 namespace {
 
 constexpr int BM = 128, BN = 256, BK = 128;  // largest tile; elements of k of a stage, one byte each in shared memory
-constexpr int AHEAD = 3;                      // stages of packed weights that a loader holds in registers
+constexpr int AHEAD = 2;                      // stages of packed weights that a loader holds in registers (3 to 6: 1 to 2 us slower)
 constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
 constexpr int SF_BYTES = 512;  // scales of 128 rows and one stage
 constexpr int LOADERS = 8, THREADS = 64 + 32 * LOADERS;  // warp 0: TMA, warp 1: MMA, then the loaders
