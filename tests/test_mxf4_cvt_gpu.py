@@ -1,5 +1,5 @@
 """Quantisation to MX-FP4 and the way back, through the C ABI.  Both are defined down to the bit (the header gives scale and
-rounding), so every comparison is of bits; the checker is tests/mxf4_plain.py in 64 bits."""
+rounding), so every comparison is of bits; the oracle is tests/mxf4_plain.py in 64 bits."""
 import numpy as np
 import pytest
 

@@ -329,3 +329,83 @@ def test_quantise_multiply_and_gradient_as_a_layer_uses_them(skl):
         diff = ((forward(ub) - y) * f64("bf16", dy)).sum(1)
         slack = 2 * tolerance("f32", want, (np.abs(f64("bf16", x)) + 8) @ np.abs(W).T, k)
         assert np.all(np.abs(diff - step * dx[:, col]) <= (slack * np.abs(f64("bf16", dy))).sum(1) + 8 * 2.0 ** -16 * np.abs(wantdx).max())
+
+
+@pytest.mark.parametrize("m,ta,grad", [(2, "bf16", False), (9, "bf16", False), (9, "f16", False), (300, "bf16", False), (9, "f16", True)])
+def test_offsets_past_32_bits(skl, m, ta, grad):
+    """The last rows of every operand lie more than 4 GiB behind the first.  Whole numbers: the sums are exact."""
+    import torch
+
+    n, k = 40, 96
+    rows, length = (k, n) if grad else (n, k)
+    kb = -(-length // 32)
+    step = lambda r: (((1 << 32) // (r - 1) + 4096) // 256) * 256  # noqa: E731  bytes from row to row
+    g = H.rng(m)
+    codes, _ = MX.random_packed(g, (rows, length))
+    scales = np.full((rows, kb), 127, np.uint8)
+    a = g.integers(-8, 9, (m, k)).astype(np.float64)
+
+    def far(v):
+        v = np.ascontiguousarray(v).view(np.uint8).reshape(v.shape[0], -1)
+        by = step(v.shape[0])
+        buf = torch.empty((v.shape[0] - 1) * by + v.shape[1], dtype=torch.uint8, device="cuda")
+        torch.as_strided(buf, v.shape, (by, 1)).copy_(torch.from_numpy(v).cuda())
+        return buf, by
+
+    (da, sa), (db, sb), (ds, ss), (dc, sc) = (far(v) for v in (bits(ta, a), codes, scales, np.zeros((m, n), np.float32)))
+    fn = getattr(skl, f"skl_gemm_{ta}_mxf4e2m1{'r' if grad else ''}_f32_sm100a")
+    fn(m, n, k, 1.0, da.data_ptr(), sa // 2, db.data_ptr(), sb, ds.data_ptr(), ss, 0.0, dc.data_ptr(), sc // 4)
+    S.check()
+    got = torch.as_strided(dc, (m, 4 * n), (sc, 1)).contiguous().cpu().numpy().view(np.float32)
+    W = MX.values(codes, scales, length)
+    assert np.array_equal(got, (a @ (W if grad else W.T)).astype(np.float32))
+
+
+def test_two_threads_at_once(skl):
+    """Every path from two threads, each on a stream of its own; the calls share the library's pool of scratch memory."""
+    import threading
+
+    import torch
+
+    lib, n, k = S.lib(), 520, 1024
+    shapes = [(2, False), (30, False), (400, False), (50, True)]
+    jobs = []
+    for t in range(2):
+        g = H.rng(t)
+        for m, grad in shapes:
+            rows, length = (k, n) if grad else (n, k)
+            codes, _ = MX.random_packed(g, (rows, length))
+            scales = np.full((rows, -(-length // 32)), 127, np.uint8)
+            a = g.integers(-8, 9, (m, k)).astype(np.float64)
+            W = MX.values(codes, scales, length)
+            jobs.append((t, m, grad, *(torch.from_numpy(v.view(np.uint8)).cuda() for v in (bits("bf16", a), codes, scales)), length,
+                         torch.zeros(m, n, device="cuda"), (a @ (W if grad else W.T)).astype(np.float32)))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(t):
+        torch.cuda.set_device(0)
+        stream = torch.cuda.Stream()
+        lib.skl_b200_set_stream(stream.cuda_stream)
+        lib.skl_b200_set_async(1)
+        for _ in range(20):
+            for owner, m, grad, a, b, s, length, c, _want in jobs:
+                if owner == t:
+                    fn = lib.skl_gemm_bf16_mxf4e2m1r_f32_sm100a if grad else lib.skl_gemm_bf16_mxf4e2m1_f32_sm100a
+                    kb = -(-length // 32)
+                    fn(m, n, k, 1.0, a.data_ptr(), k, b.data_ptr(), 16 * kb, s.data_ptr(), kb, 0.0, c.data_ptr(), n)
+                    if lib.skl_b200_last_status() != 0:
+                        failed.append((t, m, grad))
+        lib.skl_b200_synchronize()
+        if lib.skl_b200_last_status() != 0:
+            failed.append((t, "synchronize"))
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    torch.cuda.synchronize()
+    for _t, m, grad, _a, _b, _s, _l, c, want in jobs:
+        assert np.array_equal(c.cpu().numpy(), want), (m, grad)
