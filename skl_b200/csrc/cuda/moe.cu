@@ -6,7 +6,8 @@
 //
 // With few tokens the layer is a stream of the met experts' weights from HBM (2 bytes or 17/32 byte per element) with a few
 // multiply-adds each.  Two kernels of one CTA of 16 warps per SM; each warp streams 16-row pieces of the weights through a
-// ring in shared memory (mxf4_mma.cuh), so that about 100 KB are in flight on an SM and no weight is read twice:
+// ring in shared memory (mxf4_mma.cuh), so that about 100 KB are in flight on an SM; weights are read once for up to 4 tokens of an
+// expert, and in `down` for any number:
 //   up     every CTA finds the routing itself (a warp per token; cheaper than a kernel before it) and takes an equal run of the
 //          tiles of all met experts, 8 gate rows with their 8 up rows to a tile, so that both sums of a feature end in the
 //          same CTA.  Warps split d, their sums meet in shared memory, where h is formed.
@@ -16,6 +17,11 @@
 // the sum of two bf16 values in two columns (16 significant bits, so that h is not rounded to 8).  4-bit weights:
 // mxf4_mma.cuh; h is kept as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result), which
 // every CTA of `down` can copy as it is: converting fp32 there took as many instructions as the products.
+//
+// d 2048, f 1024, 8 of 64 experts: one token, bf16 weights (100 MB), 25.2 us in a graph: the routing (about 5 us), two streams at
+// 6.6 TB/s, each with its start and end; MX-FP4 17.3.  16 tokens, MX-FP4 (187 MB): 72 us, 51 of them `up`; bound by the issue
+// slots (half busy) and the latency of dependent instructions, about 400 instructions of a warp for 16 x 256 weights.
+// 16 tokens, bf16: 145 us, 4.8 TB/s.
 #include "mxf4_mma.cuh"
 
 namespace sklb {

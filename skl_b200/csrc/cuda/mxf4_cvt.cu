@@ -160,6 +160,7 @@ __device__ __forceinline__ uint32_t encode_eight(const Eight<DT> &v, uint32_t &s
 // Rows with unit stride, 16-byte aligned.  Four lanes share a block: a lane takes 8 elements (one or two 16-byte loads), the
 // block's largest magnitude is two shuffles, the lane's 8 codes are one 4-byte store; loads and stores of a warp are
 // contiguous.  UNROLL groups per thread keep that many loads in flight, and the warp's 32 scale bytes leave in one store.
+// bf16 16384 x 4096: 28.9 us, 5.9 TB/s, 0.91 of a copy's rate (66 % of the issue slots are busy); fp32 14336 x 4096: 39.6 us.
 template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     quant_rows_kernel(uint8_t *__restrict__ dst, int64_t rsd, uint8_t *__restrict__ scales, int64_t rss,
@@ -383,7 +384,8 @@ __device__ __forceinline__ void store_eight(void *dst, int64_t at, const float (
 
 // A thread widens 8 elements: one 4-byte load, one (16-bit types) or two 16-byte stores; the loads and stores of a warp are
 // contiguous, its 32 scale bytes come in one load.  vec: 4-byte aligned packed rows and 16-byte aligned output rows; without
-// it, and in the ragged end of a row, single bytes and elements.
+// it, and in the ragged end of a row, single bytes and elements.  16384 x 4096 to bf16: 27.7 us, 6.1 TB/s, 0.95 of a copy's
+// rate; 14336 x 4096 to fp32: 47.8 us.
 template <int DT, int UNROLL>
 __global__ void __launch_bounds__(THREADS)
     widen_rows_kernel(void *__restrict__ dst, int64_t rsd, const uint8_t *__restrict__ src, int64_t rsa,

@@ -19,6 +19,10 @@
 // warp 1 copies the scales to TMEM and issues the MMAs (K = 32 each, 4 to a stage and tile).  At the end all warps read the
 // accumulator, the cluster adds its parts through distributed shared memory in a fixed order, and every CTA stores a share of
 // the rows.  Every wait is bounded.
+//
+// 14336 x 4096, both kernels, in a graph: 5 rows 20.2 us, 32 rows 22.3, 61 rows 27.1, 128 rows 32.6 (31 MB: 4.9 us of HBM; W
+// widened to bf16 and multiplied: 59 us); 4096 x 4096 with 5 rows 12.8, 1024 x 1024 9.0, which is what the two launches, filling
+// and emptying cost.  Beyond that a stage takes about 0.7 us: the hand-over from the loaders to the MMAs, not HBM.
 #include <cuda.h>
 
 #include "loads.cuh"
