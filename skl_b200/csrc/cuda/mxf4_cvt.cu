@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(THREADS)
 // Unit stride along the rows' index (a column of a row-major source becomes a packed row).  A lane owns RPL neighbouring
 // packed rows and a whole block of each, so the maximum is its own; the warp reads runs of 32 * RPL elements, the CTA's
 // eight warps take eight blocks of k, and the codes go through shared memory so that each packed row is written as a run of
-// 128 bytes.  RPL is chosen for 8-byte loads; 1 serves any alignment.
+// 128 bytes.  RPL is chosen for 8-byte loads; 1 serves any alignment.  fp32 14336 x 4096: 49.2 us, 5.4 TB/s, 0.84 of a copy's rate;
+// bf16 16384 x 4096: 36.8 us, 0.71, where the instructions per element (half the issue slots) weigh more against fewer bytes.
 template <int DT, int RPL>
 __global__ void __launch_bounds__(THREADS)
     quant_columns_kernel(uint8_t *__restrict__ dst, int64_t rsd, uint8_t *__restrict__ scales, int64_t rss,
