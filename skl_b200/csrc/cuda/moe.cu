@@ -838,9 +838,14 @@ cudaError_t launch_moe(MoeParams &p, cudaStream_t s) {
     if (3 * slot + sums <= MAX_SMEM) return launch<down_mx_kernel<MODE, 3>>(grid, 3 * slot + sums, s, p);
     return launch<down_mx_kernel<MODE, 2>>(grid, 2 * slot + sums, s, p);
   } else {
+    // An item of `down` is two steps: rows of whole steps may still end in the middle of an item (f an odd multiple of 64), and
+    // what lies behind a row is not the row's (nor, behind the last one, the caller's).
+    constexpr int SAFE = MODE == WHOLE ? (int)ALIGNED : MODE;
     const size_t slot = (size_t)WARPS * F::SLOT, stage = (size_t)WARPS * WIDE_STAGE;
-    if (4 * slot + stage + sums <= MAX_SMEM) return launch<down_wide_kernel<MODE, 4>>(grid, 4 * slot + stage + sums, s, p);
-    return launch<down_wide_kernel<MODE, 3>>(grid, 3 * slot + stage + sums, s, p);
+    const bool deep = 4 * slot + stage + sums <= MAX_SMEM, safe = p.f % 128u != 0;
+    const size_t smem = (deep ? 4 : 3) * slot + stage + sums;
+    if (safe) return deep ? launch<down_wide_kernel<SAFE, 4>>(grid, smem, s, p) : launch<down_wide_kernel<SAFE, 3>>(grid, smem, s, p);
+    return deep ? launch<down_wide_kernel<MODE, 4>>(grid, smem, s, p) : launch<down_wide_kernel<MODE, 3>>(grid, smem, s, p);
   }
 }
 

@@ -245,6 +245,49 @@ def test_a_masked_expert_may_hold_anything(skl, mx):
 
 
 @pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("d,f", [(64, 64), (64, 192), (128, 320), (64, 128), (72, 40)])
+def test_nothing_behind_a_row_of_the_second_weights_is_used(skl, d, f, mx):
+    """NaN in masked experts on both sides of the one that is used, and in memory behind the last row of w2: rows that are whole
+    128-byte steps but no whole items of the kernel (f = 64, 192, 320 in 16 bits) end where they end."""
+    import torch
+
+    for used in range(3):  # the used expert's last row is followed by another expert's first, or by the end of w2
+        logits = np.full((3, 3), -np.inf)
+        logits[:, used] = 1.0
+        c = Case(3, d, f, 3, 2, mx, logits=logits, seed=used)
+        for i, w in enumerate(c.w):
+            room = torch.empty(w.numel() + 4096, dtype=torch.uint8, device="cuda")
+            if mx:
+                room.fill_(255)
+            else:
+                room.view(torch.int16).fill_(0x7FFF)
+            per = w.numel() // 3
+            room[used * per:(used + 1) * per] = w[used * per:(used + 1) * per]
+            c.w[i] = room
+        for e in range(3):
+            if e != used:
+                c.w1[e], c.w2[e] = 0.0, 0.0
+        c.call()
+        c.check()
+
+
+def test_a_row_of_the_second_weights_may_hold_nan(skl):
+    """... and its NaN reaches that row's output only, not the row's before it."""
+    import torch
+
+    m, d, f = 2, 64, 192
+    c = Case(m, d, f, 2, 1, False, logits=np.array([[1.0, 0.0]] * m))
+    c.call()
+    torch.cuda.synchronize()
+    plain = c.y.clone()
+    c.w[1].view(torch.int16).view(2, d, f)[:, 1::2] = 0x7FFF
+    c.out()
+    c.call()
+    torch.cuda.synchronize()
+    assert torch.equal(c.y[:, 0:d:2], plain[:, 0:d:2]) and torch.all(torch.isnan(c.y[:, 1:d:2]))
+
+
+@pytest.mark.parametrize("mx", [False, True])
 def test_same_bits_every_time(skl, mx):
     import torch
 
