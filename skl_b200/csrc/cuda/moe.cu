@@ -34,6 +34,11 @@ constexpr int PASS = 4;  // tokens of an expert at a time
 constexpr int MAX_TOKENS = 64, MAX_EXPERTS = 1024, MAX_TOPK = 32;
 constexpr size_t MAX_SMEM = 226 * 1024;
 
+// 4-bit weights: the factors of h's blocks reach 2^113, and a block's sum of 2^23 times that would leave fp32's range before the
+// weights' scale brings it back (see Columns).  They are kept divided by this, and the gates multiplied by it; a block's sum is then
+// exact to 2^-141 times its scale.
+constexpr float H_LIFT = 512.0f;
+
 // The routed pairs (token * topk + j) sorted by expert: n experts met, in ascending order, expert[a] with the pairs
 // pairs[first[a]] .. pairs[first[a + 1] - 1], in token order; they are taken `per_pass` at a time, passes before expert a: turn[a].
 // turn[] only in the first kernel; token[], gate[]: of the pairs, in the same order, only in the workspace for the second.
@@ -160,7 +165,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, uint32_t tok, ui
 // how many there are and which comes when; one scan over the experts places them.  (Comparing every pair with every other took
 // several times as long from 16 tokens on.)  scratch, in words: totals of the warps [32] | tokens [2][experts] | first pair of an
 // expert [experts] | slots [pairs] | with more than 128 experts keys [warps][experts].
-__device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, bool write) {
+__device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, bool mx, bool write) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t pairs = p.m * p.topk;
   unsigned long long *totals = reinterpret_cast<unsigned long long *>(scratch);
@@ -229,7 +234,7 @@ __device__ void route(const MoeParams &p, uint32_t *scratch, const Lists &out, b
     if (write) {
       p.list.pairs[at] = (int32_t)i;
       p.list.token[at] = (int32_t)tok;
-      p.list.gate[at] = p.gates[i];  // written by this CTA, before a barrier
+      p.list.gate[at] = p.gates[i] * (mx ? H_LIFT : 1.0f);  // written by this CTA, before a barrier
     }
   }
   __syncthreads();
@@ -335,6 +340,7 @@ __device__ __forceinline__ void up_columns(const MoeParams &p, const int32_t *pa
       for (int i = 0; i < 4; ++i) e[2 * i] = dec_bf16(w[c][i] & 0xFFFFu), e[2 * i + 1] = u2f(w[c][i] & 0xFFFF0000u);
       gather_chunk(x[q], c, e, lane);
     }
+    limit_factors(x[q]);
   }
 }
 
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
   list.turn = list.first + p.met + 1;
   list.pairs = list.turn + p.met + 1;
 
-  route(p, reinterpret_cast<uint32_t *>(smem), list, blockIdx.x == 0);
+  route(p, reinterpret_cast<uint32_t *>(smem), list, MX, blockIdx.x == 0);
   const int32_t n = *list.n;
   constexpr uint32_t UNIT = MX ? 4 : 1;  // tiles that stay together
   const uint64_t total = (uint64_t)list.turn[n] * (tiles / UNIT);  // every pass over an expert counts
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
               fill();
               multiply_step<1>(ring + slot * F::SLOT, one, lane, y);
               slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
-              keep_sums<1>(round + ((v - r0) * KW + kw) * (PASS * 16), y, step == kw, lane);
+              keep_sums<1>(round + ((v - r0) * KW + kw) * (PASS * 16), one, y, step == kw, lane);
             }
           } else {
             if (fresh) up_columns<2>(p, list.pairs + pair0, cnt, step, lane, cols);
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
               fill();
               multiply_step<2>(ring + slot * F::SLOT, cols, lane, y);
               slot = slot + 1 == UP_DEPTH ? 0 : slot + 1;
-              keep_sums<2>(round + ((v - r0) * KW + kw) * (PASS * 16), y, step == kw, lane);
+              keep_sums<2>(round + ((v - r0) * KW + kw) * (PASS * 16), cols, y, step == kw, lane);
             }
           }
         }
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) up_kernel(const MoeParams p) {
         float back;
         const float factor = block_factor(top, back);
         p.h16[(uint64_t)pair * h_pitch(p.f) + feature] = (uint16_t)(pack_f16x2_no_nan(h * factor, 0.0f) & 0xFFFFu);
-        if (lane == 0) p.hf[(uint64_t)pair * (h_pitch(p.f) / 32u) + feature / 32u] = back;
+        if (lane == 0) p.hf[(uint64_t)pair * (h_pitch(p.f) / 32u) + feature / 32u] = back * (1.0f / H_LIFT);
       } else if (feature < p.f) {
         p.h[(uint64_t)pair * p.f + feature] = h;
       }

@@ -134,9 +134,15 @@ __device__ __forceinline__ float block_factor(uint32_t top, float &back) {
 // One group of two tokens as the mma's second operand, for one step, in registers: lane (g, t) with g % 4 == t holds block t of
 // both chunks of token g / 4 as fp16 pairs, every other lane zeros.  factor[chunk][i]: what undoes the block factors of the
 // sums this lane ends up with, token t / 2, blocks 2 (t % 2) + i.
+//
+// A step's sums y are the products' sums divided by `lift`, 1 unless the factors are very large: a block's unscaled sum is below
+// 32 * 6 * 2^15 < 2^23, and times a factor above 2^104 (activations from 2^119 on) it may leave fp32's range before the weights'
+// scale brings it back.  A lane and its neighbour, which share the token, then take 2^9 off the factors, whose largest is 2^113, and
+// `lift` gives it back to the scaled sum.  (Next to such a block the sums of others are exact to 2^-141 times their scale.)
+// A branch to another order of the two products instead cost 5 % of the experts' layer.
 struct Columns {
   uint32_t v[2][16];
-  float factor[2][2];
+  float factor[2][2], lift;
 };
 // Chunk c of a group from 8 fp32 elements of every lane: lane L brings elements 8 (L % 4) .. + 7 of block L / 4 % 4 of token
 // L / 16 (zeros where there is none).  The four lanes of a quad are the four parts of one block, and the lane that has to hold
@@ -165,6 +171,16 @@ __device__ __forceinline__ void gather_chunk(Columns &x, int c, const float (&e)
   // the factors travel to the lanes whose sums they scale: block b of token h is quad 4 h + b's
 #pragma unroll
   for (int i = 0; i < 2; ++i) x.factor[c][i] = __shfl_sync(0xFFFFFFFFu, back, 16 * (t >> 1) + 4 * (2 * (t & 1) + i));
+}
+// Behind both chunks' gather_chunk: limits the factors.
+__device__ __forceinline__ void limit_factors(Columns &x) {
+  float most = fmaxf(fmaxf(x.factor[0][0], x.factor[0][1]), fmaxf(x.factor[1][0], x.factor[1][1]));
+  most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+  const bool large = most > 0x1p104f;
+  x.lift = large ? 512.0f : 1.0f;
+  const float down = large ? 1.0f / 512.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.factor[i >> 1][i & 1] *= down;
 }
 // 8 consecutive 16-bit elements of a row (zeros from `len` on) as packed words
 __device__ __forceinline__ void load_row8(uint32_t (&w)[4], const uint16_t *row, uint32_t at, uint32_t len, bool vec) {
@@ -227,9 +243,9 @@ __device__ __forceinline__ void multiply_step(uint32_t slot, const Columns (&x)[
   }
 }
 
-// y of a tile and step into (first) or onto the warp's own sums [2 TG tokens][16 rows]
+// y of a tile and step, times lift, into (first) or onto the warp's own sums [2 TG tokens][16 rows]
 template <int TG>
-__device__ __forceinline__ void keep_sums(float *sums, float (&y)[TG][2], bool first, int lane) {
+__device__ __forceinline__ void keep_sums(float *sums, const Columns (&x)[TG], float (&y)[TG][2], bool first, int lane) {
   const int g = lane >> 2, t = lane & 3;
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(sums + (t >> 1) * 16 + g);
 #pragma unroll
@@ -237,11 +253,9 @@ __device__ __forceinline__ void keep_sums(float *sums, float (&y)[TG][2], bool f
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v = y[q][h] + __shfl_xor_sync(0xFFFFFFFFu, y[q][h], 1);
-      if (!first) {
-        float old;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(old) : "r"(at + (32 * q + 8 * h) * 4));
-        v += old;
-      }
+      float old = 0.0f;
+      if (!first) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(old) : "r"(at + (32 * q + 8 * h) * 4));
+      v = __fmaf_rn(v, x[q].lift, old);
       asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %2, 0;\n\t@p st.shared.f32 [%0], %1;\n\t}" ::"r"(at + (32 * q + 8 * h) * 4), "f"(v), "r"(t & 1)
                    : "memory");
     }

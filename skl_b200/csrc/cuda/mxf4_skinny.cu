@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParam
         }
         gather_chunk(x[q], c, e, lane);
       }
+      limit_factors(x[q]);
     }
     for (uint32_t tile = tw; tile < tiles; tile += TW) {
       float y[TG][2];
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) skinny_kernel(const SkinnyParam
       fill();
       multiply_step<TG>(ring + slot * SLOT_BYTES, x, lane, y);
       slot = slot + 1 == DEPTH ? 0 : slot + 1;
-      keep_sums<TG>(sums + (tile * KW + kw) * (2 * TG * 16), y, step == kw, lane);
+      keep_sums<TG>(sums + (tile * KW + kw) * (2 * TG * 16), x, y, step == kw, lane);
     }
   }
   __syncthreads();

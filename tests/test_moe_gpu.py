@@ -244,6 +244,30 @@ def test_a_masked_expert_may_hold_anything(skl, mx):
     c.check()
 
 
+@pytest.mark.parametrize("m", [1, 2, 5, 9])
+def test_large_values_and_small_scales(skl, m):
+    """4-bit weights: tokens near the largest bf16 numbers under small scales of w1, then h that large under small scales of w2."""
+    import torch
+
+    d, f, experts = 192, 96, 2
+    put = lambda v: torch.from_numpy(np.ascontiguousarray(v).view(np.uint8).reshape(-1)).cuda()  # noqa: E731
+    c = Case(m, d, f, experts, 2, True, seed=m)
+    c.x = c.x * 2.0 ** 122
+    c.tx = put(bf(c.x))
+    c.w[1] -= 116
+    c.w1 = c.w1 * 2.0 ** -116
+    assert np.all(np.isfinite(f64(bf(c.x))))
+    c.call()
+    c.check()
+    c = Case(m, d, f, experts, 2, True, seed=m + 20)
+    c.w[1].view(experts, 2 * f, -1)[:, f:] += 120
+    c.w1[:, f:] *= 2.0 ** 120
+    c.w[3] -= 116
+    c.w2 = c.w2 * 2.0 ** -116
+    c.call()
+    c.check()
+
+
 @pytest.mark.parametrize("mx", [False, True])
 @pytest.mark.parametrize("d,f", [(64, 64), (64, 192), (128, 320), (64, 128), (72, 40)])
 def test_nothing_behind_a_row_of_the_second_weights_is_used(skl, d, f, mx):

@@ -164,6 +164,59 @@ def test_far_scales(skl, m):
     assert np.all(np.abs(got - want) <= tolerance("f32", want, np.abs(f64("bf16", b)) @ np.abs(W), k))
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 8, 60, 300])
+@pytest.mark.parametrize("top", [-118, -100, 104, 118, 119, 123, 127])
+def test_large_activations_meet_small_scales(skl, m, top):
+    """Activations up to the largest bf16 numbers whose products with small weights are ordinary numbers, and the reverse; in
+    every other row the activations are ordinary, and some blocks of weights have the smallest scale or none but zero codes."""
+    g = H.rng(abs(top + m))
+    n, k = 37, 520
+    codes, scales = MX.random_packed(g, (n, k), 128 - top, 134 - top) if top < 127 else MX.random_packed(g, (n, k), 1, 6)
+    scales[g.random(scales.shape) < 0.1] = 0
+    codes[3, 32:48] = 0
+    a = g.uniform(0.5, 0.99, (m, k)) * np.where(g.random((m, k)) < 0.5, -1, 1) * 2.0 ** (top + 1)
+    a[:, ::5] *= 2.0 ** -12
+    a[1::2] *= 2.0 ** -top
+    b = bits("bf16", a)
+    assert np.all(np.isfinite(f64("bf16", b)))
+    got = call(skl, "bf16", "f32", False, m, n, k, 1.0, b, k, codes.reshape(-1), 16 * 17, scales.reshape(-1), 17, 0.0,
+               np.zeros(m * n, np.float32), n).reshape(m, n)
+    W = MX.values(codes, scales, k).T
+    want = f64("bf16", b) @ W
+    absum = np.abs(f64("bf16", b)) @ np.abs(W)
+    # every partial sum is at most the sum of the magnitudes: where that is below 2^127 nothing may overflow (the ordinary rows
+    # under scales of 2^118 and more pass the range of 32 bits by their definition and are not compared)
+    inside = absum < 2.0 ** 127
+    assert np.all(inside) or top == -118
+    with np.errstate(invalid="ignore"):
+        err = np.abs(got - want)
+    assert np.all(err[inside] <= tolerance("f32", want, absum, k)[inside])
+
+
+def test_a_block_of_large_and_equal_activations(skl):
+    """One row, 32 activations of 2^123, codes of 6, scale 2^-20: 32 * 6 * 2^103."""
+    got = call(skl, "bf16", "f32", False, 1, 1, 32, 1.0, bits("bf16", np.full(32, 2.0 ** 123)), 32, np.full(16, 0x77, np.uint8), 16,
+               np.full(1, 107, np.uint8), 1, 0.0, np.zeros(1, np.float32), 1)
+    assert got[0] == np.float32(192 * 2.0 ** 103)
+
+
+@pytest.mark.parametrize("m", [1, 3, 8])
+def test_a_sum_past_the_range_is_infinite_and_a_scale_of_255_stays(skl, m):
+    """Large activations again: zero codes under the largest scale stay zero, sums past fp32's range become infinities of
+    their sign, a block of scale 255 makes its column NaN, all in the same blocks of activations."""
+    n, k = 4, 64
+    codes, scales = np.full((n, 32), 0x22, np.uint8), np.full((n, 2), 127 - 110, np.uint8)  # ones times 2^-110
+    codes[1, :16], scales[1, 0] = 0, 252
+    codes[2, :] = 0xAA  # minus ones
+    scales[2] = 200
+    scales[3, 1] = 255
+    b = bits("bf16", np.full((m, k), 2.0 ** 125))
+    got = call(skl, "bf16", "f32", False, m, n, k, 1.0, b, k, codes.reshape(-1), 32, scales.reshape(-1), 2, 0.0,
+               np.zeros(m * n, np.float32), n).reshape(m, n)
+    assert np.all(got[:, 0] == 64 * 2.0 ** 15) and np.all(got[:, 1] == 32 * 2.0 ** 15)
+    assert np.all(got[:, 2] == -np.inf) and np.all(np.isnan(got[:, 3]))
+
+
 @pytest.mark.parametrize("ta", ["bf16", "f16"])
 @pytest.mark.parametrize("m", [2, 8, 24])
 def test_not_finite_values_stay_where_they_are(skl, ta, m):
