@@ -304,7 +304,7 @@ SKL_FUNC void skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k
  * matrices.  On the first two, elements of A far below the largest of their block of 32 lose bits: bf16 elements under
  * 2^-31 of it (first kernel), elements under 2^-29 of it (second kernel), which changes a sum by less than 2^-36 of the
  * block's largest magnitude per element.  In the second kernel a block of A with an infinity or a NaN makes its row NaN, and
- * sums whose magnitudes add up to more than 15/16 of the largest 32-bit float may come out infinite.
+ * sums whose magnitudes add up to more than 7/8 of the largest 32-bit float may come out infinite.
  * Scratch memory for the second and third comes from a pool of the library's own, ordered on the call's stream
  * (cudaMallocFromPoolAsync: captured calls own theirs, so graphs may run side by side). */
 SKL_FUNC void skl_gemm_bf16_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,

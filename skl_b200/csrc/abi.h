@@ -140,6 +140,8 @@ int skl_b200_launch_widen_mxf4(void *dst, int dst_type, int64_t rsd, const void 
 
 /* An fp16 matrix as the exact sum of two bf16 ones: dst rows of 2 * ld elements, [hi | lo], zeros behind column k (ld >= k) */
 int skl_b200_launch_split_f16(void *dst, uint32_t ld, const void *src, int64_t rs, uint32_t m, uint32_t k, void *stream);
+/* 16-bit rows copied to rows of ld elements (a multiple of 8, >= k) at a 16-byte aligned dst, zeros behind column k */
+int skl_b200_launch_align_rows16(void *dst, uint32_t ld, const void *src, int64_t rs, uint32_t m, uint32_t k, void *stream);
 
 /* C = alpha * A W^T + beta * C, A m x k (ta = BF16 / F16, unit column stride), W n x k MX-FP4, for m <= 4 */
 int skl_b200_mxf4_skinny_supported(uint64_t m, uint64_t n, uint64_t k);

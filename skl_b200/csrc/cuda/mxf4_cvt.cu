@@ -457,6 +457,25 @@ __global__ void __launch_bounds__(THREADS)
   }
 }
 
+// Rows of 16-bit elements at any pitch and 2-byte alignment to rows of `ld` elements (a multiple of 8) on 16-byte boundaries, zeros
+// behind column k: what the TMA of the tensor-core kernel asks of an operand.  A thread writes 8 elements at once; its 2-byte
+// loads meet the lines that its neighbours bring to the L1.
+__global__ void __launch_bounds__(THREADS)
+    align_rows_kernel(uint16_t *__restrict__ dst, uint32_t ld, const uint16_t *__restrict__ src, int64_t rs, uint32_t m, uint32_t k) {
+  dep_wait();
+  const uint32_t per_row = ld / 8u;
+  const uint64_t total = (uint64_t)m * per_row, stride = (uint64_t)gridDim.x * THREADS;
+  for (uint64_t i = (uint64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += stride) {
+    const uint32_t row = (uint32_t)(i / per_row), col = (uint32_t)(i - (uint64_t)row * per_row) * 8u;
+    const uint16_t *from = src + (int64_t)row * rs + col;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (col + e < k) w[e >> 1] |= ld_u16(from + e) << (16 * (e & 1));
+    *reinterpret_cast<uint4 *>(dst + (uint64_t)row * ld + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // Launches as a programmatic dependent: the kernel's set-up overlaps the end of the one before it on the stream; every
 // kernel here waits (griddepcontrol.wait) before it touches memory.
 template <typename... P, typename... A>
@@ -551,4 +570,10 @@ extern "C" int skl_b200_launch_split_f16(void *dst, uint32_t ld, const void *src
   uint64_t grid = ceil_div((uint64_t)m * ld, THREADS * 4);
   if (grid > 148 * 32) grid = 148 * 32;
   return (int)launch(split_f16_kernel, grid, (cudaStream_t)stream, (uint16_t *)dst, ld, (const uint16_t *)src, rs, m, k);
+}
+
+extern "C" int skl_b200_launch_align_rows16(void *dst, uint32_t ld, const void *src, int64_t rs, uint32_t m, uint32_t k, void *stream) {
+  uint64_t grid = ceil_div((uint64_t)m * (ld / 8u), THREADS);
+  if (grid > 148 * 64) grid = 148 * 64;
+  return (int)launch(align_rows_kernel, grid, (cudaStream_t)stream, (uint16_t *)dst, ld, (const uint16_t *)src, rs, m, k);
 }

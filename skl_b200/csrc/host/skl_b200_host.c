@@ -1414,12 +1414,14 @@ typedef struct {
 } mxf4_product_t;
 
 /* W widened exactly to bf16 and the product on the 16-bit tensor-core kernel.  fp16 activations become [hi | lo], two bf16
- * matrices side by side, against W twice: every product stays exact.  All pointers are device memory here. */
+ * matrices side by side, against W twice: every product stays exact.  bf16 activations whose rows are not on 16 bytes, which
+ * that kernel's loads need, are copied to rows that are.  All pointers are device memory here. */
 static void mxf4_product_widened(const mxf4_product_t *q) {
   const int split = q->ta == SKL_DT_F16;
+  const int copy = !split && g_ctx.force_path != SKL_B200_PATH_GENERIC && (((uintptr_t)q->a & 15u) || (q->m > 1 && q->rsa % 8));
   const size_t k8 = (q->k + 7) / 8 * 8, n8 = (q->n + 7) / 8 * 8, copies = split ? 2 : 1;
   const size_t kdeep = split ? 2 * k8 : q->k;
-  const size_t wbytes = (q->along_n ? copies * k8 * n8 : q->n * copies * k8) * 2, abytes = split ? q->m * 2 * k8 * 2 : 0;
+  const size_t wbytes = (q->along_n ? copies * k8 * n8 : q->n * copies * k8) * 2, abytes = split ? q->m * 2 * k8 * 2 : (copy ? q->m * k8 * 2 : 0);
   uint8_t *w = (uint8_t *)scratch_get(wbytes + abytes);
   if (!w) return;
   do {
@@ -1441,14 +1443,17 @@ static void mxf4_product_widened(const mxf4_product_t *q) {
     if (split && !cuda_ok((cudaError_t)skl_b200_launch_split_f16(w + wbytes, (uint32_t)k8, q->a, (int64_t)q->rsa,
                                                                  (uint32_t)q->m, (uint32_t)q->k, g_ctx.stream)))
       break;
+    if (copy && !cuda_ok((cudaError_t)skl_b200_launch_align_rows16(w + wbytes, (uint32_t)k8, q->a, (int64_t)q->rsa,
+                                                                   (uint32_t)q->m, (uint32_t)q->k, g_ctx.stream)))
+      break;
     skl_b200_gemm_args g;
     memset(&g, 0, sizeof g);
     g.m0 = q->m; g.n0 = q->n; g.k0 = kdeep;
     g.m1 = g.n1 = g.k1 = 1;
     g.ta = g.tb = SKL_DT_BF16; g.tc = q->tc;
     g.epilogue = SKL_EPI_FLOAT;
-    g.a = split ? w + wbytes : q->a;
-    g.rsa0 = (int64_t)(split ? 2 * k8 : q->rsa); g.csa0 = 1;
+    g.a = split || copy ? w + wbytes : q->a;
+    g.rsa0 = (int64_t)(split ? 2 * k8 : (copy ? k8 : q->rsa)); g.csa0 = 1;
     g.b = w;
     if (q->along_n) { g.rsb0 = (int64_t)n8; g.csb0 = 1; }
     else { g.rsb0 = 1; g.csb0 = (int64_t)(copies * k8); }

@@ -109,6 +109,52 @@ def test_gradient(skl, ta, tc):
         case(skl, ta, tc, True, m, n, k, alpha=(1.0, 0.25)[i % 2], beta=(0.0, 2.0)[i % 2], pad=(0, 5, 8)[i % 3], seed=i)
 
 
+@pytest.mark.parametrize("ta,tc", PAIRS)
+@pytest.mark.parametrize("grad", [False, True])
+def test_activations_on_any_boundary_run_on_the_tensor_cores(skl, ta, tc, grad):
+    """Rows of odd length, rows at odd pitches and bases off 16 bytes, above the batches of the block-scaled kernel (and for the
+    gradient from one row on): the path is the one that the header names."""
+    for i, (m, n, k) in enumerate([(600, 136, 515), (520, 257, 72), (1 if grad else 513, 300, 4099)]):
+        for pad, off in ((0, 0), (5, 0), (8, 1), (2, 7)):
+            case(skl, ta, tc, grad, m, n, k, alpha=(1.0, -0.5)[i % 2], beta=(0.0, 0.5)[i % 2], pad=pad, off=off, seed=i)
+            assert skl.skl_b200_last_path() == S.PATH_TCGEN05, (m, n, k, pad, off)
+    case(skl, ta, tc, grad, 530, 40, 333, where="host")
+    assert skl.skl_b200_last_path() == S.PATH_TCGEN05
+
+
+def test_captured_with_activations_off_16_bytes(skl):
+    """The copy's scratch belongs to the graph, as the widened weights' does; the activations are read at each replay."""
+    import torch
+
+    m, n, k = 300, 64, 259
+    a, b, s, want, tol = tensors(m, n, k, 31)
+    kb, c = -(-k // 32), torch.zeros(m, n, device="cuda")
+    run = lambda: skl.skl_gemm_bf16_mxf4e2m1_f32_sm100a(m, n, k, 1.0, a.data_ptr(), k, b.data_ptr(), 16 * kb, s.data_ptr(), kb,  # noqa: E731
+                                                        0.0, c.data_ptr(), n)
+    run()
+    S.check()
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    skl.skl_b200_set_async(1)
+    try:
+        skl.skl_b200_set_stream(st.cuda_stream)
+        with torch.cuda.graph(graph, stream=st):
+            run()
+            assert skl.skl_b200_last_status() == 0 and skl.skl_b200_last_path() == S.PATH_TCGEN05
+    finally:
+        skl.skl_b200_set_stream(None)
+        skl.skl_b200_set_async(0)
+    old = a.clone()
+    for flip in (0, 1):
+        a.copy_(old)
+        a.view(-1)[1::2] ^= 0x80 * flip  # the sign of every element
+        torch.cuda.synchronize()
+        c.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.all(np.abs(c.cpu().numpy() - (1 - 2 * flip) * want) <= tol)
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_host_operands(skl, grad):
     for m, n, k in ((1, 40, 100), (12, 33, 64)):
