@@ -155,7 +155,8 @@ int skl_b200_mxf4_planes_supported(uint64_t m, uint64_t n, uint64_t k, const voi
 size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t k, int ta);
 int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                 const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
-                                int64_t rsc, void *scratch, uint32_t wait_limit_ms, uint32_t *dev_status, void *stream);
+                                int64_t rsc, void *scratch, uint32_t wait_limit_ms, int debug_skip_loads,
+                                uint32_t *dev_status, void *stream);
 
 /* Mixture-of-experts layer for few tokens (device pointers; see moe.cu).  mx: the weights are MX-FP4 with scales s1 / s2,
  * else bf16.  workspace: skl_b200_moe_scratch_bytes, 4-byte aligned. */

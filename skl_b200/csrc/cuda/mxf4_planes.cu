@@ -62,6 +62,7 @@ struct PlanesParams {
   int tc, c_vec, b_vec, s_vec;
   uint64_t wait_ns;
   uint32_t *status;
+  int skip_loads;  // testing aid: loads are announced, not issued
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -94,6 +95,16 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         return false;
       }
     }
+  }
+}
+// For a warp's own copies in flight: nobody to tell, nothing to give up.  t0: when the first such wait began.
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity, uint64_t &t0, uint64_t limit_ns) {
+  for (uint32_t spins = 0; !bar_try(bar, parity); ++spins) {
+    if ((spins & 63u) != 63u) continue;
+    uint64_t now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (t0 == 0) t0 = now;
+    if (now - t0 > limit_ns) return;
   }
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int x, int y) {
@@ -232,6 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (i >= C::STAGES && !bar_wait(empty + 8 * st, (uint32_t)(i / C::STAGES - 1) & 1u, abort_flag, p.status, ERR_EMPTY, p.wait_ns)) break;
         const uint32_t at = tiles + st * C::STAGE, fb = full + 8 * st, sf = at + PLANES * A_BYTES + B_BYTES;
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"((uint32_t)C::TX) : "memory");
+        if (p.skip_loads) continue;
 #pragma unroll
         for (int q = 0; q < PLANES; ++q) {
           const int row_tile = q * p.plane_tiles + mi;
@@ -239,10 +251,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           bulk(sf + q * SF_BYTES, p.sfa + ((int64_t)row_tile * p.stages + s) * SF_BYTES, SF_BYTES, fb);
         }
       }
-      // the copies of the last stages land before the memory is used for anything else, also when a wait has run out
-      for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
-        for (uint32_t spins = 0; spins < (1u << 20) && !bar_try(full + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u); ++spins) {
-        }
+      // the copies of the last stages land before the memory is used for anything else; after a wait has run out their barriers miss
+      // the loaders' arrivals, and one limit for all of them is long past the time that a copy takes
+      uint64_t t0 = 0;
+      for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued && !p.skip_loads; ++i)
+        bar_drain(full + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, t0, p.wait_ns);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -574,7 +587,8 @@ extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t k, int ta) {
 
 extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                            const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
-                                           int64_t rsc, void *scratch, uint32_t wait_limit_ms, uint32_t *dev_status, void *stream) {
+                                           int64_t rsc, void *scratch, uint32_t wait_limit_ms, int debug_skip_loads,
+                                           uint32_t *dev_status, void *stream) {
   EncodeFn enc = encoder();
   if (!enc) return (int)cudaErrorNotSupported;
   const Layout l = layout(m, k, ta);
@@ -620,7 +634,7 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
   p.alpha = alpha, p.beta = beta, p.tc = tc;
   p.c_vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0 && (m == 1 || rsc * es % 16 == 0);
   p.wait_ns = (uint64_t)(wait_limit_ms ? wait_limit_ms : 2000u) * 1000000ull;
-  p.status = dev_status;
+  p.status = dev_status, p.skip_loads = debug_skip_loads;
   switch (l.tiles) {
     case 1: return (int)launch_product<1>(tma, p, s);
     case 2: return (int)launch_product<2>(tma, p, s);

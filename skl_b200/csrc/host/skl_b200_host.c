@@ -1520,7 +1520,7 @@ static void run_mxf4_product(mxf4_product_t *q) {
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_planes((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
                                                            q->beta, q->c, q->tc, (int64_t)q->rsc, scratch,
-                                                           g_ctx.wait_limit_ms, st, g_ctx.stream));
+                                                           g_ctx.wait_limit_ms, g_ctx.debug_skip_loads, st, g_ctx.stream));
     scratch_put(scratch);
   } else {
     g_ctx.static_weights = 0; /* the widened copy is written by this call */

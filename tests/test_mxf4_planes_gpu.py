@@ -107,3 +107,32 @@ def test_same_bits_every_time(skl):
     for _ in range(3):
         again, _ = run(skl, "bf16", "f32", m, n, k, 1.0, 0.0, 0, g, a, codes, scales)
         assert np.array_equal(first.view(np.uint32), again.view(np.uint32))
+
+
+@pytest.mark.parametrize("ta,m", [("bf16", 8), ("bf16", 60), ("bf16", 130), ("f16", 100)])
+def test_expired_wait_is_reported_and_the_context_survives(skl, ta, m):
+    """One, two, three and four tiles to a stage: the loads are announced and not issued, the waits run out after 5 ms, the call says
+    so in time, and the next call is right."""
+    import time
+
+    n, k = 700, 4096
+    g = H.rng(m)
+    codes, _ = MX.random_packed(g, (n, k))
+    scales = np.full((n, k // 32), 127, np.uint8)
+    a = g.integers(-8, 9, (m, k)).astype(np.float64)
+    args = (skl, ta, "f32", False, m, n, k, 1.0, bits(ta, a), k, codes.reshape(-1), k // 2, scales.reshape(-1), k // 32, 0.0,
+            np.zeros(m * n, np.float32), n)
+    want = (a @ MX.values(codes, scales, k).T).astype(np.float32)
+    assert np.array_equal(call(*args).reshape(m, n), want)
+    skl.skl_b200_set_wait_limit(5)
+    skl.skl_b200_debug_skip_loads(1)
+    try:
+        t0 = time.perf_counter()
+        with pytest.raises(S.SklB200Error, match="stage code 0x40[123]"):
+            call(*args)
+        assert time.perf_counter() - t0 < 1.0, "the give-up path must not take longer than a few wait limits"
+        assert skl.skl_b200_last_status() == 4 and skl.skl_b200_last_path() == S.PATH_TCGEN05
+    finally:
+        skl.skl_b200_debug_skip_loads(0)
+        skl.skl_b200_set_wait_limit(0)
+    assert np.array_equal(call(*args).reshape(m, n), want)
