@@ -800,10 +800,10 @@ cudaError_t launch(unsigned grid, size_t smem, cudaStream_t s, const MoeParams &
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (!ready[dev & 63]) {
+  if (!__atomic_load_n(&ready[dev & 63], __ATOMIC_ACQUIRE)) {  // threads that meet here do the same
     e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MAX_SMEM);
     if (e != cudaSuccess) return e;
-    ready[dev & 63] = true;
+    __atomic_store_n(&ready[dev & 63], true, __ATOMIC_RELEASE);
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

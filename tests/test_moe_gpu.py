@@ -6,6 +6,8 @@ k-deep fp32 sum): the first products are off by gamma(d) |W1||x| (and 2^-38 of a
 second product with 11 significant bits of its own or, below 2^-17 of its block's largest, 2^-39 of that (4-bit weights), or
 with 16 bits (two bf16 values); the second sums add gamma(f + topk); gates are off by 2^-20 of themselves; the result is
 rounded to bf16, 2^-8 of the value."""
+import os
+
 import numpy as np
 import pytest
 
@@ -356,6 +358,47 @@ def test_captured_side_by_side_and_on_other_streams(skl, mx):
     finally:
         skl.skl_b200_set_stream(None)
         skl.skl_b200_set_async(0)
+
+
+def test_two_threads_at_once(skl):
+    """Both kinds of weights from two threads that start together in a new process, each on a stream and a workspace of its own."""
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+import test_moe_gpu as T
+torch.zeros(1, device="cuda")
+jobs = [[T.Case(3 + t, 128 * (t + 1), 192, 6, 2, mx, seed=t) for mx in (False, True)] for t in range(2)]
+torch.cuda.synchronize()
+gate, failed = threading.Barrier(2), []
+def work(t):
+    try:
+        torch.cuda.set_device(0)
+        lib, stream = T.S.lib(), torch.cuda.Stream()
+        lib.skl_b200_set_stream(stream.cuda_stream)
+        lib.skl_b200_set_async(1)
+        gate.wait()
+        for _ in range(20):
+            for c in jobs[t]:
+                c.call()
+        lib.skl_b200_synchronize()
+        assert lib.skl_b200_last_status() == 0
+    except BaseException as e:
+        failed.append(repr(e))
+threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not failed, failed
+for cases in jobs:
+    for c in cases:
+        c.check()
+print("fine")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here), os.environ.get("PYTHONPATH", "")]))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
 
 
 def test_from_the_router_on(skl):
