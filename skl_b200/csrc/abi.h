@@ -150,13 +150,14 @@ int skl_b200_launch_mxf4_skinny(uint32_t m, uint32_t n, uint32_t k, float alpha,
                                 int64_t rsc, int static_b, void *stream);
 
 /* The same product on the block-scaled tensor-core instruction, A as three (bf16) or four (fp16) E5M2 planes: packed rows
- * on 8 bytes.  scratch: skl_b200_mxf4_planes_scratch bytes, 256-byte aligned. */
+ * on 8 bytes.  scratch: skl_b200_mxf4_planes_scratch bytes, 256-byte aligned.  before_product: NULL, or an event recorded
+ * between the kernel that writes the planes and the product's. */
 int skl_b200_mxf4_planes_supported(uint64_t m, uint64_t n, uint64_t k, const void *b, int64_t csb);
 size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t k, int ta);
 int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                 const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
                                 int64_t rsc, void *scratch, uint32_t wait_limit_ms, int debug_skip_loads,
-                                uint32_t *dev_status, void *stream);
+                                uint32_t *dev_status, void *before_product, void *stream);
 
 /* Mixture-of-experts layer for few tokens (device pointers; see moe.cu).  mx: the weights are MX-FP4 with scales s1 / s2,
  * else bf16.  workspace: skl_b200_moe_scratch_bytes, 4-byte aligned. */

@@ -588,7 +588,7 @@ extern "C" size_t skl_b200_mxf4_planes_scratch(uint64_t m, uint64_t k, int ta) {
 extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, float alpha, const void *a, int ta, int64_t rsa,
                                            const void *b, int64_t csb, const void *sb, int64_t cssb, float beta, void *c, int tc,
                                            int64_t rsc, void *scratch, uint32_t wait_limit_ms, int debug_skip_loads,
-                                           uint32_t *dev_status, void *stream) {
+                                           uint32_t *dev_status, void *before_product, void *stream) {
   EncodeFn enc = encoder();
   if (!enc) return (int)cudaErrorNotSupported;
   const Layout l = layout(m, k, ta);
@@ -635,6 +635,7 @@ extern "C" int skl_b200_launch_mxf4_planes(uint32_t m, uint32_t n, uint32_t k, f
   p.c_vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0 && (m == 1 || rsc * es % 16 == 0);
   p.wait_ns = (uint64_t)(wait_limit_ms ? wait_limit_ms : 2000u) * 1000000ull;
   p.status = dev_status, p.skip_loads = debug_skip_loads;
+  if (before_product) (void)cudaEventRecord((cudaEvent_t)before_product, s);
   switch (l.tiles) {
     case 1: return (int)launch_product<1>(tma, p, s);
     case 2: return (int)launch_product<2>(tma, p, s);

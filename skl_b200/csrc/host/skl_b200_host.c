@@ -468,6 +468,19 @@ static int widen_fp8_operand(skl_b200_gemm_args *g) {
   return 1;
 }
 
+/* The events around a call's main kernel while skl_b200_profile_begin's calls last; NULL otherwise. */
+static cudaEvent_t prof_event(int end) {
+  return g_ctx.prof_ev && g_ctx.prof_used < g_ctx.prof_cap ? g_ctx.prof_ev[2 * g_ctx.prof_used + end] : 0;
+}
+static void prof_begin(void) {
+  if (prof_event(0)) (void)cudaEventRecord(prof_event(0), (cudaStream_t)g_ctx.stream);
+}
+static void prof_end(void) {
+  if (!prof_event(1)) return;
+  (void)cudaEventRecord(prof_event(1), (cudaStream_t)g_ctx.stream);
+  g_ctx.prof_used++;
+}
+
 /* Chooses the kernel family for a device-resident problem and enqueues it on the library stream. */
 /* Does the epilogue read C's previous contents (so that a host C has to be copied in first)? */
 static int reads_old_c(const skl_b200_gemm_args *g) {
@@ -520,8 +533,7 @@ static int dispatch_launch(const skl_b200_gemm_args *gin) {
     }
   }
   int rc = 0;
-  const int prof = g_ctx.prof_ev && g_ctx.prof_used < g_ctx.prof_cap;
-  if (prof) (void)cudaEventRecord(g_ctx.prof_ev[2 * g_ctx.prof_used], (cudaStream_t)g_ctx.stream);
+  prof_begin();
   if (path == SKL_B200_PATH_GEMV) {
     uint32_t *st = device_status_words();
     if (!st) return 0;
@@ -533,10 +545,7 @@ static int dispatch_launch(const skl_b200_gemm_args *gin) {
   } else {
     rc = skl_b200_launch_gemm_generic(g, g_ctx.stream);
   }
-  if (prof) {
-    (void)cudaEventRecord(g_ctx.prof_ev[2 * g_ctx.prof_used + 1], (cudaStream_t)g_ctx.stream);
-    g_ctx.prof_used++;
-  }
+  prof_end();
   g_ctx.last_path = (skl_b200_path_t)path;
   return cuda_ok((cudaError_t)rc);
 }
@@ -1508,9 +1517,11 @@ static void run_mxf4_product(mxf4_product_t *q) {
     run_gemm_body(&g);
   } else if (!q->along_n && g_ctx.force_path == 0 && skl_b200_mxf4_skinny_supported(q->m, q->n, q->k)) {
     g_ctx.last_path = SKL_B200_PATH_GEMV;
+    prof_begin();
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_skinny((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
                                                            q->beta, q->c, q->tc, (int64_t)q->rsc, static_b, g_ctx.stream));
+    prof_end();
   } else if (!q->along_n && q->m <= (q->ta == SKL_DT_BF16 ? MXF4_PLANES_MAX_BF16 : MXF4_PLANES_MAX_F16) && g_ctx.force_path != SKL_B200_PATH_GENERIC &&
              skl_b200_mxf4_planes_supported(q->m, q->n, q->k, q->b, (int64_t)q->rsb)) {
     uint32_t *st = device_status_words();
@@ -1520,7 +1531,8 @@ static void run_mxf4_product(mxf4_product_t *q) {
     (void)cuda_ok((cudaError_t)skl_b200_launch_mxf4_planes((uint32_t)q->m, (uint32_t)q->n, (uint32_t)q->k, q->alpha, q->a, q->ta,
                                                            (int64_t)q->rsa, q->b, (int64_t)q->rsb, q->sb, (int64_t)q->rss,
                                                            q->beta, q->c, q->tc, (int64_t)q->rsc, scratch,
-                                                           g_ctx.wait_limit_ms, g_ctx.debug_skip_loads, st, g_ctx.stream));
+                                                           g_ctx.wait_limit_ms, g_ctx.debug_skip_loads, st, prof_event(0), g_ctx.stream));
+    prof_end();
     scratch_put(scratch);
   } else {
     g_ctx.static_weights = 0; /* the widened copy is written by this call */

@@ -460,6 +460,28 @@ def test_offsets_past_32_bits(skl, m, ta, grad):
     assert np.array_equal(got, (a @ (W if grad else W.T)).astype(np.float32))
 
 
+@pytest.mark.parametrize("m,grad", [(1, False), (4, False), (30, False), (300, False), (2, True)])
+def test_profiled_calls_are_counted_and_timed(skl, m, grad):
+    """skl_b200_profile_begin / _end around the products of every path: as many records as calls, no more than were asked for."""
+    import ctypes
+
+    import torch
+
+    n, k = 2048, 1024
+    a, b, s, want, tol = tensors(m, n, k, m, grad)
+    kb, c = -(-(n if grad else k) // 32), torch.zeros(m, n, device="cuda")
+    fn = skl.skl_gemm_bf16_mxf4e2m1r_f32_sm100a if grad else skl.skl_gemm_bf16_mxf4e2m1_f32_sm100a
+    for asked, calls in ((3, 3), (2, 4)):
+        skl.skl_b200_profile_begin(asked)
+        for _ in range(calls):
+            fn(m, n, k, 1.0, a.data_ptr(), k, b.data_ptr(), 16 * kb, s.data_ptr(), kb, 0.0, c.data_ptr(), n)
+            S.check()
+        ms = ctypes.c_double(0.0)
+        assert skl.skl_b200_profile_end(ctypes.byref(ms)) == min(asked, calls)
+        assert 0.0 < ms.value < 100.0
+    assert np.all(np.abs(c.cpu().numpy() - want) <= tol)
+
+
 def test_two_threads_at_once(skl):
     """Every path from two threads, each on a stream of its own; the calls share the library's pool of scratch memory."""
     import threading
