@@ -360,6 +360,85 @@ def test_captured_side_by_side_and_on_other_streams(skl, mx):
         skl.skl_b200_set_async(0)
 
 
+@pytest.mark.parametrize("mx", [False, True])
+def test_values_that_are_not_finite_stay_with_their_tokens(skl, mx):
+    """An infinity and a NaN in two tokens' activations, a NaN in a weight of an expert that some tokens have: every other token's
+    result is what it is without them."""
+    import torch
+
+    m, d, f, experts, topk = 9, 192, 160, 6, 2
+    logits = H.rng(77).standard_normal((m, experts)).astype(np.float32)
+    logits[:, 5] = -9.0
+    logits[3, 5] = 9.0  # only this token has expert 5
+    c = Case(m, d, f, experts, topk, mx, logits=logits, seed=77)
+    c.call()
+    torch.cuda.synchronize()
+    plain = c.y.clone()
+    x = bf(c.x)
+    x[1, 40], x[6, 191] = 0x7F80, 0x7FC0
+    c.tx = torch.from_numpy(x.view(np.uint8).reshape(-1)).cuda()
+    if mx:
+        c.w[1].view(experts, 2 * f, -1)[5, f + 7, 3] = 255  # an element of h
+        c.w[3].view(experts, d, -1)[5, 11, 0] = 255  # and a row of the result
+    else:
+        c.w[0].view(torch.int16).view(experts, 2 * f, d)[5, f + 7, 100] = 0x7FC0
+        c.w[1].view(torch.int16).view(experts, d, f)[5, 11, 3] = 0x7FC0
+    c.out()
+    c.call()
+    torch.cuda.synchronize()
+    fine = [i for i in range(m) if i not in (1, 3, 6)]
+    assert torch.equal(c.y[fine], plain[fine])
+    assert not torch.any(torch.isfinite(c.y[1])) and torch.all(torch.isnan(c.y[[3, 6]]))
+
+
+@pytest.mark.parametrize("byte", [0, 1, 245, 252])
+def test_scales_at_the_ends_of_their_range(skl, byte):
+    """4-bit weights whose gate rows and down rows have the smallest or the largest scales; the activations make up for them."""
+    import torch
+
+    m, d, f, experts = 3, 96, 64, 2
+    c = Case(m, d, f, experts, 2, True, seed=byte)
+    c.x = c.x * 2.0 ** (100 if byte < 118 else -100)
+    c.tx = torch.from_numpy(bf(c.x).view(np.uint8).reshape(-1)).cuda()
+    c.w[1].fill_(byte)
+    c.w[1].view(experts, 2 * f, -1)[:, f:] = 120
+    c.w[3].fill_(byte)
+    rows = lambda v, n: v.cpu().numpy().reshape(experts, n, -1)  # noqa: E731
+    c.w1, c.w2 = MX.values(rows(c.w[0], 2 * f), rows(c.w[1], 2 * f), d), MX.values(rows(c.w[2], d), rows(c.w[3], d), f)
+    with np.errstate(over="ignore"):
+        c.call()
+        c.check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_weights_past_32_bits(skl, mx):
+    """1024 experts whose last one lies more than 4 GiB behind the first in both matrices; nothing else of them is used."""
+    import torch
+
+    d, f, experts = (4096, 4096, 1024) if mx else (2048, 2048, 1024)
+    logits = np.full((2, experts), -np.inf, np.float32)
+    logits[:, -1] = 0.5
+    small = Case(2, d, f, 1, 1, mx, logits=logits[:, -1:], seed=5)
+    c = object.__new__(Case)
+    c.__dict__.update(small.__dict__)
+    c.shape, c.logits, c.rsl = (2, d, f, experts, 1), logits, experts
+    c.tl = torch.from_numpy(logits.view(np.uint8).reshape(-1)).cuda()
+    c.w = []
+    for w in small.w:
+        big = torch.empty(w.numel() * experts, dtype=torch.uint8, device="cuda")
+        big[-w.numel():] = w
+        c.w.append(big)
+    assert min(w.numel() - w.numel() // experts for w in c.w[::2 if mx else 1]) > 1 << 32
+    c.out()
+    c.call()
+    torch.cuda.synchronize()
+    want, tol = layer(small.x, small.w1, small.w2, np.zeros((2, 1), int), np.ones((2, 1)), np.ones((2, 1), bool), mx)
+    tol = tol + 2.0 ** -8 * (np.abs(want) + tol) + 2.0 ** -130
+    assert torch.all(c.ids == experts - 1) and torch.all(c.gates == 1.0)
+    got = f64(c.y.view(torch.int16).cpu().numpy().view(np.uint16))
+    assert np.all(np.abs(got - want) <= tol)
+
+
 def test_two_threads_at_once(skl):
     """Both kinds of weights from two threads that start together in a new process, each on a stream and a workspace of its own."""
     import subprocess
