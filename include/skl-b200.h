@@ -302,8 +302,8 @@ SKL_FUNC void skl_gemm_mxf4e2m1_mxf4e2m1_f32_sm100a(size_t m, size_t n, size_t k
  * packed rows on 8-byte boundaries, on the block-scaled tensor-core instruction; everything else, and the gradient, widens
  * W exactly to bf16 and runs on the 16-bit tensor-core kernel, where fp16 activations enter as the exact sum of two bf16
  * matrices.  On the first two, elements of A far below the largest of their block of 32 lose bits: bf16 elements under
- * 2^-31 of it (first kernel), elements under 2^-29 of it (second kernel), which changes a sum by less than 2^-36 of the
- * block's largest magnitude per element.  In the second kernel a block of A with an infinity or a NaN makes its row NaN, and
+ * 2^-31 of it and, where the largest is 2^15 or more, fp16 elements under 2^-13 (first kernel), elements under 2^-29 of it
+ * (second kernel), which changes a sum by less than 2^-36 of the block's largest magnitude per element.  In the second kernel a block of A with an infinity or a NaN makes its row NaN, and
  * sums whose magnitudes add up to more than 7/8 of the largest 32-bit float may come out infinite.
  * Scratch memory for the second and third comes from a pool of the library's own, ordered on the call's stream
  * (cudaMallocFromPoolAsync: captured calls own theirs, so graphs may run side by side). */
@@ -343,8 +343,10 @@ SKL_FUNC void skl_gemm_f16_mxf4e2m1r_f16_sm100a(size_t m, size_t n, size_t k, fl
  * takes packed rows as skl_cvt_<t>rc_mxf4e2m1 writes them with dense strides (16 ceil(d / 32) code bytes and ceil(d / 32)
  * scale bytes to a row of w1 / s1, the same with f for w2 / s2).
  * A chosen expert whose logit is minus infinity is masked: gate 0, its weights are not used; a token whose logits are all
- * minus infinity gets zeros.  Sums are fp32, h is kept in fp32 and enters the second product with at least 11 significant
- * bits, y is rounded once.
+ * minus infinity gets zeros.  Sums are fp32, y is rounded once.  Between the products h is kept in fp32 and enters the second
+ * one as the sum of two bf16 values (16 significant bits) with 16-bit weights; with 4-bit weights it is kept as fp16 with a
+ * power of two per block of 32: 11 significant bits, and elements off by up to 2^-39 of their block's largest magnitude where
+ * that is more.
  * 1 <= topk <= 32, experts <= 1024, m <= 64, d and f from 1 to 32768; larger calls are refused (SKL_B200_ERR_UNSUPPORTED).
  * All pointers are device memory.  `workspace`: skl_b200_moe_workspace_size bytes of the caller's, 4-byte aligned,
  * not initialised, one for each call or captured graph that may run at the same time; ids and gates are dense

@@ -3,7 +3,7 @@
 // Such a kernel may run before its predecessor on the stream has finished and waits for it with griddepcontrol.wait.  A
 // load that the compiler knows to be invariant (__ldg, a const __restrict__ pointer) could be moved above that wait, so
 // these are volatile: they stay where they are written, behind the wait.  None of these kernels lets its successor start early
-// (griddepcontrol.launch_dependents): with a grid far larger than the chip in front of a kernel of clusters that hung the chip.
+// (griddepcontrol.launch_dependents): with a grid far larger than the chip in front of a kernel of clusters such a call did not return.
 #pragma once
 
 #include <cstdint>

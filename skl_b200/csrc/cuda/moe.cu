@@ -15,13 +15,15 @@
 //          piece of f) items in turn, each adding gate * product to sums of its own, which are added in order at the end.
 // Columns of the mma hold the tokens of an expert, at most 4 at a time.  16-bit weights: mma.sync bf16; x enters as it is, h as
 // the sum of two bf16 values in two columns (16 significant bits, so that h is not rounded to 8).  4-bit weights:
-// mxf4_mma.cuh; h is kept as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result), which
-// every CTA of `down` can copy as it is: converting fp32 there took as many instructions as the products.
+// mxf4_mma.cuh; h is kept as fp16 with a power of two per block of 32 (11 significant bits, against 8 of the result; elements
+// below 2^-28 of their block's largest have fewer), which every CTA of `down` can copy as it is: converting fp32 there took as
+// many instructions as the products.  Against h in fp32 a tenth of the results differ in their last bit, 8.6e-4 in the 2-norm,
+// half of bf16's own rounding (1.65e-3 either way against 64 bits).
 //
-// d 2048, f 1024, 8 of 64 experts: one token, bf16 weights (100 MB), 25.2 us in a graph: the routing (about 5 us), two streams at
-// 6.6 TB/s, each with its start and end; MX-FP4 17.3.  16 tokens, MX-FP4 (187 MB): 72 us, 51 of them `up`; bound by the issue
-// slots (half busy) and the latency of dependent instructions, about 400 instructions of a warp for 16 x 256 weights.
-// 16 tokens, bf16: 145 us, 4.8 TB/s.
+// d 2048, f 1024, 8 of 64 experts, in a graph over three sets of weights: one token, bf16 weights (100 MB), 28.5 us: the routing
+// (about 5 us) and two streams, each with its start and end; MX-FP4 17.0.  16 tokens, MX-FP4 (187 MB): 74 us, two thirds of them
+// `up`; bound by the issue slots (half busy) and the latency of dependent instructions, about 400 instructions of a warp for
+// 16 x 256 weights.  16 tokens, bf16: 145 us, 4.8 TB/s.
 #include "mxf4_mma.cuh"
 
 namespace sklb {

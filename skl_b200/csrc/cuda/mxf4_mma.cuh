@@ -13,10 +13,10 @@
 // on the whole chip, against 12 T that HBM delivers (17/32 byte per element at 6.4 TB/s); placing the bits of bf16 with
 // integer instructions reached 12 T.
 //
-// fp16 activations are used as they are.  bf16 activations are brought into fp16's range with one power of two per block of
-// 32 that puts the block's largest magnitude into [2^14, 2^15): a bf16 value has 8 significant bits, so every value down to
-// 2^-31 of the block's largest stays exact, smaller ones are rounded to a multiple of 2^-38 of it -- far under the rounding
-// of the fp32 sums.
+// Activations are brought into fp16's range with one power of two per block of 32 that puts the block's largest magnitude into
+// [2^14, 2^15).  A bf16 value has 8 significant bits, so every value down to 2^-31 of the block's largest stays exact, smaller
+// ones are rounded to a multiple of 2^-38 of it -- far under the rounding of the fp32 sums.  fp16 values stay exact, but for
+// those under 2^-13 in a block whose largest is 2^15 or more, which is halved: they are rounded to a multiple of 2^-23.
 #pragma once
 
 #include <cstdint>

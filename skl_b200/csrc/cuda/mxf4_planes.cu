@@ -20,8 +20,8 @@
 // accumulator, the cluster adds its parts through distributed shared memory in a fixed order, and every CTA stores a share of
 // the rows.  Every wait is bounded.
 //
-// 14336 x 4096, both kernels, in a graph: 5 rows 20.2 us, 32 rows 22.3, 61 rows 27.1, 128 rows 32.6 (31 MB: 4.9 us of HBM; W
-// widened to bf16 and multiplied: 59 us); 4096 x 4096 with 5 rows 12.8, 1024 x 1024 9.0, which is what the two launches, filling
+// 14336 x 4096, both kernels, in a graph: 5 rows 19.9 us, 32 rows 22.3, 61 rows 26.7, 128 rows 31.8 (31 MB: 4.9 us of HBM; W
+// widened to bf16 and multiplied: 64 rows 50 us); 4096 x 4096 with 5 rows 12.8, 1024 x 1024 9.0, which is what the two launches, filling
 // and emptying cost.  Beyond that a stage takes about 0.7 us: the hand-over from the loaders to the MMAs, not HBM.
 #include <cuda.h>
 
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t da = operand_desc(at + q * A_BYTES);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            // E5M2 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; N = 256, M = 128
+            // E5M2 x E2M1 with E8M0 scales, byte j of the scales' 4-byte columns; M = 128, N = p.bn
             const uint32_t idesc = (uint32_t)j << 4 | 1u << 7 | 5u << 10 | (uint32_t)(p.bn >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 |
                                    (uint32_t)j << 29;
             const uint32_t accumulate = (i | q | j) != 0;

@@ -5,8 +5,8 @@
 // their steps of 16 rows x 256 elements through rings in shared memory (mxf4_mma.cuh).  The partial sums of the warps meet
 // in shared memory once, at the end, and are added in a fixed order, so results do not change from run to run.
 //
-// 14336 x 4096, in a graph: 1 or 2 rows 9.1 us, 3 or 4 rows 11.6 (31 MB: 4.9 us of HBM; about 2 us pass until the first weights
-// arrive, the rest is the stream and the join); 4096 x 14336 11.2 and 16.0; 4096 x 4096 4.5 and 6.0; 1024 x 1024 2.7 and 3.2.
+// 14336 x 4096, in a graph: 1 or 2 rows 8.9 us, 3 or 4 rows 11.7 (31 MB: 4.9 us of HBM; about 2 us pass until the first weights
+// arrive, the rest is the stream and the join); 4096 x 14336 (fp16) 11.2 and 15.4; 4096 x 4096 4.5 and 6.0; 1024 x 1024 2.7 and 3.2.
 // Plain loads into registers instead of the rings: 18.0 us for the first.
 #include "mxf4_mma.cuh"
 
@@ -26,7 +26,7 @@ struct SkinnyParams {
   uint32_t m, n, k, kblocks, steps;
   uint32_t cta_rows, k_warps;  // rows of a CTA; warps that split k (a power of two)
   float alpha, beta;
-  int ta, tc, a_vec;
+  int tc, a_vec;
   int static_b;
 };
 
@@ -185,7 +185,7 @@ extern "C" int skl_b200_launch_mxf4_skinny(uint32_t m, uint32_t n, uint32_t k, f
   p.a = a, p.b = (const uint8_t *)b, p.sb = (const uint8_t *)sb, p.c = c;
   p.rsa = rsa, p.csb = csb, p.cssb = cssb, p.rsc = rsc;
   p.m = m, p.n = n, p.k = k, p.kblocks = (k + 31) / 32;
-  p.alpha = alpha, p.beta = beta, p.ta = ta, p.tc = tc, p.static_b = static_b;
+  p.alpha = alpha, p.beta = beta, p.tc = tc, p.static_b = static_b;
   p.a_vec = (reinterpret_cast<uintptr_t>(a) & 15u) == 0 && (m == 1 || rsa % 8 == 0);
   const bool vec = (reinterpret_cast<uintptr_t>(b) & 15u) == 0 && (n == 1 || csb % 16 == 0);
   const bool svec = (reinterpret_cast<uintptr_t>(sb) & 7u) == 0 && (n == 1 || cssb % 8 == 0);

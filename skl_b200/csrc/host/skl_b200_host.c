@@ -1408,8 +1408,18 @@ static void scratch_trim(void) {
 }
 
 /* Rows up to which 16-bit x MX-FP4 products run on the block-scaled tensor-core kernel, whose work grows with the planes that
- * A is cut into; above it widening W once pays.  Measured on 14336 x 4096: bf16 256 rows 51 us against 91, 512 rows 140
- * against 93; fp16 (four planes, and two products of the widened kind) 512 rows 167 us against 180, 1024 about even. */
+ * A is cut into and with tiles of 128 rows; above it widening W once pays.  Planes / widened in us, in a graph, for n x k =
+ * 14336 x 4096, 4096 x 14336, 4096 x 4096, 1024 x 1024:
+ *   bf16  128 rows  32 / 51   37 / 86   18 / 28    9.9 / 10.6
+ *         256       51 / 60   52 / 87   24 / 28   12.3 / 10.8
+ *         257       85 / 82   76 / 91   32 / 30   12.6 / 10.8
+ *         512      137 / 82  101 / 96   37 / 31   12.8 / 10.8
+ *   fp16  (four planes, and two products of the widened kind)
+ *         512 rows 170 / 165 129 / 214  45 / 64   14.0 / 19.5
+ *         640      149 / 183 177 / 244  59 / 72   17.4 / 20.1
+ *        1024      277 / 287 252 / 293  79 / 88   20.0 / 21.3
+ * so that bf16 crosses at the third tile of rows; fp16 crosses beyond 1024 rows (3 to 40 % are left there: the limit was set by
+ * the first of these matrices alone). */
 #define MXF4_PLANES_MAX_BF16 256
 #define MXF4_PLANES_MAX_F16 512
 
