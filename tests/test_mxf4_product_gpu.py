@@ -308,6 +308,30 @@ def tensors(m, n, k, seed, grad=False):
     return [torch.from_numpy(v.view(np.uint8).copy()).cuda() for v in (a, codes, scales)] + [want, tolerance("f32", want, absum, k)]
 
 
+@pytest.mark.parametrize("ta", ["bf16", "f16"])
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 992), (1100, 5000, 1515)])
+def test_several_rounds_of_tiles(skl, ta, grad, m, n, k):
+    """Widened products with more tiles than the chip takes at once, on pairs of SMs where the shape allows; compared on the GPU."""
+    import torch
+
+    g = H.rng(m + n)
+    rows, length = (k, n) if grad else (n, k)
+    kb = -(-length // 32)
+    codes, scales = MX.random_packed(g, (rows, length), 112, 122)
+    a = bits(ta, g.standard_normal((m, k)) * np.exp2(g.integers(-4, 4, (m, 1))))
+    A, B, SC = (torch.from_numpy(np.ascontiguousarray(v).view(np.uint8)).cuda() for v in (a, codes, scales))
+    c = torch.zeros(m, n, device="cuda")
+    fn = getattr(skl, f"skl_gemm_{ta}_mxf4e2m1{'r' if grad else ''}_f32_sm100a")
+    fn(m, n, k, 1.0, A.data_ptr(), k, B.data_ptr(), 16 * kb, SC.data_ptr(), kb, 0.0, c.data_ptr(), n)
+    S.check()
+    assert skl.skl_b200_last_path() == S.PATH_TCGEN05
+    x, W = torch.from_numpy(f64(ta, a)).cuda(), torch.from_numpy(MX.values(codes, scales, length)).cuda()
+    W = W if grad else W.T
+    absum = x.abs() @ W.abs()
+    assert torch.all((c.double() - x @ W).abs() <= tolerance("f32", 0.0, absum, k))
+
+
 @pytest.mark.parametrize("m", [1, 40])
 def test_two_graphs_side_by_side(skl, m):
     """Two captured products, replayed together on two streams, then after a larger call has come and gone."""
